@@ -109,6 +109,42 @@ int sj_rope(void *stream, const void *x, void *y, int dtype, long rows, long ld,
  * sj_attention_bwd. */
 int sj_rope_table(void *stream, float *table, long t, long head_dim, float theta);
 
+/* Rotary positions in the forms that decoding and long contexts need (no
+ * counterpart in the reference, whose rope counts rows and rotates whole
+ * heads).  A table of frequencies is made once and kept: turns [rotary_dim /
+ * 2], entry i the fraction of a turn that pair i makes per position, in 64-bit
+ * fixed point (2^64 = one turn).  f_i = theta^(-2i / rotary_dim), scaled by
+ * kind: NONE; LINEAR f / factor; BASE theta' = theta factor^(d / (d - 2)), d =
+ * rotary_dim; PARTS f (g + (1 - g) / factor) with g = (context f / 2 pi -
+ * slow_turns) / (fast_turns - slow_turns) clamped to 0 .. 1 (pairs that turn
+ * often within the original context keep their frequency, slow ones are
+ * interpolated).  Formed in double.  rotary_dim even, at most 1024. */
+#define SJ_ROPE_SCALE_NONE 0
+#define SJ_ROPE_SCALE_LINEAR 1
+#define SJ_ROPE_SCALE_BASE 2
+#define SJ_ROPE_SCALE_PARTS 3
+typedef struct {
+  float theta;
+  int kind;
+  float factor, context, fast_turns, slow_turns;
+} sj_rope_scaling;
+int sj_rope_frequencies(void *stream, uint64_t *turns, long rotary_dim, const sj_rope_scaling *scaling);
+/* y [rows][ldy] = x [rows][ldx] with the first rotary_dim columns of each
+ * head rotated by the row's position (any int32; negative turns back), the
+ * rest of the head copied; columns past heads * head_dim are neither read nor
+ * written.  Pairs: INTERLEAVED (2i, 2i + 1), as sj_rope; HALF (i, i +
+ * rotary_dim / 2).  (a, b) -> amplitude (a cos - b sin, a sin + b cos);
+ * inverse != 0 negates the sine: the gradient of the forward call.  The angle
+ * is good to 2^-22 up to position 2^27.  x and y fp32 or bf16 (stored value in, fp32
+ * products, one rounding); y may be x.  head_dim even, at most 1024; any
+ * strides and element alignment (16-byte rows are fastest).  turns may be
+ * null when rotary_dim is 0. */
+#define SJ_ROPE_INTERLEAVED 0
+#define SJ_ROPE_HALF 1
+int sj_rope_rows(void *stream, const void *x, long ldx, void *y, long ldy, int dtype, long rows, long heads,
+                 long head_dim, long rotary_dim, int layout, const int32_t *positions, const uint64_t *turns,
+                 float amplitude, int inverse);
+
 /* Engine::swiglu / swiglu_backward, lib.rs:700-733 (kernels.py:90-101). */
 int sj_swiglu_fwd(void *stream, const void *g, const void *u, void *h, int dtype, long n);
 int sj_swiglu_bwd(void *stream, const void *g, const void *u, int gu_dtype,
@@ -333,6 +369,68 @@ int sj_attention_bwd_p(void *stream, const uint16_t *q, long ldq, const uint16_t
                        long head_dim, const float *rope_table, uint16_t *g_hi, uint16_t *g_lo, long ldg,
                        uint16_t *g_t_hi, uint16_t *g_t_lo, long ldgt, void *workspace, size_t workspace_bytes);
 size_t sj_attention_bwd_p_workspace_bytes(long batch, long t, long hq, long hk, long head_dim);
+
+/* -------------------------------------------------- Paged key-value cache
+ * Decoding many sequences at once (no counterpart in the reference, whose
+ * cache holds one sequence: model lib.rs:36-50).  The cache is a pool of
+ * `pages` pages of page_size slots; a slot is one row of k_cache and v_cache
+ * [pages * page_size][ldkv] (hk heads of head_dim), the layout of
+ * sj_attention_fwd_cached's cache.  Request r's position p lies in slot
+ * table[r][p / page_size] * page_size + p % page_size; table [requests][ldt]
+ * (ldt entries a row, also its stride).  A step is: sj_paged_plan, then per
+ * layer the QKV product, sj_paged_append, sj_paged_attention.  pages *
+ * page_size and ldt * page_size are at most 2^31 - 1; byte offsets are 64-bit.
+ *
+ * The plan of a step, on the device (one launch, no host synchronisation, no
+ * workspace): request r holds lengths[r] tokens and gets counts[r] more (0
+ * allowed).  The pages it grows into are taken from free_pages [free_count],
+ * from position free_head[0] (device; null: 0) on, in the order of the
+ * requests, and written to its table row; the entries it has stay.  Token j of
+ * request r is row starts[r] + j (starts [requests + 1], exclusive sums):
+ * positions, slots and owners (the request) [capacity]; rows behind the last
+ * token get -1 in all three, which the calls below skip.  A token whose page
+ * id is not in 0 .. pages - 1 gets slot -1.  lengths_after (nullable) =
+ * lengths + counts.  summary [4] = tokens, the free list's position after the
+ * step, status bits (0: good), the longest length after the step.  With any
+ * status bit the step is void: every row is -1, starts are 0, and the table,
+ * the free list's position and the lengths stay.  lengths_after may not be
+ * lengths or counts, nor free_head summary + 1 (a captured loop alternates two
+ * of each).  Calls on one table must not overlap. */
+#define SJ_PLAN_NO_PAGES 1    /* the free list is too short */
+#define SJ_PLAN_TABLE_WIDTH 2 /* a request outgrows its table row */
+#define SJ_PLAN_ROWS 4        /* more tokens than capacity */
+#define SJ_PLAN_LENGTHS 8     /* a negative length or count, or a length past 2^31 - 1 */
+int sj_paged_plan(void *stream, const int32_t *lengths, const int32_t *counts, long requests, long page_size,
+                  long pages, int32_t *table, long ldt, const int32_t *free_pages, long free_count,
+                  const int32_t *free_head, int32_t *lengths_after, int32_t *starts, int32_t *positions,
+                  int32_t *slots, int32_t *owners, long capacity, int32_t *summary);
+/* The step's queries rotated (q [rows][ldq] -> q_out [rows][ldqo]) and its
+ * keys rotated and values copied into the cache rows of their slots; the
+ * rotation as sj_rope_rows.  A row whose slot is not in 0 .. cache_slots - 1
+ * is left out whole (q_out too).  The slots of one call are distinct.  q_out
+ * may be q; hq may be 0.  Any strides and element alignment. */
+int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, int dtype,
+                    long rows, long hq, long hk, long head_dim, long rotary_dim, int layout, const int32_t *positions,
+                    const int32_t *slots, const uint64_t *turns, float amplitude, void *q_out, long ldqo,
+                    void *k_cache, void *v_cache, long ldkv, long cache_slots);
+/* Grouped attention of the step's tokens over the pages: query row i (of
+ * request owners[i]; owners null: request i) at position positions[i] sees its
+ * request's keys 0 .. positions[i], with window > 0 the `window` last of them;
+ * scale head_dim^-1/2.  Several rows may belong to one request (drafted
+ * tokens, chunks of a prompt).  o [rows][ldo] in the q dtype, lse (nullable)
+ * fp32 [rows][hq] natural log of the sum of exp(score).  Keys whose page id is
+ * not in 0 .. pages - 1, and scores of -inf, have no share; a row without any
+ * key gives o = 0 and lse = -inf; rows with position or owner below 0 (or an
+ * owner past the requests) are left as they were.  Slots past a request's
+ * length are never read into a result, whatever they hold.  head_dim at most
+ * 256, any strides and alignment.  Workspace:
+ * sj_paged_attention_workspace_bytes, not cleared and not kept; calls that
+ * share one must not overlap. */
+size_t sj_paged_attention_workspace_bytes(long rows, long hq, long hk, long head_dim);
+int sj_paged_attention(void *stream, const void *q, long ldq, const void *k_cache, const void *v_cache, long ldkv,
+                       int dtype, long pages, long page_size, const int32_t *table, long ldt, long requests,
+                       const int32_t *owners, const int32_t *positions, long rows, long hq, long hk, long head_dim,
+                       long window, void *o, long ldo, float *lse, void *workspace, size_t workspace_bytes);
 
 /* ------------------------------------------- Hierarchical model patches
  * The byte <-> patch maps of the hierarchical (cfg3) model (hidden_from_
@@ -621,6 +719,31 @@ int sj_sum_f64(void *stream, const double *x, long n, double *out);
 int sj_cross_entropy(void *stream, const float *x, long ldx, const int32_t *targets,
                      float *loss, float *dx, long lddx, long rows, long vocab,
                      const float *dy, float dy_scalar);
+/* Log probabilities of given tokens (no counterpart in the reference, whose
+ * cross entropy gives the loss alone).  Per row of logits x [rows][ldx] (fp32
+ * or bf16): logprob = ln softmax(x)[tokens[r]], 0 where the token is not in 0
+ * .. vocab - 1; entropy = -sum p ln p; stats [rows][2] = (max x, ln sum
+ * e^(x - max)), what the backward needs; the `top` largest entries, the lowest
+ * index first among equals, top_ids and their log probabilities top_logprob
+ * [rows][top].  logprob (then tokens too), entropy and stats are nullable.
+ * Entries of -inf have no share; a row of nothing else has entropy 0, log
+ * probabilities -inf and stats (0, 0).  A NaN makes its row's numbers NaN and
+ * is ranked behind everything.  top at most SJ_LOGPROBS_MAX_TOP and vocab.
+ * Any stride and element alignment.  Workspace:
+ * sj_token_logprobs_workspace_bytes, not cleared and not kept. */
+#define SJ_LOGPROBS_MAX_TOP 64
+size_t sj_token_logprobs_workspace_bytes(long rows, long vocab, long top);
+int sj_token_logprobs(void *stream, const void *x, int dtype, long ldx, long rows, long vocab, const int32_t *tokens,
+                      long top, float *logprob, float *entropy, float *stats, int32_t *top_ids, float *top_logprob,
+                      void *workspace, size_t workspace_bytes);
+/* Its gradient: dx [rows][lddx] (fp32 or bf16) = dlogprob[r] (1[v = token] -
+ * p_v) - dentropy[r] p_v (ln p_v + entropy[r]), written, not accumulated.
+ * dlogprob (then tokens too) and dentropy (then entropy too) are nullable; a
+ * token outside the vocabulary has no share through dlogprob.  stats and
+ * entropy as the forward left them. */
+int sj_token_logprobs_bwd(void *stream, const void *x, int dtype, long ldx, long rows, long vocab,
+                          const int32_t *tokens, const float *stats, const float *entropy, const float *dlogprob,
+                          const float *dentropy, void *dx, int dx_dtype, long lddx);
 /* Engine::gather, lib.rs:1010-1028 (kernel gather, kernels.py:241-245):
  * y [rows][d] = x[idx[r]] (row stride ldx) in y's dtype (a gather followed
  * by Graph::cast to F32 when yd = SJ_F32). */

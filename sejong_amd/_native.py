@@ -12,6 +12,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsejong_hip.so")
 
 SJ_F32, SJ_F64, SJ_F16, SJ_I32, SJ_BF16 = 0, 1, 2, 3, 4
+SJ_ROPE_INTERLEAVED, SJ_ROPE_HALF = 0, 1
+SJ_ROPE_SCALE_NONE, SJ_ROPE_SCALE_LINEAR, SJ_ROPE_SCALE_BASE, SJ_ROPE_SCALE_PARTS = 0, 1, 2, 3
+SJ_PLAN_NO_PAGES, SJ_PLAN_TABLE_WIDTH, SJ_PLAN_ROWS, SJ_PLAN_LENGTHS = 1, 2, 4, 8
+SJ_LOGPROBS_MAX_TOP = 64
 
 _P = ctypes.c_void_p
 _L = ctypes.c_long
@@ -72,6 +76,12 @@ class AdamStep(ctypes.Structure):
                 ("clip_enabled", ctypes.c_int32)]
 
 
+class RopeScaling(ctypes.Structure):
+    """sj_rope_scaling of include/sejong_hip.h."""
+    _fields_ = [("theta", _F), ("kind", _I), ("factor", _F), ("context", _F), ("fast_turns", _F),
+                ("slow_turns", _F)]
+
+
 # name -> (restype, argtypes); int-returning functions are status-checked
 SIGNATURES = {
     "sj_status_string": (ctypes.c_char_p, [_I]),
@@ -95,6 +105,17 @@ SIGNATURES = {
     "sj_embedding_bwd": (_I, [_P, _P, _P, _P, _L, _L, _L, _P, _S]),
     "sj_rope": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _F, _I]),
     "sj_rope_table": (_I, [_P, _P, _L, _L, _F]),
+    "sj_rope_frequencies": (_I, [_P, _P, _L, ctypes.POINTER(RopeScaling)]),
+    "sj_rope_rows": (_I, [_P, _P, _L, _P, _L, _I, _L, _L, _L, _L, _I, _P, _P, _F, _I]),
+    "sj_paged_plan": (_I, [_P, _P, _P, _L, _L, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "sj_paged_append": (_I, [_P, _P, _L, _P, _L, _P, _L, _I, _L, _L, _L, _L, _L, _I, _P, _P, _P, _F, _P, _L, _P, _P,
+                             _L, _L]),
+    "sj_paged_attention_workspace_bytes": (_S, [_L, _L, _L, _L]),
+    "sj_paged_attention": (_I, [_P, _P, _L, _P, _P, _L, _I, _L, _L, _P, _L, _L, _P, _P, _L, _L, _L, _L, _L, _P, _L,
+                                _P, _P, _S]),
+    "sj_token_logprobs_workspace_bytes": (_S, [_L, _L, _L]),
+    "sj_token_logprobs": (_I, [_P, _P, _I, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _P, _S]),
+    "sj_token_logprobs_bwd": (_I, [_P, _P, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P, _I, _L]),
     "sj_swiglu_fwd": (_I, [_P, _P, _P, _P, _I, _L]),
     "sj_swiglu_bwd": (_I, [_P, _P, _P, _I, _P, _P, _P, _L]),
     "sj_rmsnorm_fwd": (_I, [_P, _P, _I, _P, _I, _P, _L, _L, _F]),

@@ -1,0 +1,279 @@
+// Rotary positions at given positions (no counterpart in the reference, whose
+// rope, kernels.py:103-113, counts rows and rotates whole heads): interleaved
+// or half layout, the first rotary_dim columns of each head, frequencies
+// scaled for long contexts; and the same fused with the write of a step's keys
+// and values into the slots of a paged cache.
+//
+//   (a, b) -> A (a cos t - b sin t, a sin t + b cos t),  t = position * f_i
+//
+// A frequency is held as the fraction of a turn it makes per position, in
+// 64-bit fixed point: position * turns modulo 2^64 is the angle's fraction of
+// a turn with no further rounding (in fp32 the angle of position 2^20 is
+// already 0.06 off), for one integer multiply instead of a double multiply and
+// its range reduction.  A workgroup forms the cosines and sines
+// of its rows once in LDS (one pair per thread and turn), then all the heads
+// of those rows read them: the bound is the read and the write of the rows.
+#include <math.h>
+
+#include "common.h"
+
+using namespace sj;
+
+namespace {
+
+constexpr int RT = 256;
+constexpr int RPAIRS = 512;  // at most this many (row, pair) angles of a workgroup in LDS
+
+// one frequency per thread, in double
+__global__ void k_rope_frequencies(uint64_t* turns, int half, sj_rope_scaling s) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= half) return;
+  const double d = 2.0 * half;
+  double lt = log((double)s.theta);
+  if (s.kind == SJ_ROPE_SCALE_BASE && half > 1) lt += log((double)s.factor) * d / (d - 2.0);
+  double f = exp(-2.0 * i / d * lt);
+  const double tau = 6.283185307179586476925286766559;
+  if (s.kind == SJ_ROPE_SCALE_LINEAR) f /= (double)s.factor;
+  if (s.kind == SJ_ROPE_SCALE_PARTS) {
+    const double n = (double)s.context * f / tau;
+    double g = (n - (double)s.slow_turns) / ((double)s.fast_turns - (double)s.slow_turns);
+    g = g < 0.0 ? 0.0 : g > 1.0 ? 1.0 : g;
+    f = f * (g + (1.0 - g) / (double)s.factor);
+  }
+  double t = f / tau;
+  t -= floor(t);
+  turns[i] = (uint64_t)(t * 18446744073709551616.0);
+}
+
+// where a group of heads of a row comes from and goes to
+struct RopeSeg {
+  const void* x;
+  long ldx;
+  void* y;
+  long ldy;
+  int heads;   // heads of this segment
+  int rotate;  // 0: copied
+  int slots;   // the destination row is the row's slot, not the row
+};
+
+struct RopeArgs {
+  RopeSeg seg[3];
+  int nseg;
+  long rows;
+  int heads;  // of all segments
+  int D, half, layout;
+  const int32_t* positions;
+  const int32_t* slots;  // null: every row counts
+  long nslots;
+  const uint64_t* turns;
+  float amplitude, sign;
+  int rb;  // rows of a workgroup
+};
+
+// EL elements of T as they lie (element-aligned: the hardware takes
+// global vectors at any element alignment)
+template <typename T, int EL>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+  T v[EL];
+};
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(bf16_t v) { return bf2f(v); }
+__device__ __forceinline__ void from_f(float v, float& o) { o = v; }
+__device__ __forceinline__ void from_f(float v, bf16_t& o) { o = f2bf(v); }
+
+// EL: elements of a unit.  Interleaved: a unit is EL / 2 pairs, or EL copied
+// columns.  Half: a unit is EL first and EL second elements of pairs, or EL
+// copied columns.  The rounding is sj_rope's: stored values in, fp32 products,
+// one rounding to the storage type.
+template <typename T, int EL, bool HALF>
+__global__ __launch_bounds__(RT) void k_rope_rows(RopeArgs a) {
+  __shared__ float2 cs[RPAIRS];
+  const int t = threadIdx.x, half = a.half, D = a.D;
+  const int rot_units = HALF ? half / EL : 2 * half / EL;
+  const int units = rot_units + (D - 2 * half) / EL;
+  // blocks of rows, and within them blocks of pairs where a head has more
+  // than LDS holds (rb is 1 then, and half <= RPAIRS is checked on the host)
+  const long r0 = (long)blockIdx.x * a.rb;
+  const int nr = (int)(a.rows - r0 < a.rb ? a.rows - r0 : a.rb);
+  for (int i = t; i < nr * half; i += RT) {
+    const int r = i / half, p = i - r * half;
+    const uint64_t ph = (uint64_t)(int64_t)a.positions[r0 + r] * a.turns[p];
+    float s, c;
+    sincospif((float)(int32_t)(ph >> 32) * 4.656612873077393e-10f, &s, &c);  // half turns: 2^-31
+    cs[i] = make_float2(c * a.amplitude, s * a.amplitude * a.sign);
+  }
+  __syncthreads();
+  const int per_row = a.heads * units;
+  for (int i = t + (int)blockIdx.y * RT; i < nr * per_row; i += RT * (int)gridDim.y) {
+    const int r = i / per_row, hu = i - r * per_row;
+    int h = hu / units;
+    const int u = hu - h * units;
+    const long row = r0 + r;
+    long dst = row;
+    if (a.slots) {
+      const int sl = a.slots[row];
+      if (sl < 0 || sl >= a.nslots) continue;  // a padded row: nothing of it is written
+      dst = sl;
+    }
+    RopeSeg sg = a.seg[0];
+    if (a.nseg > 1) {  // q | k | v
+      if (h >= a.seg[0].heads) {
+        h -= a.seg[0].heads;
+        sg = a.seg[1];
+        if (h >= sg.heads) h -= sg.heads, sg = a.seg[2];
+      }
+      if (!sg.slots) dst = row;
+    }
+    const T* x = (const T*)sg.x + row * sg.ldx + (long)h * D;
+    T* y = (T*)sg.y + dst * sg.ldy + (long)h * D;
+    typedef Pack<T, EL> P;
+    const float2* c = cs + r * half;
+    if (u >= rot_units || !sg.rotate) {
+      if (HALF && u < rot_units) {
+        const P lo = *(const P*)(x + u * EL), hi = *(const P*)(x + half + u * EL);
+        *(P*)(y + u * EL) = lo;
+        *(P*)(y + half + u * EL) = hi;
+      } else {
+        const int o = HALF ? 2 * half + (u - rot_units) * EL : u * EL;
+        *(P*)(y + o) = *(const P*)(x + o);
+      }
+    } else if constexpr (HALF) {
+      P lo = *(const P*)(x + u * EL), hi = *(const P*)(x + half + u * EL);
+#pragma unroll
+      for (int e = 0; e < EL; e++) {
+        const float va = to_f(lo.v[e]), vb = to_f(hi.v[e]);
+        const float2 q = c[u * EL + e];
+        from_f(va * q.x - vb * q.y, lo.v[e]);
+        from_f(va * q.y + vb * q.x, hi.v[e]);
+      }
+      *(P*)(y + u * EL) = lo;
+      *(P*)(y + half + u * EL) = hi;
+    } else {
+      P v = *(const P*)(x + u * EL);
+#pragma unroll
+      for (int e = 0; e < EL / 2; e++) {
+        const float va = to_f(v.v[2 * e]), vb = to_f(v.v[2 * e + 1]);
+        const float2 q = c[u * (EL / 2) + e];
+        from_f(va * q.x - vb * q.y, v.v[2 * e]);
+        from_f(va * q.y + vb * q.x, v.v[2 * e + 1]);
+      }
+      *(P*)(y + u * EL) = v;
+    }
+  }
+}
+
+template <typename T, int EL>
+void launch_el(hipStream_t s, const RopeArgs& a, dim3 grid) {
+  if (a.layout == SJ_ROPE_HALF)
+    k_rope_rows<T, EL, true><<<grid, RT, 0, s>>>(a);
+  else if constexpr (EL > 1)
+    k_rope_rows<T, EL, false><<<grid, RT, 0, s>>>(a);
+}
+
+int launch(hipStream_t s, RopeArgs& a, int dtype) {
+  const int width = dtype == SJ_BF16 ? 8 : 4;
+  int el = width;  // the widest unit that divides the head, its rotated part and (half layout) each half
+  const int part = a.layout == SJ_ROPE_HALF ? a.half : 2 * a.half;
+  while (el > 1 && (a.D % el || part % el)) el >>= 1;
+  a.rb = a.half < RPAIRS ? (a.half ? RPAIRS / a.half : 8) : 1;
+  if (a.rb > 8) a.rb = 8;
+  // few rows: fewer of them to a workgroup, down to one, so that they reach more CUs
+  while (a.rb > 1 && (a.rows + a.rb - 1) / a.rb < 512) a.rb >>= 1;
+  const dim3 grid((unsigned)((a.rows + a.rb - 1) / a.rb), 1);
+  if (dtype == SJ_BF16) {
+    if (el == 8) launch_el<bf16_t, 8>(s, a, grid);
+    else if (el == 4) launch_el<bf16_t, 4>(s, a, grid);
+    else if (el == 2) launch_el<bf16_t, 2>(s, a, grid);
+    else launch_el<bf16_t, 1>(s, a, grid);
+  } else {
+    if (el == 4) launch_el<float, 4>(s, a, grid);
+    else if (el == 2) launch_el<float, 2>(s, a, grid);
+    else launch_el<float, 1>(s, a, grid);
+  }
+  SJ_LAUNCH_CHECK("rope rows");
+  return SJ_OK;
+}
+
+bool head_ok(long head_dim, long rotary_dim, int layout) {
+  return head_dim > 0 && head_dim % 2 == 0 && head_dim <= 1024 && rotary_dim >= 0 && rotary_dim % 2 == 0 &&
+         rotary_dim <= head_dim && (layout == SJ_ROPE_INTERLEAVED || layout == SJ_ROPE_HALF);
+}
+
+}  // namespace
+
+extern "C" int sj_rope_frequencies(void* stream, uint64_t* turns, long rotary_dim, const sj_rope_scaling* scaling) {
+  SJ_REQUIRE(turns && scaling && rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= 1024,
+             "rope frequencies: rotary width %ld", rotary_dim);
+  const sj_rope_scaling s = *scaling;
+  SJ_REQUIRE(s.kind >= SJ_ROPE_SCALE_NONE && s.kind <= SJ_ROPE_SCALE_PARTS, "rope frequencies: scaling kind %d", s.kind);
+  SJ_REQUIRE(isfinite(s.theta) && s.theta > 0.f && (s.kind == SJ_ROPE_SCALE_NONE || (isfinite(s.factor) && s.factor > 0.f)),
+             "rope frequencies: theta %g, factor %g", (double)s.theta, (double)s.factor);
+  SJ_REQUIRE(s.kind != SJ_ROPE_SCALE_PARTS || (isfinite(s.context) && s.context > 0.f && isfinite(s.fast_turns) &&
+                                               isfinite(s.slow_turns) && s.fast_turns > s.slow_turns),
+             "rope frequencies: original context %g, turns %g .. %g", (double)s.context, (double)s.slow_turns,
+             (double)s.fast_turns);
+  const int half = (int)(rotary_dim / 2);
+  k_rope_frequencies<<<(half + 63) / 64, 64, 0, (hipStream_t)stream>>>(turns, half, s);
+  SJ_LAUNCH_CHECK("rope frequencies");
+  return SJ_OK;
+}
+
+extern "C" int sj_rope_rows(void* stream, const void* x, long ldx, void* y, long ldy, int dtype, long rows, long heads,
+                            long head_dim, long rotary_dim, int layout, const int32_t* positions,
+                            const uint64_t* turns, float amplitude, int inverse) {
+  SJ_REQUIRE(dtype == SJ_F32 || dtype == SJ_BF16, "rope rows dtype %d", dtype);
+  SJ_REQUIRE(head_ok(head_dim, rotary_dim, layout), "rope rows: head width %ld, rotary width %ld, layout %d", head_dim,
+             rotary_dim, layout);
+  SJ_REQUIRE(rows >= 0 && heads > 0 && heads <= 65536 && ldx >= heads * head_dim && ldy >= heads * head_dim,
+             "rope rows dimensions");
+  if (rows == 0) return SJ_OK;
+  SJ_REQUIRE(x && y && positions && (turns || rotary_dim == 0), "rope rows: null");
+  SJ_REQUIRE(rows <= 0x7fffffffL, "rope rows: %ld rows", rows);
+  RopeArgs a = {};
+  a.seg[0] = RopeSeg{x, ldx, y, ldy, (int)heads, 1, 0};
+  a.nseg = 1;
+  a.rows = rows;
+  a.heads = (int)heads;
+  a.D = (int)head_dim;
+  a.half = (int)(rotary_dim / 2);
+  a.layout = layout;
+  a.positions = positions;
+  a.turns = turns;
+  a.amplitude = amplitude;
+  a.sign = inverse ? -1.f : 1.f;
+  return launch((hipStream_t)stream, a, dtype);
+}
+
+extern "C" int sj_paged_append(void* stream, const void* q, long ldq, const void* k, long ldk, const void* v, long ldv,
+                               int dtype, long rows, long hq, long hk, long head_dim, long rotary_dim, int layout,
+                               const int32_t* positions, const int32_t* slots, const uint64_t* turns, float amplitude,
+                               void* q_out, long ldqo, void* k_cache, void* v_cache, long ldkv, long cache_slots) {
+  SJ_REQUIRE(dtype == SJ_F32 || dtype == SJ_BF16, "paged append dtype %d", dtype);
+  SJ_REQUIRE(head_ok(head_dim, rotary_dim, layout), "paged append: head width %ld, rotary width %ld, layout %d",
+             head_dim, rotary_dim, layout);
+  SJ_REQUIRE(rows >= 0 && hq >= 0 && hk > 0 && hq <= 65536 && hk <= 65536 && ldq >= hq * head_dim &&
+                 ldqo >= hq * head_dim && ldk >= hk * head_dim && ldv >= hk * head_dim && ldkv >= hk * head_dim &&
+                 cache_slots >= 0,
+             "paged append dimensions");
+  if (rows == 0) return SJ_OK;
+  SJ_REQUIRE(k && v && positions && slots && (turns || rotary_dim == 0) && k_cache && v_cache && (hq == 0 || (q && q_out)),
+             "paged append: null");
+  SJ_REQUIRE(rows <= 0x7fffffffL, "paged append: %ld rows", rows);
+  RopeArgs a = {};
+  a.seg[0] = RopeSeg{q, ldq, q_out, ldqo, (int)hq, 1, 0};
+  a.seg[1] = RopeSeg{k, ldk, k_cache, ldkv, (int)hk, 1, 1};
+  a.seg[2] = RopeSeg{v, ldv, v_cache, ldkv, (int)hk, 0, 1};
+  a.nseg = 3;
+  a.rows = rows;
+  a.heads = (int)(hq + 2 * hk);
+  a.D = (int)head_dim;
+  a.half = (int)(rotary_dim / 2);
+  a.layout = layout;
+  a.positions = positions;
+  a.slots = slots;
+  a.nslots = cache_slots;
+  a.turns = turns;
+  a.amplitude = amplitude;
+  a.sign = 1.f;
+  return launch((hipStream_t)stream, a, dtype);
+}

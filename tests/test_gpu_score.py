@@ -1,0 +1,267 @@
+"""sj_token_logprobs and its gradient against the 64-bit definitions.
+
+Tolerances: a term e^(x - m) is off by its argument's rounding, 2^-24 |x - m|,
+and expf's 2^-23; a sum of V of them in fp32, over threads and then a tree, by
+at most (V / 64 + 32) 2^-24 of itself."""
+import numpy as np
+import pytest
+
+from tests import gpu_util as G
+from tests import paged_util as PU
+from tests import score_util as U
+
+pytestmark = pytest.mark.gpu
+ULP = 2.0 ** -24
+
+
+def native():
+    from sejong_amd import _native as N
+    return N, N.load()
+
+
+CODE = {"f32": 0, "bf16": 4}
+
+
+class Score:
+    """One call's buffers, each with guard values behind it."""
+
+    def __init__(self, x, dtype, tokens, top, ld=None, offset=0):
+        N, lib = native()
+        self.n, self.V, self.top, self.dtype = x.shape[0], x.shape[1], top, dtype
+        self.ld = ld or self.V
+        wide = np.full((self.n, self.ld), 777.0)  # columns past the vocabulary are never read
+        wide[:, :self.V] = x
+        flat = np.concatenate([np.zeros(offset), wide.ravel()])
+        self.off = offset
+        self.x = G.dev(flat, dtype)
+        self.tokens = PU.ints(tokens)
+        self.lp, self.ent, self.stats = (G.dev(np.full(k * self.n + 4, 55.0)) for k in (1, 1, 2))
+        self.ids = PU.ints(np.full(self.n * top + 4, 99))
+        self.alt = G.dev(np.full(self.n * top + 4, 55.0))
+        self.ws = G.empty(max(lib.sj_token_logprobs_workspace_bytes(self.n, self.V, top), 16), "u8")
+
+    def forward(self, stream=None):
+        native()[0].api.sj_token_logprobs(stream, self.x.at(self.off), CODE[self.dtype], self.ld, self.n, self.V,
+                                          self.tokens.p, self.top, self.lp.p, self.ent.p, self.stats.p, self.ids.p,
+                                          self.alt.p, self.ws.p, self.ws.nbytes)
+
+    def host(self):
+        out = [b.host() for b in (self.lp, self.ent, self.stats, self.ids, self.alt)]
+        assert all((b[-4:] == (99 if b.dtype == np.int32 else 55.0)).all() for b in out)  # nothing behind the rows
+        lp, ent, stats, ids, alt = (b[:-4] for b in out)
+        return dict(lp=lp, ent=ent, stats=stats.reshape(-1, 2), ids=ids.reshape(self.n, -1), alt=alt.reshape(self.n, -1))
+
+    def backward(self, dlp, dent, dx_dtype, lddx=None, stream=None):
+        lddx = lddx or self.V
+        dx = G.dev(np.full(self.n * lddx + 4, 55.0), dx_dtype)
+        a = G.dev(dlp) if dlp is not None else None
+        b = G.dev(dent) if dent is not None else None
+        native()[0].api.sj_token_logprobs_bwd(stream, self.x.at(self.off), CODE[self.dtype], self.ld, self.n, self.V,
+                                              self.tokens.p, self.stats.p, self.ent.p, a and a.p, b and b.p, dx.p,
+                                              CODE[dx_dtype], lddx)
+        h = dx.host()
+        assert (h[-4:] == 55.0).all()
+        h = h[:-4].reshape(self.n, lddx)
+        assert (h[:, self.V:] == 55.0).all()  # columns past the vocabulary are left
+        return h[:, :self.V]
+
+
+def check_forward(got, x, tokens, top):
+    want = U.scores(x, tokens, top)
+    V = x.shape[1]
+    np.testing.assert_array_equal(got["ids"], want["ids"])
+    with np.errstate(invalid="ignore"):
+        spread = np.abs(x - want["ref"][:, None])
+        e_lp = np.where(np.isfinite(want["lp"]), ULP * (8 + 2 * spread + (V / 64 + 32)), 0.0)
+    row = ULP * (16 + V / 64 + 32) * (1 + want["ll"])
+    tok = np.where(want["ok"], e_lp[np.arange(len(x)), want["at"]], 0.0)
+    for name, g, w, tol in (("logprob", got["lp"], want["logprob"], tok),
+                            ("alternatives", got["alt"], want["alt"], np.take_along_axis(e_lp, want["ids"], 1)),
+                            ("max", got["stats"][:, 0], want["ref"], 0.0), ("log sum", got["stats"][:, 1], want["ll"], row)):
+        same = (g == w)  # infinities among them
+        with np.errstate(invalid="ignore"):
+            assert (same | (np.abs(g - w) <= tol)).all(), (name, np.nanmax(np.abs(g - w) - tol))
+    with np.errstate(invalid="ignore"):
+        mean = np.where(want["p"] > 0, want["p"] * spread, 0.0).sum(1)
+        part = np.where(want["p"] > 0, want["p"] * spread * spread, 0.0).sum(1)
+    tol = row * (1 + mean) + ULP * part + 8 * ULP * (want["ll"] + mean)
+    assert (np.abs(got["ent"] - want["entropy"]) <= tol).all(), np.max(np.abs(got["ent"] - want["entropy"]) - tol)
+    return want
+
+
+def check_backward(dx, x, tokens, dlp, dent, dtype):
+    want, s = U.gradient(x, tokens, dlp, dent), U.scores(x, tokens)
+    V = x.shape[1]
+    with np.errstate(invalid="ignore"):
+        e = ULP * (40 + V / 64 + 2 * np.abs(x - s["ref"][:, None]) + 2 * s["ll"][:, None])
+        a = np.abs(dlp)[:, None] if dlp is not None else 0.0
+        b = np.abs(dent)[:, None] if dent is not None else 0.0
+        lpH = np.where(s["p"] > 0, np.abs(s["lp"]) + s["entropy"][:, None], 0.0)
+        tol = np.where(s["p"] > 0, s["p"] * e * (a + b * (1 + lpH)) + s["p"] * b * ULP * (V / 64 + 64) * (2 + lpH), 0.0)
+    tol = tol + np.abs(want) * (2.0 ** -8 if dtype == "bf16" else 4 * ULP) + 1e-37
+    assert (np.abs(dx - want) <= tol).all(), np.max(np.abs(dx - want) / tol)
+
+
+def logits(rng, n, V, dtype, spread=2.0):
+    x = rng.normal(0, spread, (n, V))
+    x[np.arange(n), rng.integers(0, V, n)] += rng.random(n) * 15
+    return G.O.round_to(x, dtype)
+
+
+@pytest.mark.parametrize("n,V,top,dtype,ld,offset", [
+    (1, 1, 1, "f32", 0, 0), (3, 2, 2, "bf16", 0, 0), (5, 63, 5, "f32", 64, 1), (70, 257, 5, "f32", 264, 0),
+    (33, 257, 20, "bf16", 257, 3), (9, 1000, 64, "f32", 1001, 0), (7, 4099, 8, "bf16", 0, 1), (4, 8193, 32, "f32", 8200, 2),
+    (3, 32768, 20, "bf16", 0, 0), (2, 50001, 1, "bf16", 50008, 0), (2, 131072, 64, "f32", 0, 0), (17, 5000, 0, "f32", 0, 0),
+    (1, 200001, 33, "f32", 0, 1), (600, 300, 3, "bf16", 301, 0), (1030, 16, 4, "f32", 0, 0)])
+def test_scores_and_gradient(n, V, top, dtype, ld, offset):
+    rng = np.random.default_rng(V + n)
+    x = logits(rng, n, V, dtype)
+    tokens = rng.integers(0, V, n)
+    tokens[::3] = x.argmax(1)[::3]
+    tokens[1::7] = -1
+    tokens[2::7] = V
+    s = Score(x, dtype, tokens, top, ld or None, offset)
+    s.forward()
+    got = s.host()
+    check_forward(got, x, tokens, top)
+    dlp, dent = rng.normal(size=n).astype(np.float32), rng.normal(size=n).astype(np.float32)
+    for a, b, d in ((dlp, dent, dtype), (dlp, None, "f32"), (None, dent, "bf16")):
+        check_backward(s.backward(a, b, d, V + (3 if d == "f32" else 0)), x, tokens, a, b, d)
+    s.forward()  # the same again: equal bits
+    again = s.host()
+    assert all((again[k] == got[k]).all() for k in got)
+
+
+@pytest.mark.parametrize("V", [5, 64, 257, 1000, 9000, 40000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_equal_and_ordered_rows(V, dtype):
+    """Ties go to the lowest index; rows sorted either way, constant rows, rows of two values."""
+    i = np.arange(V)
+    x = np.stack([np.zeros(V), i // 3 * 0.5, (V - i) // 4 * 0.25, i % 2, np.where(i < V // 2, 1.0, -1.0), -(i % 7) * 1.0,
+                  np.where(i == V - 1, -0.0, 0.0)])
+    x = G.O.round_to(np.clip(x, -60, 60), dtype)
+    tokens = np.arange(len(x)) % V
+    top = min(V, 48)
+    s = Score(x, dtype, tokens, top)
+    s.forward()
+    check_forward(s.host(), x, tokens, top)
+
+
+@pytest.mark.parametrize("V", [6, 257, 5000, 33000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_masked_vocabularies(V, dtype):
+    """Entries of -inf and of the type's lowest value, rows that hold little or nothing else."""
+    rng = np.random.default_rng(V)
+    low = float(G.O.round_to(np.array([-3.38e38]), dtype)[0])
+    x = logits(rng, 6, V, dtype)
+    x[0, ::2] = -np.inf
+    x[1] = -np.inf
+    x[2] = -np.inf
+    x[2, V - 2] = 3.0
+    x[3, 1:] = low
+    x[4] = low
+    x[5, 2:] = -np.inf
+    tokens = np.array([1, 0, V - 2, 0, V - 1, 0])
+    s = Score(x, dtype, tokens, 5)
+    s.forward()
+    check_forward(s.host(), x, tokens, 5)
+    dlp, dent = np.ones(6, np.float32), np.ones(6, np.float32)
+    dx = s.backward(dlp, dent, "f32")
+    keep = [0, 2, 3, 4, 5]
+    check_backward(dx[keep], x[keep], tokens[keep], dlp[keep], dent[keep], "f32")
+    assert np.isfinite(dx).all()
+
+
+def test_nan_stays_in_its_row_and_ranks_last():
+    for V in (40, 300, 20000):
+        x = logits(np.random.default_rng(1), 3, V, "f32")
+        x[1, 7] = np.nan
+        s = Score(x, "f32", np.array([0, 1, 2]), 4)
+        s.forward()
+        got = s.host()
+        assert np.isnan(got["lp"][1]) and np.isnan(got["ent"][1]) and np.isnan(got["alt"][1]).all()
+        y = x.copy()
+        y[1, 7] = -np.inf
+        np.testing.assert_array_equal(got["ids"], U.scores(y, [0, 1, 2], 4)["ids"])
+        for r in (0, 2):
+            check_forward({k: v[r:r + 1] for k, v in got.items()}, x[r:r + 1], [r], 4)
+        dx = s.backward(np.ones(3, np.float32), np.ones(3, np.float32), "f32")
+        assert np.isnan(dx[1]).all() and np.isfinite(dx[[0, 2]]).all()
+
+
+def test_peaked_rows_keep_what_is_beside_the_peak():
+    """ln p of the peak is -rest, of the order 1e-8: a sum that holds the peak's 1 would lose it."""
+    x = np.zeros((2, 4))
+    x[0] = [18.0, 0, -1, -2]
+    x[1] = [0, 25.0, 25.0 - 16.0, 3.0]
+    tokens = np.array([0, 1])
+    s = Score(x, "f32", tokens, 2)
+    s.forward()
+    got, want = s.host(), U.scores(x, tokens, 2)
+    np.testing.assert_allclose(got["lp"], want["logprob"], rtol=1e-5)
+    np.testing.assert_allclose(got["ent"], want["entropy"], rtol=1e-5)
+    dx = s.backward(np.ones(2, np.float32), np.zeros(2, np.float32), "f32")
+    np.testing.assert_allclose(dx, U.gradient(x, tokens, np.ones(2), np.zeros(2)), rtol=1e-5, atol=1e-30)
+
+
+def test_gradient_against_differences_of_the_forward():
+    """The forward's own outputs at x +- h d: the difference is off by h^2 / 6 |f'''| (|f'''| < 8 max|d|^3 sum|w|
+    for the log-sum and the entropy's fourth moment) and by the outputs' rounding over h."""
+    rng = np.random.default_rng(11)
+    n, V, h = 6, 700, 2.0 ** -5
+    x = G.O.round_to(rng.normal(0, 1, (n, V)), "bf16")  # x +- h d is exact in fp32
+    d = np.sign(rng.normal(size=(n, V)))
+    tokens = rng.integers(0, V, n)
+    dlp, dent = rng.normal(size=n).astype(np.float32), rng.normal(size=n).astype(np.float32)
+    f = []
+    for sign in (1, -1):
+        s = Score(x + sign * h * d, "f32", tokens, 0)
+        s.forward()
+        g = s.host()
+        f.append(float(dlp.astype(np.float64) @ g["lp"] + dent.astype(np.float64) @ g["ent"]))
+    s = Score(x, "f32", tokens, 0)
+    s.forward()
+    dx = s.backward(dlp, dent, "f32")
+    weight = np.abs(dlp).sum() + np.abs(dent).sum() * 10
+    assert abs((f[0] - f[1]) / (2 * h) - (dx * d).sum()) < weight * (8 * h * h / 6 + 50 * ULP * 10 / h)
+
+
+def test_rows_past_32_bits():
+    """Rows whose first element lies past 2^31 elements."""
+    N, lib = native()
+    ld, V = 1 << 30, 300
+    x = G.empty(2 * ld + V, "bf16")
+    rng = np.random.default_rng(4)
+    rows = logits(rng, 3, V, "bf16")
+    for r in range(3):
+        raw = (rows[r].astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)
+        N.api.sj_upload(x.at(r * ld), raw.ctypes.data, raw.nbytes)
+    s = Score(rows, "bf16", np.array([5, 6, 7]), 3)
+    s.x, s.ld = x, ld
+    s.forward()
+    check_forward(s.host(), rows, np.array([5, 6, 7]), 3)
+    check_backward(s.backward(np.ones(3, np.float32), np.ones(3, np.float32), "f32"), rows, np.array([5, 6, 7]), np.ones(3),
+                   np.ones(3), "f32")
+
+
+@pytest.mark.parametrize("n,V", [(40, 257), (3, 60000)])
+def test_captured_scores_replay(n, V):
+    """Forward and backward in one graph; new logits between the replays, every replay against the definitions."""
+    rng = np.random.default_rng(9)
+    x = logits(rng, n, V, "f32")
+    tokens = rng.integers(0, V, n)
+    s = Score(x, "f32", tokens, 6)
+    N, lib = native()
+    dlp, dent, dx = G.dev(np.ones(n)), G.dev(np.full(n, 0.5)), G.empty(n * V)
+
+    def record(stream):
+        s.forward(stream)
+        N.api.sj_token_logprobs_bwd(stream, s.x.p, 0, s.ld, n, V, s.tokens.p, s.stats.p, s.ent.p, dlp.p, dent.p, dx.p, 0, V)
+    g = PU.Graph(record)
+    for k in range(3):
+        x = logits(rng, n, V, "f32")
+        s.x.upload(x)
+        g.replay()
+        check_forward(s.host(), x, tokens, 6)
+        check_backward(dx.host().reshape(n, V), x, tokens, np.ones(n), np.full(n, 0.5), "f32")
+    g.close()
