@@ -26,7 +26,8 @@ HIPFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
 # allocator rotated them through v_accvgpr moves inside the hot loops (the
 # token-split dW kernel every step, the attention forward's output tile).
 _VGPR_ACC = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-EXTRA = {"gemm_fast.hip": _VGPR_ACC, "attention_t.hip": _VGPR_ACC, "attention.hip": _VGPR_ACC, "gemm.hip": _VGPR_ACC}
+EXTRA = {"gemm_fast.hip": _VGPR_ACC, "attention_t.hip": _VGPR_ACC, "attention.hip": _VGPR_ACC, "gemm.hip": _VGPR_ACC,
+         "paged.hip": _VGPR_ACC}
 
 
 def _hipcc():

@@ -42,6 +42,7 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
   long long tok = 0, need = 0;
   uint32_t want = 0, longest = 0;
   int bad = 0;
+#pragma unroll 1
   for (int r = r0; r < r1; r++) {
     const int n = a.lengths[r], m = a.counts[r];
     if ((n | m) < 0) {
@@ -89,6 +90,7 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
   const long t0 = (long)blockIdx.x * PT;
   long long s = st - tok, f = sn - need;
   const bool lead = blockIdx.x == 0;
+#pragma unroll 1
   for (int r = r0; r < r1; r++) {
     const int n = a.lengths[r], m = a.counts[r];
     if (lead) {
@@ -146,6 +148,27 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
 }
 
 // -------------------------------------------------------------- attention
+//
+//   o = sum_j e^(s_j - m) v_j / l,  m = max s_j,  l = sum_j e^(s_j - m)
+//
+// One wave walks tiles of 16 to 64 keys of one KV head for up to 16 of its
+// query heads at once, with the running maximum and sum of each query: the
+// group's query heads are the columns of one MFMA tile, so a key is read once
+// for all of them, and padding the group to 16 columns costs matrix time that
+// a memory-bound walk has to spare.
+//   S^T [keys][queries] = K q^T: the K rows go from memory straight into the
+//     operand (lane = key, 16 bytes of the row).
+//   O^T [columns][queries] += V^T P^T: a lane holds P^T for the keys 4g .. 4g
+//     + 3 of each 16, exactly as S^T left it, so the product takes its keys in
+//     that order and P moves nowhere; a query is one lane column in both, so
+//     the rescaling by the running maximum needs no exchange either.
+// bf16: V^T is read from a tile that the wave keeps in LDS for itself (no
+// barriers), with ds_read_b64_tr_b16.  P feeds the product as two bf16 planes:
+// one rounding to 8 bits would cost as much as the output's own, the second
+// plane costs matrix time that is free here.  fp32: the fp32 MFMA, whose
+// operands are single values, takes V as it lies; nothing is rounded.
+// The loads of a tile are in flight while the one before is computed, its page
+// ids one tile earlier still.
 
 struct PagedArgs {
   const void* q;
@@ -160,8 +183,14 @@ struct PagedArgs {
   float* lse;
   int requests, rows, HQ, HK, D;
   int pages, P;
+  uint32_t pmul, pshift;  // division by P (page_col)
   long window;
   float scale;  // log2(e) / sqrt(D): the softmax in powers of two
+  int G, QT;    // query heads of a KV head, and their tiles of 16
+  // split walks
+  float* part;    // [2 * waves][slot]
+  int32_t* plan;  // tiles of a wave, then the rows' exclusive tile counts
+  int slot;       // floats of a partial: 16 maxima, 16 sums, min(G, 16) rows of D
 };
 
 // the keys a row sees, [lo, hi), and its request; false for a padded row
@@ -176,9 +205,498 @@ __device__ __forceinline__ bool row_range(const PagedArgs& a, int row, int& owne
   return true;
 }
 
-// The first row of scores and sums a wave carries along a walk, merged over
-// the four waves of a workgroup (one row and query head).  A lane owns a key
-// in the products with q and columns lane + 64 c in the sums over v.
+// n / P for n < 2^31: the multiplier is floor(2^32 (2^shift - P) / P) + 1
+// with 2^shift >= P, and the 33rd bit of 2^32 + multiplier is the added n
+__device__ __forceinline__ int page_col(const PagedArgs& a, int n) {
+  return (int)((__umulhi(a.pmul, (uint32_t)n) + (uint32_t)n) >> a.pshift);
+}
+
+// 16 bytes at any alignment
+struct __attribute__((packed, aligned(2))) Raw16 {
+  u32x4 v;
+};
+__device__ __forceinline__ u32x4 load16(const void* p) { return ((const Raw16*)p)->v; }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef float f32x2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t cvt2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){a, b}, bf16x2v));
+}
+
+// A wave's walk.  DC: the head in units of 32 columns.  E: elements of 16
+// bytes, KT: keys of a tile, NC: 16-byte chunks that a lane holds of a row.
+template <typename T, int DC>
+struct Walk {
+  static constexpr bool BF = sizeof(T) == 2;
+  static constexpr int DP = 32 * DC, E = BF ? 8 : 4;
+  static constexpr int KT = BF ? (DC <= 2 ? 64 : 32) : (DC <= 2 ? 32 : 16), KS = KT / 16;
+  static constexpr int NC = DP / (4 * E);
+  // fp32 V: a lane takes VW columns of a key, 16 lanes NV blocks of them
+  static constexpr int VW = BF ? 1 : (DC == 1 ? 2 : 4), NV = BF ? 1 : DP / (16 * VW);
+  static constexpr int NO = DP / 16;            // output tiles of 16 columns
+  static constexpr int STRIDE = DP + 8;         // bf16 V tile in LDS: rows 16 bytes apart in the banks
+  static constexpr int LDS = BF ? (KT * STRIDE * 2 > 64 * DP ? KT * STRIDE * 2 : 64 * DP) : 64 * DP;  // >= 16 x DP floats
+  // chunks that may lie past the head
+  static constexpr int FIRST_TAIL = DC == 1 ? 0 : DC == 8 ? NC / 2 : BF ? DC - 1 : (DC == 4 ? 4 : NC - 2);
+
+  u32x4 q[NC];
+  u32x4 k[KS][NC];
+  u32x4 v[BF ? KS : 4 * KS][BF ? NC : (NV * VW + 3) / 4];
+  f32x4 o[NO];
+  float m, l;
+  int pid[KS], sl[KS];
+
+  __device__ __forceinline__ void start(const PagedArgs& a, int row, int kh, int qt, int lane) {
+    const int col = lane & 15, g = lane >> 4, h = qt * 16 + col;
+    const T* x = (const T*)a.q + (long)row * a.ldq + ((long)kh * a.G + h) * a.D;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const int d = (4 * c + g) * E;
+      q[c] = h < a.G && d < a.D ? load16(x + d) : u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int i = 0; i < NO; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  // page ids of the tile's keys (lane & 15 of each 16), -1 past the range
+  __device__ __forceinline__ void look(const PagedArgs& a, const int32_t* pages, int base, int hi, int lane) {
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const int j = base + 16 * s + (lane & 15);
+      pid[s] = j < hi ? pages[page_col(a, j)] : -1;
+    }
+  }
+  __device__ __forceinline__ void place(const PagedArgs& a, int base, int lane) {
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const int j = base + 16 * s + (lane & 15);
+      const bool in = (uint32_t)pid[s] < (uint32_t)a.pages;
+      sl[s] = in ? pid[s] * a.P + (j - page_col(a, j) * a.P) : -1;
+    }
+  }
+  // a key without a slot reads slot 0 and is masked in scores() and store_v()
+  __device__ __forceinline__ void load_k(const PagedArgs& a, const T* K, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const T* x = K + (long)max(sl[s], 0) * a.ldkv;
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        const int d = (4 * c + g) * E;
+        k[s][c] = load16(x + (c < FIRST_TAIL || d < a.D ? d : 0));
+      }
+    }
+  }
+  __device__ __forceinline__ void load_v(const PagedArgs& a, const T* V, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      if constexpr (BF) {
+        const T* x = V + (long)max(sl[s], 0) * a.ldkv;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          const int d = (4 * c + g) * E;
+          v[s][c] = load16(x + (c < FIRST_TAIL || d < a.D ? d : 0));
+        }
+      } else {
+        // lane (column block lane & 15, keys 4g + i): one value of each key
+        // and column is one operand
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int slot = __shfl(sl[s], 4 * g + i, 64);
+          const float* x = (const float*)V + (long)max(slot, 0) * a.ldkv;
+          if constexpr (VW == 4) {
+#pragma unroll
+            for (int b = 0; b < NV; b++) {
+              const int d = 64 * b + 4 * (lane & 15);
+              v[4 * s + i][b] = load16(x + (d < a.D ? d : 0));
+              if (slot < 0) v[4 * s + i][b] = u32x4{0u, 0u, 0u, 0u};
+            }
+          } else {
+            const int d = 2 * (lane & 15);
+            const uint32_t* y = (const uint32_t*)(x + (d < a.D ? d : 0));
+            const uint32_t y0 = y[0], y1 = y[1];
+            v[4 * s + i][0] = slot < 0 ? u32x4{0u, 0u, 0u, 0u} : u32x4{y0, y1, 0u, 0u};
+          }
+        }
+      }
+    }
+  }
+  // S^T of the tile, the running maximum, and P in place of S
+  __device__ __forceinline__ void scores(const PagedArgs& a, f32x4 (&p)[KS], int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        u32x4 kk = k[s][c];
+        if (c >= FIRST_TAIL && (4 * c + g) * E >= a.D) kk = u32x4{0u, 0u, 0u, 0u};
+        if constexpr (BF) {
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk), __builtin_bit_cast(bf16x8, q[c]),
+                                                        acc, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk[e]), __uint_as_float(q[c][e]), acc, 0, 0, 0);
+        }
+      }
+      const uint64_t good = __ballot(sl[s] >= 0);
+      if ((good & 0xffffu) != 0xffffu) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (!((good >> (4 * g + i)) & 1)) acc[i] = -INFINITY;
+      }
+      p[s] = acc;
+    }
+    float t = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) t = fmaxf(t, p[s][i]);
+    t = fmaxf(t, __shfl_xor(t, 16, 64));
+    t = fmaxf(t, __shfl_xor(t, 32, 64));
+    const float mn = fmaxf(m, t);
+    // no key with a share so far: the reference is 0, and every power 0.  The
+    // difference first, then the scale: s * c - m * c in one fused step would
+    // keep the rounding of m * c, at large scores more than the powers' range
+    const float c = a.scale, ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - ref) * c);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        p[s][i] = __builtin_amdgcn_exp2f((p[s][i] - ref) * c);
+        sum += p[s][i];
+      }
+    l = l * alpha + sum;  // this lane's keys alone: joined in finish()
+#pragma unroll
+    for (int i = 0; i < NO; i++) o[i] *= alpha;
+  }
+  // bf16: the V rows to the wave's LDS tile, keys without a slot as zeros
+  __device__ __forceinline__ void store_v(bf16_t* tile, int lane) {
+    if constexpr (BF) {
+      const int g = lane >> 4;
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+          *(u32x4*)(tile + (16 * s + (lane & 15)) * STRIDE + (4 * c + g) * 8) =
+              sl[s] >= 0 ? v[s][c] : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  __device__ __forceinline__ void sums(const bf16_t* tile, const f32x4 (&p)[KS], int lane) {
+    if constexpr (BF) {
+      const int g = lane >> 4, e = (lane >> 2) & 3, c4 = 4 * (lane & 3);
+#pragma unroll
+      for (int s = 0; s < KS; s += 2) {
+        u32x4 ph, pl;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const float x = p[s + h][2 * i], y = p[s + h][2 * i + 1];
+            const uint32_t w = cvt2(x, y);
+            ph[2 * h + i] = w;
+            pl[2 * h + i] = cvt2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xffff0000u));
+          }
+#pragma unroll
+        for (int d = 0; d < NO; d++) {
+          s16x4 r[2];
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            r[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(tile + (16 * (s + h) + 4 * g + e) * STRIDE + 16 * d + c4));
+          const bf16x8 vt = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, __builtin_bit_cast(bf16x8, ph), o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int b = 0; b < NV; b++)
+#pragma unroll
+            for (int t = 0; t < VW; t++)
+              o[b * VW + t] =
+                  __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[4 * s + i][b][t]), p[s][i], o[b * VW + t], 0, 0, 0);
+    }
+  }
+  // tiles t0, t0 + step, .. below t1 of the keys [lo, hi)
+  __device__ __forceinline__ void run(const PagedArgs& a, const int32_t* pages, int kh, int lo, int hi, int t0, int t1,
+                                      int step, bf16_t* tile, int lane) {
+    if (t0 >= t1) return;
+    const T* K = (const T*)a.k + (long)kh * a.D;
+    const T* V = (const T*)a.v + (long)kh * a.D;
+    const int inc = step * KT;  // keys past hi are masked, and tiles past t1 not taken
+    int base = lo + t0 * KT;
+    look(a, pages, base, hi, lane);
+    place(a, base, lane);
+    load_k(a, K, lane);
+    load_v(a, V, lane);
+    const bool more = t0 + step < t1;
+    if (more) look(a, pages, base + inc, hi, lane);
+    for (int t = t0; t < t1; t += step) {
+      f32x4 p[KS];
+      scores(a, p, lane);
+      if constexpr (BF) store_v(tile, lane);
+      const bool next = t + step < t1;
+      if (next) {
+        base += inc;
+        place(a, base, lane);
+        load_k(a, K, lane);
+        if constexpr (BF) load_v(a, V, lane);
+        if (t + 2 * step < t1) look(a, pages, base + inc, hi, lane);
+      }
+      __builtin_amdgcn_wave_barrier();
+      sums(tile, p, lane);
+      __builtin_amdgcn_wave_barrier();
+      if constexpr (!BF) {
+        if (next) load_v(a, V, lane);
+      }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+  }
+  // four columns of this lane's query: i-th quad of the lane, its first column
+  static constexpr int QUADS = DP / 16;
+  __device__ __forceinline__ int quad(int i, int lane, f32x4& x) const {
+    const int g = lane >> 4;
+    if constexpr (BF) {
+      x = o[i];
+      return 16 * i + 4 * g;
+    } else if constexpr (VW == 4) {
+      const int b = i >> 2, e = i & 3;
+#pragma unroll
+      for (int t = 0; t < 4; t++) x[t] = o[4 * b + t][e];
+      return 64 * b + 16 * g + 4 * e;
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; t++) x[t] = o[t & 1][2 * i + (t >> 1)];
+      return 8 * g + 4 * i;
+    }
+  }
+};
+
+__device__ __forceinline__ float natural_lse(float m, float l, float c) {
+  return l == 0.f ? -INFINITY : (m * c + log2f(l)) * 0.6931471805599453f;
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* y, const f32x4& x, float inv) {
+  if constexpr (sizeof(T) == 2) {
+    struct __attribute__((packed, aligned(2))) P { uint32_t a, b; };
+    *(P*)y = P{cvt2(x[0] * inv, x[1] * inv), cvt2(x[2] * inv, x[3] * inv)};
+  } else {
+    struct __attribute__((packed, aligned(4))) P { float a, b, c, d; };
+    *(P*)y = P{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+  }
+}
+
+// One workgroup per row, KV head and tile of 16 query heads: its waves take
+// the key tiles in turn and join in LDS.  For walks that are short, or rows
+// that are many.
+constexpr int direct_waves(int dc) { return dc == 8 ? 4 : 8; }  // 256 registers a lane at most hold 8
+template <typename T, int DC>
+__global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArgs a) {
+  typedef Walk<T, DC> W;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ float wm[8][16], wl[8][16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int nb = a.HK * a.QT, row = blockIdx.x / nb, hb = blockIdx.x - row * nb, kh = hb / a.QT, qt = hb - kh * a.QT;
+  int owner, lo, hi;
+  if (!row_range(a, row, owner, lo, hi)) return;
+  W wk;
+  wk.start(a, row, kh, qt, lane);
+  const int tiles = (hi - lo + W::KT - 1) / W::KT;
+  bf16_t* tile = (bf16_t*)(lds + w * W::LDS);
+  wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, w, tiles, nw, tile, lane);
+  const int q = lane & 15, n = min(16, a.G - qt * 16);
+  if (lane < 16) wm[w][lane] = wk.m, wl[w][lane] = wk.l;
+  float* mine = (float*)(lds + w * W::LDS);
+#pragma unroll
+  for (int i = 0; i < W::QUADS; i++) {
+    f32x4 x;
+    const int d = wk.quad(i, lane, x);
+    if (q < n) *(f32x4*)(mine + q * W::DP + d) = x;
+  }
+  __syncthreads();
+  const int quads = a.D / 4;
+  for (int u = threadIdx.x; u < n * quads; u += blockDim.x) {
+    const int r = u / quads, d = 4 * (u - r * quads);
+    float M = -INFINITY, L = 0.f;
+    for (int i = 0; i < nw; i++) M = fmaxf(M, wm[i][r]);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < nw; i++) {
+      const float li = wl[i][r];
+      if (li == 0.f) continue;
+      const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((wm[i][r] - M) * a.scale);
+      L += li * f;
+      s += *(const f32x4*)((const float*)(lds + i * W::LDS) + r * W::DP + d) * f;
+    }
+    const long h = (long)kh * a.G + qt * 16 + r;
+    put4((T*)a.o + (long)row * a.ldo + h * a.D + d, s, L == 0.f ? 0.f : 1.f / L);
+    if (a.lse && d == 0) a.lse[(long)row * a.HQ + h] = natural_lse(M, L, a.scale);
+  }
+}
+
+// Long walks, or few: all the tiles of all rows and heads in one line, and
+// every wave an equal piece of it, whatever the rows' lengths.  A piece that
+// holds a whole walk writes its result; a walk that is cut leaves partial
+// maxima, sums and rows, which k_paged_join joins in the order of the keys.
+// A wave has at most two of them: the end of one walk and the beginning of
+// another.  Each workgroup sums the rows' tiles itself (one block scan).
+constexpr int STREAM_ROWS = 2048;
+template <typename T, int DC>
+__global__ __launch_bounds__(256) void k_paged_stream(PagedArgs a) {
+  typedef Walk<T, DC> W;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int pre[STREAM_ROWS + 1], ws[4];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, nb = a.HK * a.QT;
+  constexpr int MOST = STREAM_ROWS / 256;
+  const int per = (a.rows + 255) / 256;
+  int n[MOST], mine = 0;
+#pragma unroll
+  for (int i = 0; i < MOST; i++) {
+    n[i] = 0;
+    const int r = t * per + i;
+    int owner, lo, hi;
+    if (i < per && r < a.rows && row_range(a, r, owner, lo, hi)) n[i] = (hi - lo + W::KT - 1) / W::KT;
+    mine += n[i];
+  }
+  int at = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(at, o, 64);
+    if (lane >= o) at += u;
+  }
+  if (lane == 63) ws[w] = at;
+  __syncthreads();
+  for (int i = 0; i < w; i++) at += ws[i];
+  at -= mine;
+#pragma unroll
+  for (int i = 0; i < MOST; i++) {
+    const int r = t * per + i;
+    if (i < per && r < a.rows) {
+      pre[r] = at;
+      if (blockIdx.x == 0) a.plan[1 + r] = at;
+      at += n[i];
+    }
+  }
+  const int all = ws[0] + ws[1] + ws[2] + ws[3];
+  const int total = all * nb, waves = gridDim.x * 4;
+  const int piece = max(1, (int)(((long)total + waves - 1) / waves));
+  if (t == 0) {
+    pre[a.rows] = all;
+    if (blockIdx.x == 0) a.plan[0] = piece, a.plan[1 + a.rows] = all;
+  }
+  __syncthreads();
+  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + w);
+  if ((long)wave * piece >= total) return;
+  int x = wave * piece;
+  const int e = (int)min((long)total, (long)x + piece);
+  bf16_t* tile = (bf16_t*)(lds + w * W::LDS);
+  W wk;
+  while (x < e) {
+    // the row that holds tile x: the last whose tiles begin at or before it
+    int r0 = 0, r1 = a.rows;
+    const int y = x / nb;
+    while (r1 - r0 > 1) {
+      const int mid = (r0 + r1) >> 1;
+      if (pre[mid] <= y) r0 = mid; else r1 = mid;
+    }
+    const int row = __builtin_amdgcn_readfirstlane(r0);
+    const int first = __builtin_amdgcn_readfirstlane(pre[row]);
+    const int nt = __builtin_amdgcn_readfirstlane(pre[row + 1]) - first;
+    const int in = x - first * nb, hb = in / nt, t0 = in - hb * nt, t1 = min(nt, t0 + e - x);
+    const int kh = hb / a.QT, qt = hb - kh * a.QT;
+    int owner, lo, hi;
+    row_range(a, row, owner, lo, hi);
+    owner = __builtin_amdgcn_readfirstlane(owner);
+    wk.start(a, row, kh, qt, lane);
+    wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, t0, t1, 1, tile, lane);
+    const int q = lane & 15, nq = min(16, a.G - qt * 16);
+    if (t0 == 0 && t1 == nt) {
+      const long h = (long)kh * a.G + qt * 16 + q;
+      T* y = (T*)a.o + (long)row * a.ldo + h * a.D;
+      const float inv = wk.l == 0.f ? 0.f : 1.f / wk.l;
+#pragma unroll
+      for (int i = 0; i < W::QUADS; i++) {
+        f32x4 v;
+        const int d = wk.quad(i, lane, v);
+        if (q < nq && d < a.D) put4(y + d, v, inv);
+      }
+      if (a.lse && lane < nq) a.lse[(long)row * a.HQ + h] = natural_lse(wk.m, wk.l, a.scale);
+    } else {
+      float* s = a.part + ((long)2 * wave + (t0 == 0)) * a.slot;
+      if (lane < 16) s[lane] = wk.m, s[16 + lane] = wk.l;
+#pragma unroll
+      for (int i = 0; i < W::QUADS; i++) {
+        f32x4 v;
+        const int d = wk.quad(i, lane, v);
+        if (q < nq && d < a.D) *(f32x4*)(s + 32 + q * a.D + d) = v;
+      }
+    }
+    x += t1 - t0;
+  }
+}
+
+// The cut walks of one row and query head: partial i is that of wave first +
+// i, in the order of the keys.  Threads own columns and share the partials.
+template <typename T>
+__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
+  __shared__ float red[2][4];
+  __shared__ f32x4 acc[256];
+  const int row = blockIdx.x, h = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int piece = a.plan[0], p0 = a.plan[1 + row], nt = a.plan[2 + row] - p0;
+  if (nt == 0) return;
+  const int kh = h / a.G, hg = h - kh * a.G, qt = hg >> 4, q = hg & 15, nb = a.HK * a.QT;
+  const int x0 = p0 * nb + (kh * a.QT + qt) * nt, w0 = x0 / piece, w1 = (x0 + nt - 1) / piece, n = w1 - w0 + 1;
+  if (n == 1) return;
+  auto slot = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0)) * a.slot; };
+  float M = -INFINITY;
+  for (int i = t; i < n; i += 256) M = fmaxf(M, slot(i)[q]);
+  M = wave_max(M);
+  if (lane == 0) red[0][w] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const int quads = a.D / 4, groups = 256 / quads, gr = t / quads, d = 4 * (t - gr * quads);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  if (gr < groups)
+    for (int i = gr; i < n; i += groups) {
+      const float* p = slot(i);
+      const float l = p[16 + q];
+      if (l == 0.f) continue;
+      const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((p[q] - M) * a.scale);
+      s += *(const f32x4*)(p + 32 + q * a.D + d) * f;
+      L += l * f;
+    }
+  acc[t] = s;
+  __shared__ float ls[256];
+  ls[t] = L;
+  __syncthreads();
+  if (gr) return;
+  for (int i = 1; i < groups; i++) {
+    s += acc[i * quads + t];
+    L += ls[i * quads + t];
+  }
+  put4((T*)a.o + (long)row * a.ldo + (long)h * a.D + d, s, L == 0.f ? 0.f : 1.f / L);
+  if (a.lse && t == 0) a.lse[(long)row * a.HQ + h] = natural_lse(M, L, a.scale);
+}
+
+// Heads that are no whole 16-byte chunks: one workgroup per row and query
+// head.  A lane owns a key in the products with q and columns lane + 64 c in
+// the sums over v.
 template <typename T>
 __global__ __launch_bounds__(256) void k_paged_rows(PagedArgs a) {
   __shared__ float q[256], p[4][64], acc[4][256], wm[4], wl[4];
@@ -280,8 +798,81 @@ extern "C" int sj_paged_plan(void* stream, const int32_t* lengths, const int32_t
   return SJ_OK;
 }
 
+namespace {
+
+// waves of the split walks: as many as the chip holds at once
+constexpr int STREAM_GROUPS = 1024;
+
+// whether sj_paged_attention splits: a rule on sizes alone, so that the
+// workspace query knows it too
+bool split_ok(long rows, long head_dim) { return rows <= STREAM_ROWS && head_dim % 4 == 0; }
+long slot_floats(long g, long head_dim) { return 32 + (g < 16 ? g : 16) * head_dim; }
+
+// f(Walk<T, DC>) for the head's width
+template <typename T, class F>
+void by_width(long D, F f) {
+  if (D <= 32) f(Walk<T, 1>());
+  else if (D <= 64) f(Walk<T, 2>());
+  else if (D <= 96 && sizeof(T) == 2) f(Walk<T, sizeof(T) == 2 ? 3 : 4>());
+  else if (D <= 128) f(Walk<T, 4>());
+  else f(Walk<T, 8>());
+}
+template <typename T, int DC>
+int launch_direct(hipStream_t s, const PagedArgs& a, int waves, Walk<T, DC>) {
+  static sj::OncePerDevice once;
+  if (int st = sjh::once_per_device(once, [] {
+        SJ_HIP(hipFuncSetAttribute((const void*)k_paged_direct<T, DC>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   direct_waves(DC) * Walk<T, DC>::LDS));
+        return SJ_OK;
+      }))
+    return st;
+  waves = waves < direct_waves(DC) ? waves : direct_waves(DC);
+  k_paged_direct<T, DC><<<(unsigned)((long)a.rows * a.HK * a.QT), 64 * waves, waves * Walk<T, DC>::LDS, s>>>(a);
+  return SJ_OK;
+}
+template <typename T, int DC>
+int launch_stream(hipStream_t s, const PagedArgs& a, Walk<T, DC>) {
+  static sj::OncePerDevice once;
+  if (int st = sjh::once_per_device(once, [] {
+        SJ_HIP(hipFuncSetAttribute((const void*)k_paged_stream<T, DC>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   4 * Walk<T, DC>::LDS));
+        return SJ_OK;
+      }))
+    return st;
+  k_paged_stream<T, DC><<<STREAM_GROUPS, 256, 4 * Walk<T, DC>::LDS, s>>>(a);
+  k_paged_join<T><<<dim3((unsigned)a.rows, (unsigned)a.HQ), 256, 0, s>>>(a);
+  return SJ_OK;
+}
+
+template <typename T>
+int attend(hipStream_t s, PagedArgs& a, long most, void* workspace) {
+  if (a.D % (16 / (int)sizeof(T))) {
+    k_paged_rows<T><<<dim3((unsigned)a.rows, (unsigned)a.HQ), 256, 0, s>>>(a);
+    return SJ_OK;
+  }
+  const long units = (long)a.rows * a.HK * a.QT;
+  // a direct walk's waves take a tile each in turn; past 2048 keys a row the
+  // split walks pay for their second launch
+  const bool direct = most <= 2048 || !split_ok(a.rows, a.D) || (most / 16 + 1) * units > 0x7fffffffL;
+  int st = SJ_OK;
+  if (direct) {
+    int waves = units >= 1024 ? 4 : 8;
+    if (most <= 256) waves = 4;
+    by_width<T>(a.D, [&](auto w) { st = launch_direct(s, a, waves, w); });
+    return st;
+  }
+  a.slot = (int)slot_floats(a.G, a.D);
+  a.plan = (int32_t*)workspace;
+  a.part = (float*)((uint8_t*)workspace + 4 * (STREAM_ROWS + 8));
+  by_width<T>(a.D, [&](auto w) { st = launch_stream(s, a, w); });
+  return st;
+}
+
+}  // namespace
+
 extern "C" size_t sj_paged_attention_workspace_bytes(long rows, long hq, long hk, long head_dim) {
-  return 0;
+  if (rows <= 0 || hq <= 0 || hk <= 0 || head_dim <= 0 || hq % hk || !split_ok(rows, head_dim)) return 0;
+  return 4 * (STREAM_ROWS + 8) + 8 * STREAM_GROUPS * (size_t)slot_floats(hq / hk, head_dim) * sizeof(float);
 }
 
 extern "C" int sj_paged_attention(void* stream, const void* q, long ldq, const void* k_cache, const void* v_cache,
@@ -311,12 +902,15 @@ extern "C" int sj_paged_attention(void* stream, const void* q, long ldq, const v
   a.requests = (int)requests; a.rows = (int)rows; a.HQ = (int)hq; a.HK = (int)hk; a.D = (int)head_dim;
   a.pages = (int)pages; a.P = (int)page_size; a.window = window;
   a.scale = (float)(1.4426950408889634 / sqrt((double)head_dim));
-  const dim3 grid((unsigned)rows, (unsigned)hq);
+  a.G = (int)(hq / hk);
+  a.QT = (a.G + 15) / 16;
+  while ((1UL << a.pshift) < (unsigned long)page_size) a.pshift++;
+  a.pmul = (uint32_t)((((1UL << a.pshift) - (unsigned long)page_size) << 32) / (unsigned long)page_size + 1);
+  SJ_REQUIRE(rows <= 0x7fffffffL / (hk * a.QT), "paged attention: %ld rows of %ld heads", rows, hk);
+  long most = ldt * page_size;
+  if (window > 0 && window < most) most = window;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == SJ_BF16)
-    k_paged_rows<bf16_t><<<grid, 256, 0, s>>>(a);
-  else
-    k_paged_rows<float><<<grid, 256, 0, s>>>(a);
+  if (int st = dtype == SJ_BF16 ? attend<bf16_t>(s, a, most, workspace) : attend<float>(s, a, most, workspace)) return st;
   SJ_LAUNCH_CHECK("paged attention");
   return SJ_OK;
 }
