@@ -138,7 +138,7 @@ int sj_rope_frequencies(void *stream, uint64_t *turns, long rotary_dim, const sj
  * is good to 2^-22 up to position 2^27.  x and y fp32 or bf16 (stored value in, fp32
  * products, one rounding); y may be x.  head_dim even, at most 1024; any
  * strides and element alignment (16-byte rows are fastest).  turns may be
- * null when rotary_dim is 0. */
+ * null when rotary_dim is 0; at most 2^24 rows. */
 #define SJ_ROPE_INTERLEAVED 0
 #define SJ_ROPE_HALF 1
 int sj_rope_rows(void *stream, const void *x, long ldx, void *y, long ldy, int dtype, long rows, long heads,
@@ -408,7 +408,7 @@ int sj_paged_plan(void *stream, const int32_t *lengths, const int32_t *counts, l
  * keys rotated and values copied into the cache rows of their slots; the
  * rotation as sj_rope_rows.  A row whose slot is not in 0 .. cache_slots - 1
  * is left out whole (q_out too).  The slots of one call are distinct.  q_out
- * may be q; hq may be 0.  Any strides and element alignment. */
+ * may be q; hq may be 0.  Any strides and element alignment; at most 2^24 rows. */
 int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, int dtype,
                     long rows, long hq, long hk, long head_dim, long rotary_dim, int layout, const int32_t *positions,
                     const int32_t *slots, const uint64_t *turns, float amplitude, void *q_out, long ldqo,
@@ -423,7 +423,7 @@ int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long l
  * key gives o = 0 and lse = -inf; rows with position or owner below 0 (or an
  * owner past the requests) are left as they were.  Slots past a request's
  * length are never read into a result, whatever they hold.  head_dim at most
- * 256, any strides and alignment.  Workspace:
+ * 256; rows times hk at most 2^23; any strides and element alignment.  Workspace:
  * sj_paged_attention_workspace_bytes, not cleared and not kept; calls that
  * share one must not overlap. */
 size_t sj_paged_attention_workspace_bytes(long rows, long hq, long hk, long head_dim);
@@ -728,7 +728,8 @@ int sj_cross_entropy(void *stream, const float *x, long ldx, const int32_t *targ
  * [rows][top].  logprob (then tokens too), entropy and stats are nullable.
  * Entries of -inf have no share; a row of nothing else has entropy 0, log
  * probabilities -inf and stats (0, 0).  A NaN makes its row's numbers NaN and
- * is ranked behind everything.  top at most SJ_LOGPROBS_MAX_TOP and vocab.
+ * is ranked behind everything.  top at most SJ_LOGPROBS_MAX_TOP and vocab;
+ * vocab at most 2^24, and rows times vocab / 8192 (rounded up) too.
  * Any stride and element alignment.  Workspace:
  * sj_token_logprobs_workspace_bytes, not cleared and not kept. */
 #define SJ_LOGPROBS_MAX_TOP 64
@@ -740,7 +741,7 @@ int sj_token_logprobs(void *stream, const void *x, int dtype, long ldx, long row
  * p_v) - dentropy[r] p_v (ln p_v + entropy[r]), written, not accumulated.
  * dlogprob (then tokens too) and dentropy (then entropy too) are nullable; a
  * token outside the vocabulary has no share through dlogprob.  stats and
- * entropy as the forward left them. */
+ * entropy as the forward left them; dx may be x (the same type and stride). */
 int sj_token_logprobs_bwd(void *stream, const void *x, int dtype, long ldx, long rows, long vocab,
                           const int32_t *tokens, const float *stats, const float *entropy, const float *dlogprob,
                           const float *dentropy, void *dx, int dx_dtype, long lddx);

@@ -906,7 +906,7 @@ extern "C" int sj_paged_attention(void* stream, const void* q, long ldq, const v
   a.QT = (a.G + 15) / 16;
   while ((1UL << a.pshift) < (unsigned long)page_size) a.pshift++;
   a.pmul = (uint32_t)((((1UL << a.pshift) - (unsigned long)page_size) << 32) / (unsigned long)page_size + 1);
-  SJ_REQUIRE(rows <= 0x7fffffffL / (hk * a.QT), "paged attention: %ld rows of %ld heads", rows, hk);
+  SJ_REQUIRE(rows <= (1L << 23) / (hk * a.QT), "paged attention: %ld rows of %ld heads", rows, hk);
   long most = ldt * page_size;
   if (window > 0 && window < most) most = window;
   hipStream_t s = (hipStream_t)stream;

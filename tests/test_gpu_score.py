@@ -244,6 +244,38 @@ def test_rows_past_32_bits():
                    np.ones(3), "f32")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [257, 5001])
+def test_gradient_in_place(V, dtype):
+    N, lib = native()
+    rng = np.random.default_rng(V)
+    x, tokens = logits(rng, 5, V, dtype), rng.integers(0, V, 5)
+    s = Score(x, dtype, tokens, 0)
+    s.forward()
+    dlp, dent = G.dev(np.ones(5)), G.dev(np.full(5, -0.25))
+    want = s.backward(np.ones(5, np.float32), np.full(5, -0.25, np.float32), dtype)
+    N.api.sj_token_logprobs_bwd(None, s.x.p, CODE[dtype], V, 5, V, s.tokens.p, s.stats.p, s.ent.p, dlp.p, dent.p, s.x.p,
+                                CODE[dtype], V)
+    np.testing.assert_array_equal(s.x.host().reshape(5, V), want)
+
+
+def crowded(n, V, seed):
+    """Rows whose largest entries all lie with a few threads: more than LDS holds at the threshold."""
+    rng = np.random.default_rng(seed)
+    x = rng.normal(0, 1, (n, V))
+    at = np.arange(V)
+    x[:, (at // 4) % 64 < 40] += 50.0  # of each 64 units of 16 bytes (fp32), 40 tower over the rest
+    return G.O.round_to(x, "f32")
+
+
+@pytest.mark.parametrize("V,top", [(4000, 50), (8192, 64), (30000, 64)])
+def test_crowded_rows(V, top):
+    x = crowded(2, V, V)
+    s = Score(x, "f32", np.array([1, 2]), top)
+    s.forward()
+    check_forward(s.host(), x, np.array([1, 2]), top)
+
+
 @pytest.mark.parametrize("n,V", [(40, 257), (3, 60000)])
 def test_captured_scores_replay(n, V):
     """Forward and backward in one graph; new logits between the replays, every replay against the definitions."""
