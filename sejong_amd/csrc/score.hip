@@ -18,15 +18,15 @@ using namespace sj;
 namespace {
 
 // One read of the row.  A group of threads (a wave, or a workgroup) holds a
-// slice of it in registers.  Each thread keeps its largest entry apart while
-// it looks at its entries, so that the sums run over the others and the one
-// term to leave out is known; then the sums relative to the group's maximum.
+// slice of it in registers: the maximum, then the sums relative to it.  Where
+// the sum of all terms is 2 or more, taking the 1 off loses nothing; where it
+// is less, the thread that holds the maximum sums again without it.
 // The alternatives come from a threshold: the k-th largest of 64 column maxima
 // (64 disjoint sets of entries) has at least k entries at or above it and
 // rarely many more; those are collected in LDS and each finds its place by
 // counting the larger ones.  Rows longer than a slice are joined from the
 // slices' sums and lists by a second launch.
-// The bound is the read: per entry there are about 14 operations, one of them
+// The bound is the read: per entry there are about 12 operations, one of them
 // an exponential.
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -78,6 +78,33 @@ struct Unit<bf16_t> {
 __device__ __forceinline__ float at_f32(const float* x, long i) { return x[i]; }
 __device__ __forceinline__ float at_f32(const bf16_t* x, long i) { return bf2f(x[i]); }
 
+// sums and maxima over a wave without LDS: four steps within rows of 16
+// lanes, then the four rows' values as scalars, in a fixed order
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <class F>
+__device__ __forceinline__ float wave_all(float v, F f) {
+  v = f(v, dpp<0xB1>(v));   // lanes 1, 0, 3, 2
+  v = f(v, dpp<0x4E>(v));   // lanes 2, 3, 0, 1
+  v = f(v, dpp<0x141>(v));  // mirrored within 8
+  v = f(v, dpp<0x140>(v));  // mirrored within 16
+  const int b = __float_as_int(v);
+  const float r0 = __int_as_float(__builtin_amdgcn_readlane(b, 0)), r1 = __int_as_float(__builtin_amdgcn_readlane(b, 16)),
+              r2 = __int_as_float(__builtin_amdgcn_readlane(b, 32)), r3 = __int_as_float(__builtin_amdgcn_readlane(b, 48));
+  return f(f(r0, r1), f(r2, r3));
+}
+__device__ __forceinline__ float all_max(float v) {
+  return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float all_min(float v) {
+  return wave_all(v, [](float a, float b) { return fminf(a, b); });
+}
+__device__ __forceinline__ float all_sum(float v) {
+  return wave_all(v, [](float a, float b) { return a + b; });
+}
+
 struct ScoreArgs {
   const void* x;
   long ldx;
@@ -87,26 +114,42 @@ struct ScoreArgs {
   float *logprob, *entropy, *stats;
   int32_t* ids;
   float* alt;
-  uint8_t* part;  // per row and slice: rest, xs, the largest key, then `top` keys
+  uint8_t* part;  // per row: (m, rest, xs, -) of each slice, then each slice's `top` keys
 };
-__device__ __forceinline__ float* part_at(const ScoreArgs& a, long row, int slice) {
-  return (float*)(a.part + (row * a.slices + slice) * (16 + 8L * a.top));
+__device__ __forceinline__ float* part_sums(const ScoreArgs& a, long row) {
+  return (float*)(a.part + row * a.slices * (16 + 8L * a.top));
+}
+__device__ __forceinline__ u64* part_keys(const ScoreArgs& a, long row) {
+  return (u64*)(a.part + row * a.slices * (16 + 8L * a.top) + 16L * a.slices);
 }
 
-// a row's numbers from its maximum, rest and xs = sum e^(x - m) (x - m)
+// what every thread of a row's group knows of its token, asked for early
+struct Token {
+  bool scored;
+  float y;
+};
 template <typename T>
-__device__ __forceinline__ float write_row(const ScoreArgs& a, long row, float m, float rest, float xs, float& ref,
-                                           bool lead) {
+__device__ __forceinline__ Token token_of(const ScoreArgs& a, long row) {
+  const int tk = a.tokens ? a.tokens[row] : -1;
+  const bool scored = tk >= 0 && tk < a.V;
+  return Token{scored, scored ? at_f32((const T*)a.x + row * a.ldx, tk) : 0.f};
+}
+// a row's numbers from its maximum, rest and xs = sum e^(x - m) (x - m)
+__device__ __forceinline__ float write_row(const ScoreArgs& a, long row, float m, float rest, float xs, const Token& tk,
+                                           float& ref, bool lead) {
   const bool none = m == -INFINITY && !(rest != rest);
   ref = m == -INFINITY ? 0.f : m;
   const float ll = none ? 0.f : log1pf(rest);
   if (lead) {
-    const int tk = a.tokens ? a.tokens[row] : -1;
-    if (a.logprob) a.logprob[row] = tk >= 0 && tk < a.V ? at_f32((const T*)a.x + row * a.ldx, tk) - ref - ll : 0.f;
+    if (a.logprob) a.logprob[row] = tk.scored ? tk.y - ref - ll : 0.f;
     if (a.entropy) a.entropy[row] = none ? 0.f : ll - xs / (1.f + rest);
     if (a.stats) a.stats[2 * row] = ref, a.stats[2 * row + 1] = ll;
   }
   return ll;
+}
+__device__ __forceinline__ void write_alternative(const ScoreArgs& a, long row, int place, u64 k, float ref, float ll) {
+  a.ids[row * a.top + place] = key_index(k);
+  a.alt[row * a.top + place] = key_value(k) - ref - ll;
 }
 
 // One wave per row (NT = 64) or one workgroup per slice (NT = 256); a thread
@@ -115,8 +158,9 @@ template <typename T, int NT, int EV>
 __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   typedef Unit<T> U;
   constexpr int E = U::E, NU = EV / E, NW = NT / 64, GROUPS = 256 / NT;
-  __shared__ u64 s_key[256], s_cand[GROUPS][CAP], s_red[4], s_T[GROUPS];
-  __shared__ float s_sum[2][4];
+  __shared__ __attribute__((aligned(16))) float s_best[256];
+  __shared__ u64 s_cand[GROUPS][CAP], s_last[4];
+  __shared__ float s_max[4], s_sum[2][2][4], s_T[GROUPS];
   __shared__ int s_n[GROUPS];
   const int gt = threadIdx.x / NT, t = threadIdx.x % NT, lane = threadIdx.x & 63, w = t >> 6;
   auto sync = [] {
@@ -129,68 +173,55 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   const long row = NT == 64 ? g : g / a.slices;
   if (row >= a.rows) return;  // a whole wave, or nobody
   const int slice = NT == 64 ? 0 : (int)(g - row * a.slices);
-  const int base = slice * (NT * EV), end = min(a.V, base + NT * EV);
+  const int base = slice * (NT * EV), end = min(a.V, base + NT * EV), top = a.top;
   const T* x = (const T*)a.x + row * a.ldx;
+  auto index = [&](int i) { return base + E * (t + NT * (i / E)) + i % E; };
   U u[NU];
-  float f[EV];
 #pragma unroll
   for (int i = 0; i < NU; i++) {
     const int v = base + E * (t + NT * i);
     if (v + E <= end) u[i].r = *(const typename U::Raw*)(x + v);
   }
-  // the largest entry apart (the lowest index of it), the others in f
-  float best = -INFINITY;
-  int at = -1;
+  const Token tk = token_of<T>(a, row);
+  float f[EV], best = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NU; i++) {
     const int v = base + E * (t + NT * i);
     if (v + E <= end) {
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float y = u[i].get(e);
-        const bool up = y > best;
-        f[i * E + e] = up ? best : y;
-        at = up ? v + e : at;
-        best = up ? y : best;
-      }
+      for (int e = 0; e < E; e++) f[i * E + e] = u[i].get(e);
     } else {
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float y = v + e < end ? at_f32(x, v + e) : -INFINITY;
-        const bool up = y > best;
-        f[i * E + e] = up ? best : y;
-        at = up ? v + e : at;
-        best = up ? y : best;
-      }
+      for (int e = 0; e < E; e++) f[i * E + e] = v + e < end ? at_f32(x, v + e) : -INFINITY;
     }
   }
-  u64 key = 0;
-  if (at >= 0) {
-    key = order_key(best, at);
-  } else if (a.top) {  // nothing but -inf and NaN: the first of them in order
-#pragma unroll 1
-    for (int i = 0; i < EV; i++) {
-      const int v = base + E * (t + NT * (i / E)) + i % E;
-      if (v < end) {
-        const u64 k = order_key(at_f32(x, v), v);
-        key = k > key ? k : key;
-      }
-    }
-  }
-  u64 first = wave_max(key);
-  if (NT > 64) {
-    s_key[threadIdx.x] = key;
-    if (lane == 0) s_red[w] = first;
-    if (t == 0) s_n[0] = 0;
-    sync();
 #pragma unroll
-    for (int i = 0; i < NW; i++) first = s_red[i] > first ? s_red[i] : first;
-  } else if (t == 0) {
-    s_n[gt] = 0;
+  for (int i = 0; i < EV; i++) best = fmaxf(best, f[i]);
+  float m = all_max(best);
+  if (t == 0) s_n[gt] = 0;
+  if (NT > 64) {
+    s_best[threadIdx.x] = best;
+    if (lane == 0) s_max[w] = m;
+    sync();
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
   }
-  const float m = key_value(first), ref = m == -INFINITY ? 0.f : m;
-  // Two partial sums: the smallest entries of a thread's row of terms are the
-  // first (f holds what each new maximum displaced)
+  // the threshold, by the first wave of the group
+  if (w == 0 && top) {
+    float col = best;
+    if (NT > 64) col = fmaxf(fmaxf(best, s_best[lane + 64]), fmaxf(s_best[lane + 128], s_best[lane + 192]));
+    float* cols = s_best + (NT > 64 ? 0 : gt * 64);
+    cols[lane] = col;
+    sync_wave();
+    int larger = 0;
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {
+      const f32x4 c = *(const f32x4*)(cols + i);
+      larger += (c[0] > col) + (c[1] > col) + (c[2] > col) + (c[3] > col);
+    }
+    const float least = all_min(larger < top ? col : INFINITY);
+    if (lane == 0) s_T[gt] = least;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
   float rest = 0.f, xs = 0.f;
 #pragma unroll
   for (int i = 0; i < EV; i++) {
@@ -198,88 +229,102 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     rest += e;
     xs = fmaf(e, fmaxf(d, -1e30f), xs);  // a share of 0 has no entropy; a NaN is in e
   }
-  if (!(key == first && at >= 0)) {
-    const float d = best - ref, e = __builtin_amdgcn_exp2f(d * LOG2E);
-    rest += e;
-    xs = fmaf(e, fmaxf(d, -1e30f), xs);
-  }
-  rest = wave_sum(rest);
-  xs = wave_sum(xs);
-  const int top = a.top;
-  if (NT > 64) {
-    if (lane == 0) s_sum[0][w] = rest, s_sum[1][w] = xs;
-  }
-  // the threshold, by the first wave of the group
-  if (w == 0 && top) {
-    u64 col = key;
+  auto total = [&](float& r, float& y, int k) {
+    r = all_sum(r);
+    y = all_sum(y);
     if (NT > 64) {
-#pragma unroll
-      for (int i = 1; i < NW; i++) col = s_key[lane + 64 * i] > col ? s_key[lane + 64 * i] : col;
-    }
-    s_key[NT > 64 ? lane : threadIdx.x] = col;
-    sync_wave();
-    int larger = 0;
-    const u64* keys = s_key + (NT > 64 ? 0 : gt * 64);
-#pragma unroll 8
-    for (int i = 0; i < 64; i++) larger += keys[i] > col;
-    // fewer than `top` columns with an entry: everything counts
-    const u64 mask = __ballot(larger == top - 1 && col);
-    if (mask ? lane == __ffsll(mask) - 1 : lane == 0) s_T[gt] = mask ? col : 1;
-  }
-  sync();
-  if (NT > 64) {
-    rest = s_sum[0][0];
-    xs = s_sum[1][0];
-#pragma unroll
-    for (int i = 1; i < NW; i++) rest += s_sum[0][i], xs += s_sum[1][i];
-  }
-  float ll = 0.f, rref;
-  const bool whole = NT == 64 || a.slices == 1;
-  float* part = nullptr;
-  if (whole) {
-    ll = write_row<T>(a, row, m, rest, xs, rref, t == 0);
-  } else {
-    part = part_at(a, row, slice);
-    if (t == 0) part[0] = rest, part[1] = xs, *(u64*)(part + 2) = first;
-  }
-  if (!top) return;
-  auto put = [&](int place, u64 k) {
-    if (whole) {
-      a.ids[row * top + place] = key_index(k);
-      a.alt[row * top + place] = at_f32(x, key_index(k)) - rref - ll;
-    } else {
-      ((u64*)(part + 4))[place] = k;
+      if (lane == 0) s_sum[k][0][w] = r, s_sum[k][1][w] = y;
+      sync();
+      r = (s_sum[k][0][0] + s_sum[k][0][1]) + (s_sum[k][0][2] + s_sum[k][0][3]);
+      y = (s_sum[k][1][0] + s_sum[k][1][1]) + (s_sum[k][1][2] + s_sum[k][1][3]);
     }
   };
-  const u64 T0 = s_T[gt];
-  if (key >= T0) {
-#pragma unroll 1
-    for (int i = 0; i < NU; i++) {
-      const int v = base + E * (t + NT * i);
+  float l = rest, lx = xs;
+  total(l, lx, 0);
+  if (l < 2.f) {
+    int first = 0;
+    if (NT > 64) while (first < NW - 1 && s_max[first] != m) first++;
+    const u64 mask = __ballot(best == m);
+    if (w == first && mask && lane == __ffsll(mask) - 1) {
+      rest = xs = 0.f;
+      bool left = false;
+      float r = ref;
+      asm volatile("" : "+v"(r));  // or the terms above would be kept for here, in registers of their own
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        if (v + e >= end) break;
-        const u64 k = order_key(at_f32(x, v + e), v + e);
-        if (k >= T0) {
-          const int n = atomicAdd(&s_n[gt], 1);
-          if (n < CAP) s_cand[gt][n] = k;
-        }
+      for (int i = 0; i < EV; i++) {
+        const bool out = !left && f[i] == m;
+        left |= out;
+        const float d = f[i] - r, e = out ? 0.f : __builtin_amdgcn_exp2f(d * LOG2E);
+        rest += e;
+        xs = fmaf(e, fmaxf(d, -1e30f), xs);
       }
     }
+    total(rest, xs, 1);
+  } else {
+    rest = l - 1.f;
+    xs = lx;
+  }
+  const bool whole = NT == 64 || a.slices == 1;
+  float ll = 0.f, rref = 0.f;
+  if (whole) {
+    ll = write_row(a, row, m, rest, xs, tk, rref, t == 0);
+  } else if (t == 0) {
+    *(f32x4*)(part_sums(a, row) + 4 * slice) = f32x4{m, rest, xs, 0.f};
+  }
+  if (!top) return;
+  u64* list = whole ? nullptr : part_keys(a, row) + (long)slice * top;
+  auto put = [&](int place, u64 k) {
+    if (whole)
+      write_alternative(a, row, place, k, rref, ll);
+    else
+      list[place] = k;
+  };
+  sync();
+  const float T0 = s_T[gt];
+  if (best >= T0) {
+#pragma unroll
+    for (int i = 0; i < EV; i++)
+      if (f[i] >= T0 && index(i) < end) {
+        const int n = atomicAdd(&s_n[gt], 1);
+        if (n < CAP) s_cand[gt][n] = order_key(f[i], index(i));
+      }
   }
   sync();
-  const int n = s_n[gt];
-  if (n <= CAP) {
+  int n = s_n[gt];
+  const int held = min(top, end - base);  // a row's last slice may have fewer entries
+  if (n > CAP || n < held) {
+    // many entries equal to the threshold (a masked row's -inf): those above
+    // it, then the equal ones by windows of the index until there are enough
+    sync();
+    if (t == 0) s_n[gt] = 0;
+    sync();
+    auto collect = [&](int lo, int hi, bool equal) {
+      for (int v = lo + t; v < hi; v += NT) {
+        const float y = at_f32(x, v);
+        if (equal ? y == T0 : y > T0) {
+          const int k = atomicAdd(&s_n[gt], 1);
+          if (k < CAP) s_cand[gt][k] = order_key(y, v);
+        }
+      }
+      sync();
+      n = s_n[gt];
+      sync();
+    };
+    collect(base, end, false);
+    for (int lo = base; n < held && lo < end; lo += CAP / 4) collect(lo, min(lo + CAP / 4, end), true);
+  }
+  if (n <= CAP && n >= held) {
     for (int i = t; i < n; i += NT) {
       const u64 k = s_cand[gt][i];
       int place = 0;
       for (int c = 0; c < n; c++) place += s_cand[gt][c] > k;
       if (place < top) put(place, k);
     }
-    for (int i = n + t; i < top; i += NT) put(i, 0);  // a slice of fewer entries
+    for (int i = held + t; i < top; i += NT) put(i, 0);
     return;
   }
-  // more than LDS holds (no natural row): the largest below the last, `top` times
+  // more than LDS holds above the threshold, or fewer entries than asked for
+  // beside NaN: the largest below the last, `top` times (then none, key 0)
   u64 last = ~0ull;
   for (int j = 0; j < top; j++) {
     u64 k0 = 0;
@@ -290,88 +335,104 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     k0 = wave_max(k0);
     if (NT > 64) {
       sync();
-      if (lane == 0) s_red[w] = k0;
+      if (lane == 0) s_last[w] = k0;
       sync();
 #pragma unroll
-      for (int i = 0; i < NW; i++) k0 = s_red[i] > k0 ? s_red[i] : k0;
+      for (int i = 0; i < NW; i++) k0 = s_last[i] > k0 ? s_last[i] : k0;
     }
     last = k0;
     if (t == 0) put(j, k0);
   }
 }
 
-// The slices of a row, one wave per row: the sums relative to the row's
-// maximum (slice s holds e^(m_s - m) (1 + rest_s) of them), and the largest of
-// the slices' lists.
+// The slices of a row, one workgroup: the sums relative to the row's maximum
+// (slice s holds e^(m_s - m) (1 + rest_s) of them), and the largest of the
+// slices' lists.
+__device__ __forceinline__ u64 larger_of(u64 a, u64 b) { return a > b ? a : b; }
 template <typename T>
-__global__ __launch_bounds__(64) void k_score_join(ScoreArgs a) {
-  __shared__ u64 cand[CAP];
-  const int lane = threadIdx.x;
+__global__ __launch_bounds__(256) void k_score_join(ScoreArgs a) {
+  __shared__ u64 cand[CAP], s_key[4];
+  __shared__ float s_max[4], s_sum[2][4];
+  __shared__ int s_n, s_first;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   const long row = blockIdx.x;
-  const int S = a.slices, top = a.top;
-  u64 first = 0, T0 = 1;
-  for (int s = lane; s < S; s += 64) {
-    const u64* p = (const u64*)part_at(a, row, s);
-    first = p[1] > first ? p[1] : first;
-    if (top && p[1 + top] > T0) T0 = p[1 + top];  // a slice's last: `top` entries are as large
+  const int S = a.slices, top = a.top, all = S * top;
+  const f32x4* sums = (const f32x4*)part_sums(a, row);
+  const u64* keys = part_keys(a, row);
+  const Token tk = token_of<T>(a, row);
+  constexpr int HELD = 4;  // keys a thread keeps from the first look at them
+  u64 k[HELD], T0 = 1;
+#pragma unroll
+  for (int i = 0; i < HELD; i++) k[i] = t + 256 * i < all ? keys[t + 256 * i] : 0;
+  float m = -INFINITY;
+  for (int s = t; s < S; s += 256) {
+    m = fmaxf(m, sums[s][0]);
+    if (top) T0 = larger_of(T0, keys[(s + 1) * top - 1]);  // a slice's last: `top` entries are as large
   }
-  first = wave_max(first);
+  if (t == 0) s_n = 0, s_first = 0x7fffffff;
+  m = all_max(m);
   T0 = wave_max(T0);
-  const float m = key_value(first), ref0 = m == -INFINITY ? 0.f : m;
+  if (lane == 0) s_max[w] = m, s_key[w] = T0;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  T0 = larger_of(larger_of(s_key[0], s_key[1]), larger_of(s_key[2], s_key[3]));
+  for (int s = t; s < S; s += 256)
+    if (sums[s][0] == m) atomicMin(&s_first, s);  // the slice that leaves its maximum out
+  auto collect = [&](u64 key) {
+    if (key >= T0) {
+      const int n = atomicAdd(&s_n, 1);
+      if (n < CAP) cand[n] = key;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; i++) collect(k[i]);
+  for (int i = t + 256 * HELD; i < all; i += 256) collect(keys[i]);
+  __syncthreads();
+  const float ref0 = m == -INFINITY ? 0.f : m;
   float rest = 0.f, xs = 0.f;
-  for (int s = lane; s < S; s += 64) {
-    const float* p = part_at(a, row, s);
-    const u64 k = *(const u64*)(p + 2);
-    const float ms = key_value(k), r = p[0], y = p[1];
-    if (k == first || ms == -INFINITY) {  // without an entry of its own there is nothing to leave out
-      rest += r;
-      xs += y;
+  for (int s = t; s < S; s += 256) {
+    const f32x4 q = sums[s];
+    if (s == s_first || q[0] == -INFINITY) {  // without an entry of its own there is nothing to leave out
+      rest += q[1];
+      xs += q[2];
     } else {
-      const float d = ms - ref0, f = __builtin_amdgcn_exp2f(d * LOG2E);
-      rest += f * (1.f + r);
-      xs += f > 0.f ? f * fmaf(d, 1.f + r, y) : f;
+      const float d = q[0] - ref0, f = __builtin_amdgcn_exp2f(d * LOG2E);
+      rest += f * (1.f + q[1]);
+      xs += f > 0.f ? f * fmaf(d, 1.f + q[1], q[2]) : f;
     }
   }
-  rest = wave_sum(rest);
-  xs = wave_sum(xs);
+  rest = all_sum(rest);
+  xs = all_sum(xs);
+  if (lane == 0) s_sum[0][w] = rest, s_sum[1][w] = xs;
+  __syncthreads();
+  rest = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]);
+  xs = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
   float ref;
-  const float ll = write_row<T>(a, row, m, rest, xs, ref, lane == 0);
+  const float ll = write_row(a, row, m, rest, xs, tk, ref, t == 0);
   if (!top) return;
-  const T* x = (const T*)a.x + row * a.ldx;
-  auto put = [&](int place, u64 k) {
-    a.ids[row * top + place] = key_index(k);
-    a.alt[row * top + place] = at_f32(x, key_index(k)) - ref - ll;
-  };
-  int n = 0;
-  const int all = S * top;
-  for (int b = 0; b < all; b += 64) {
-    const int i = b + lane, s = i / top;
-    const u64 k = i < all ? ((const u64*)part_at(a, row, s))[2 + i - s * top] : 0;
-    const bool in = k >= T0;
-    const u64 mask = __ballot(in);
-    const int to = n + __popcll(mask & ((1ull << lane) - 1));
-    if (in && to < CAP) cand[to] = k;
-    n += __popcll(mask);
-  }
-  sync_wave();
+  const int n = s_n;
   if (n <= CAP) {
-    for (int i = lane; i < n; i += 64) {
-      const u64 k = cand[i];
+    for (int i = t; i < n; i += 256) {
+      const u64 key = cand[i];
       int place = 0;
-      for (int c = 0; c < n; c++) place += cand[c] > k;
-      if (place < top) put(place, k);
+      for (int c = 0; c < n; c++) place += cand[c] > key;
+      if (place < top) write_alternative(a, row, place, key, ref, ll);
     }
     return;
   }
   u64 last = ~0ull;
   for (int j = 0; j < top; j++) {
     u64 k0 = 0;
-    for (int i = lane; i < all; i += 64) {
-      const u64 k = ((const u64*)part_at(a, row, i / top))[2 + i % top];
-      if (k < last && k > k0) k0 = k;
+    for (int i = t; i < all; i += 256) {
+      const u64 key = keys[i];
+      if (key < last && key > k0) k0 = key;
     }
-    last = k0 = wave_max(k0);
-    if (lane == 0) put(j, k0);
+    k0 = wave_max(k0);
+    __syncthreads();
+    if (lane == 0) s_key[w] = k0;
+    __syncthreads();
+    last = k0 = larger_of(larger_of(s_key[0], s_key[1]), larger_of(s_key[2], s_key[3]));
+    if (t == 0) write_alternative(a, row, j, k0, ref, ll);
   }
 }
 
@@ -460,7 +521,7 @@ void launch_score(hipStream_t s, const ScoreArgs& a) {
     k_score<T, 256, 16><<<(unsigned)a.rows, 256, 0, s>>>(a);
   } else {
     k_score<T, 256, 32><<<(unsigned)(a.rows * a.slices), 256, 0, s>>>(a);
-    if (a.slices > 1) k_score_join<T><<<(unsigned)a.rows, 64, 0, s>>>(a);
+    if (a.slices > 1) k_score_join<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
   }
 }
 template <typename T>

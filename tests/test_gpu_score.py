@@ -276,6 +276,27 @@ def test_crowded_rows(V, top):
     check_forward(s.host(), x, np.array([1, 2]), top)
 
 
+def test_crowded_slices():
+    """Many slices of a long row with 63 large entries each, one fewer than the alternatives asked for."""
+    V = 40 * 8192 - 100
+    x = np.tile(np.random.default_rng(0).normal(0, 1, V), (2, 1))
+    for s in range(40):
+        x[:, s * 8192 + np.arange(63) * 120] += 30.0
+    x = G.O.round_to(x, "f32")
+    s = Score(x, "f32", np.array([5, V - 1]), 64)
+    s.forward()
+    check_forward(s.host(), x, np.array([5, V - 1]), 64)
+
+
+@pytest.mark.parametrize("V", [8193, 8200, 16390])
+def test_a_last_slice_of_few_entries(V):
+    x = logits(np.random.default_rng(V), 3, V, "f32")
+    x[1, -3:] = 99.0
+    s = Score(x, "f32", np.array([0, V - 1, 7]), 30)
+    s.forward()
+    check_forward(s.host(), x, np.array([0, V - 1, 7]), 30)
+
+
 @pytest.mark.parametrize("n,V", [(40, 257), (3, 60000)])
 def test_captured_scores_replay(n, V):
     """Forward and backward in one graph; new logits between the replays, every replay against the definitions."""
