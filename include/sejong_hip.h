@@ -138,7 +138,7 @@ int sj_rope_frequencies(void *stream, uint64_t *turns, long rotary_dim, const sj
  * is good to 2^-22 up to position 2^27.  x and y fp32 or bf16 (stored value in, fp32
  * products, one rounding); y may be x.  head_dim even, at most 1024; any
  * strides and element alignment (16-byte rows are fastest).  turns may be
- * null when rotary_dim is 0; at most 2^24 rows. */
+ * null when rotary_dim is 0; at most 2^24 rows and 2^14 heads. */
 #define SJ_ROPE_INTERLEAVED 0
 #define SJ_ROPE_HALF 1
 int sj_rope_rows(void *stream, const void *x, long ldx, void *y, long ldy, int dtype, long rows, long heads,
@@ -408,7 +408,8 @@ int sj_paged_plan(void *stream, const int32_t *lengths, const int32_t *counts, l
  * keys rotated and values copied into the cache rows of their slots; the
  * rotation as sj_rope_rows.  A row whose slot is not in 0 .. cache_slots - 1
  * is left out whole (q_out too).  The slots of one call are distinct.  q_out
- * may be q; hq may be 0.  Any strides and element alignment; at most 2^24 rows. */
+ * may be q; hq may be 0.  Any strides and element alignment; at most 2^24 rows, hq and hk
+ * at most 2^14. */
 int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, int dtype,
                     long rows, long hq, long hk, long head_dim, long rotary_dim, int layout, const int32_t *positions,
                     const int32_t *slots, const uint64_t *turns, float amplitude, void *q_out, long ldqo,

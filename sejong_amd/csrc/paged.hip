@@ -15,11 +15,13 @@ namespace {
 // Token S_r + j of request r (S = exclusive sum of the counts) has position
 // len_r + j; the pages that a request grows into are taken from the free list
 // in the order of the requests.  Every workgroup sums all the requests itself
-// (a few KB that stay in L2, one block scan) and expands 1024 tokens, so the
-// plan is one launch and needs no workspace: the bound is that launch, the
-// scan's latency and, for prompts, 12 bytes written per token.
+// (a few KB that stay in L2, one block scan) and expands 1024 tokens, four to
+// a thread, so the plan is one launch and needs no workspace: the bound is
+// that launch, the chain of loads lengths -> page ids, and, for prompts, the
+// 12 bytes written per token.
 
-constexpr int PT = 1024;  // threads, and tokens, of a workgroup
+constexpr int PT = 256;    // threads of a workgroup
+constexpr int PTOK = 1024; // its tokens
 
 struct PlanArgs {
   const int32_t *lengths, *counts, *free_pages, *head;
@@ -31,120 +33,173 @@ struct PlanArgs {
 
 __device__ __forceinline__ uint32_t ceil_div(uint32_t n, uint32_t d) { return n / d + (n % d != 0); }
 
+// inclusive scan over the wave: four steps within rows of 16 lanes, then the
+// rows' last values into the rows behind
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ uint32_t scan_add(uint32_t v) {
+  v += dpp_or0<0x111, 0xf>(v);  // from 1, 2, 4, 8 lanes before
+  v += dpp_or0<0x112, 0xf>(v);
+  v += dpp_or0<0x114, 0xf>(v);
+  v += dpp_or0<0x118, 0xf>(v);
+  v += dpp_or0<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  v += dpp_or0<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+  return v;
+}
+// of values >= 0
+__device__ __forceinline__ int scan_max(int v) {
+  v = max(v, dpp_or0<0x111, 0xf>(v));
+  v = max(v, dpp_or0<0x112, 0xf>(v));
+  v = max(v, dpp_or0<0x114, 0xf>(v));
+  v = max(v, dpp_or0<0x118, 0xf>(v));
+  v = max(v, dpp_or0<0x142, 0xa>(v));
+  v = max(v, dpp_or0<0x143, 0xc>(v));
+  return v;
+}
+
 __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
-  __shared__ long long w_tok[16], w_need[16];
-  __shared__ uint32_t w_want[16], w_long[16];
-  __shared__ int w_bad[16], w_at[16];
-  __shared__ int h_req[PT], h_start[PT], h_first[PT];
+  __shared__ uint32_t w_tok[4], w_need[4], w_want[4], w_long[4], w_bad[4];
+  __shared__ float w_size[4];
+  __shared__ int w_at[4];
+  // a request's marks lie where its tokens begin in this workgroup's range
+  __shared__ __attribute__((aligned(16))) int h_req[PTOK];
+  __shared__ int h_start[PTOK], h_len[PTOK], h_first[PTOK], h_tail[PTOK], h_fresh[PTOK];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.R + PT - 1) / PT;
   const int r0 = min(t * per, a.R), r1 = min(r0 + per, a.R);
-  long long tok = 0, need = 0;
-  uint32_t want = 0, longest = 0;
-  int bad = 0;
+  const int head = a.head ? a.head[0] : 0;
+  const int n0 = r0 < r1 ? a.lengths[r0] : 0, m0 = r0 < r1 ? a.counts[r0] : 0;
+  // 32-bit sums are exact wherever the sum of the counts, watched in fp32, is
+  // below 3e9: there are at most as many pages to take as tokens and requests
+  uint32_t tok = 0, need = 0, want = 0, longest = 0, bad = 0;
+  float size = 0.f;
 #pragma unroll 1
   for (int r = r0; r < r1; r++) {
-    const int n = a.lengths[r], m = a.counts[r];
+    const int n = r == r0 ? n0 : a.lengths[r], m = r == r0 ? m0 : a.counts[r];
     if ((n | m) < 0) {
       bad = 1;
     } else {
       const uint32_t w = ceil_div((uint32_t)n + (uint32_t)m, a.P);
       tok += m;
+      size += (float)m;
       need += w - ceil_div((uint32_t)n, a.P);
       want = max(want, w);
       longest = max(longest, (uint32_t)n + (uint32_t)m);
     }
   }
-  // inclusive sums over the wave, then over the 16 waves
-  long long st = tok, sn = need;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long u = __shfl_up(st, o, 64), v = __shfl_up(sn, o, 64);
-    if (lane >= o) st += u, sn += v;
-  }
+  uint32_t st = scan_add(tok), sn = scan_add(need);
   want = wave_max(want);
   longest = wave_max(longest);
+  size = wave_sum(size);
   bad = __any(bad);
-  if (lane == 63) w_tok[wave] = st, w_need[wave] = sn, w_want[wave] = want, w_long[wave] = longest, w_bad[wave] = bad;
-  h_req[t] = -1;
+  if (lane == 63) w_tok[wave] = st, w_need[wave] = sn;
+  if (lane == 0) w_want[wave] = want, w_long[wave] = longest, w_bad[wave] = bad, w_size[wave] = size;
+  *(int4*)(h_req + 4 * t) = make_int4(-1, -1, -1, -1);
   __syncthreads();
-  long long all_tok = 0, all_need = 0;
-  for (int i = 0; i < 16; i++) {
+  uint32_t all_tok = 0, all_need = 0;
+  size = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
     if (i < wave) st += w_tok[i], sn += w_need[i];
     all_tok += w_tok[i];
     all_need += w_need[i];
     want = max(want, w_want[i]);
     longest = max(longest, w_long[i]);
     bad |= w_bad[i];
+    size += w_size[i];
   }
-  const long long head = a.head ? a.head[0] : 0;
   int status = 0;
-  if (head < 0 || head + all_need > a.nfree) status |= SJ_PLAN_NO_PAGES;
-  if (want > (unsigned long long)a.ldt) status |= SJ_PLAN_TABLE_WIDTH;
-  if (all_tok > a.cap) status |= SJ_PLAN_ROWS;
+  const bool huge = size > 3e9f;
+  if (head < 0 || huge || (long)head + all_need > a.nfree) status |= SJ_PLAN_NO_PAGES;
+  if (want > (unsigned long)a.ldt) status |= SJ_PLAN_TABLE_WIDTH;
+  if (huge || all_tok > a.cap) status |= SJ_PLAN_ROWS;
   if (bad || longest > 0x7fffffffu) status |= SJ_PLAN_LENGTHS;
   const bool ok = status == 0;
 
-  // the requests again with their places: the first of a request's tokens in
-  // this workgroup's range marks where it begins
-  const long t0 = (long)blockIdx.x * PT;
-  long long s = st - tok, f = sn - need;
+  // the requests again with their places; a request's page ids are asked for
+  // at once: that of the page it is in and the first that it takes
+  const long t0 = (long)blockIdx.x * PTOK;
+  uint32_t s = st - tok, f = sn - need;
   const bool lead = blockIdx.x == 0;
 #pragma unroll 1
   for (int r = r0; r < r1; r++) {
-    const int n = a.lengths[r], m = a.counts[r];
+    const int n = r == r0 ? n0 : a.lengths[r], m = r == r0 ? m0 : a.counts[r];
     if (lead) {
       a.starts[r] = ok ? (int)s : 0;
       if (a.after) a.after[r] = ok ? n + m : n;
     }
     if (!ok) continue;
-    if (m > 0 && s < t0 + PT && s + m > t0) {
+    const uint32_t in = (uint32_t)n / a.P, have = ceil_div((uint32_t)n, a.P);
+    const uint32_t take = ceil_div((uint32_t)n + (uint32_t)m, a.P) - have;
+    if (m > 0 && s < t0 + PTOK && (long)s + m > t0) {
       const int at = s > t0 ? (int)(s - t0) : 0;
+      const int tail = in < have ? a.table[(long)r * a.ldt + in] : -1;
+      const int fresh = take ? a.free_pages[head + f] : -1;
       h_req[at] = r;
       h_start[at] = (int)s;
+      h_len[at] = n;
       h_first[at] = (int)f;
+      h_tail[at] = tail;
+      h_fresh[at] = fresh;
     }
     s += m;
-    f += ceil_div((uint32_t)n + (uint32_t)m, a.P) - ceil_div((uint32_t)n, a.P);
+    f += take;
   }
   if (lead && t == 0) {
     a.starts[a.R] = ok ? (int)all_tok : 0;
     a.summary[0] = ok ? (int)all_tok : 0;
-    a.summary[1] = (int)(head + (ok ? all_need : 0));
+    a.summary[1] = head + (ok ? (int)all_need : 0);
     a.summary[2] = status;
     a.summary[3] = longest > 0x7fffffffu ? 0x7fffffff : (int)longest;
   }
   __syncthreads();
-  // each token's request: the last mark at or before it
-  int at = h_req[t] >= 0 ? t : -1;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(at, o, 64);
-    if (lane >= o) at = max(at, u);
-  }
-  if (lane == 63) w_at[wave] = at;
+  // each token's request: the last mark at or before it (places from 1, 0: none)
+  const int4 marks = *(const int4*)(h_req + 4 * t);
+  int at[4];
+  at[0] = marks.x >= 0 ? 4 * t + 1 : 0;
+  at[1] = marks.y >= 0 ? 4 * t + 2 : at[0];
+  at[2] = marks.z >= 0 ? 4 * t + 3 : at[1];
+  at[3] = marks.w >= 0 ? 4 * t + 4 : at[2];
+  const int upto = scan_max(at[3]);
+  if (lane == 63) w_at[wave] = upto;
+  int before = __shfl_up(upto, 1, 64);
+  if (lane == 0) before = 0;
   __syncthreads();
-  for (int i = 0; i < wave; i++) at = max(at, w_at[i]);
-  const long g = t0 + t;
-  if (g >= a.cap) return;
-  int pos = -1, slot = -1, owner = -1;
-  if (ok && at >= 0 && g < all_tok) {
-    owner = h_req[at];
-    const int n = a.lengths[owner];
-    pos = n + (int)(g - h_start[at]);
-    const uint32_t col = (uint32_t)pos / a.P, off = (uint32_t)pos - col * a.P, have = ceil_div((uint32_t)n, a.P);
-    int page;
+#pragma unroll
+  for (int i = 0; i < 3; i++)
+    if (i < wave) before = max(before, w_at[i]);
+  int pos[4], slot[4], owner[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int h = max(at[i], before) - 1;
+    const long g = t0 + 4 * t + i;
+    pos[i] = slot[i] = owner[i] = -1;
+    if (!ok || h < 0 || g >= (long)all_tok || g >= a.cap) continue;
+    owner[i] = h_req[h];
+    const int n = h_len[h];
+    pos[i] = n + (int)(g - h_start[h]);
+    const uint32_t col = (uint32_t)pos[i] / a.P, off = (uint32_t)pos[i] - col * a.P, have = ceil_div((uint32_t)n, a.P);
+    int page = h_tail[h];
     if (col >= have) {
-      page = a.free_pages[head + h_first[at] + (col - have)];
-      if (off == 0) a.table[(long)owner * a.ldt + col] = page;  // a page's first position is always a new token here
-    } else {
-      page = a.table[(long)owner * a.ldt + col];
+      page = col == have ? h_fresh[h] : a.free_pages[(long)head + h_first[h] + (col - have)];
+      if (off == 0) a.table[(long)owner[i] * a.ldt + col] = page;  // a fresh page's first position is a new token
     }
-    if (page >= 0 && (uint32_t)page < a.pages) slot = (int)((uint32_t)page * a.P + off);
+    if (page >= 0 && (uint32_t)page < a.pages) slot[i] = (int)((uint32_t)page * a.P + off);
   }
-  a.positions[g] = pos;
-  a.slots[g] = slot;
-  a.owners[g] = owner;
+  const long g = t0 + 4 * t;
+  if (g + 4 <= a.cap && ((((uintptr_t)a.positions | (uintptr_t)a.slots | (uintptr_t)a.owners) & 15) == 0)) {
+    *(int4*)(a.positions + g) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    *(int4*)(a.slots + g) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    *(int4*)(a.owners + g) = make_int4(owner[0], owner[1], owner[2], owner[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (g + i < a.cap) {
+        a.positions[g + i] = pos[i];
+        a.slots[g + i] = slot[i];
+        a.owners[g + i] = owner[i];
+      }
+  }
 }
 
 // -------------------------------------------------------------- attention
@@ -792,7 +847,7 @@ extern "C" int sj_paged_plan(void* stream, const int32_t* lengths, const int32_t
   a.owners = owners; a.summary = summary;
   a.ldt = ldt; a.nfree = free_count; a.cap = capacity;
   a.R = (int)requests; a.P = (uint32_t)page_size; a.pages = (uint32_t)pages;
-  const long blocks = capacity > PT ? (capacity + PT - 1) / PT : 1;
+  const long blocks = capacity > PTOK ? (capacity + PTOK - 1) / PTOK : 1;
   k_paged_plan<<<(unsigned)blocks, PT, 0, (hipStream_t)stream>>>(a);
   SJ_LAUNCH_CHECK("paged plan");
   return SJ_OK;

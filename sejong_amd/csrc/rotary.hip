@@ -10,9 +10,10 @@
 // 64-bit fixed point: position * turns modulo 2^64 is the angle's fraction of
 // a turn with no further rounding (in fp32 the angle of position 2^20 is
 // already 0.06 off), for one integer multiply instead of a double multiply and
-// its range reduction.  A workgroup forms the cosines and sines
-// of its rows once in LDS (one pair per thread and turn), then all the heads
-// of those rows read them: the bound is the read and the write of the rows.
+// its range reduction.  A workgroup asks for all its elements first (up to four
+// units a thread), forms the cosines and sines of its rows once in LDS while
+// they come, and all the heads of those rows read them: the bound is the read
+// and the write of the rows.
 #include <math.h>
 
 #include "common.h"
@@ -22,7 +23,21 @@ using namespace sj;
 namespace {
 
 constexpr int RT = 256;
-constexpr int RPAIRS = 512;  // at most this many (row, pair) angles of a workgroup in LDS
+constexpr int RPAIRS = 1024;  // at most this many (row, pair) angles of a workgroup in LDS
+constexpr int RU = 4;         // units of a thread
+
+// n / d for n < 2^31 by multiplication: mul = floor(2^32 (2^shift - d) / d) + 1
+// with 2^shift >= d
+struct Div {
+  uint32_t mul, shift;
+};
+Div make_div(uint32_t d) {
+  Div r = {0, 0};
+  while ((1ul << r.shift) < d) r.shift++;
+  r.mul = (uint32_t)((((1ul << r.shift) - d) << 32) / d + 1);
+  return r;
+}
+__device__ __forceinline__ int div(int n, Div d) { return (int)((__umulhi(d.mul, (uint32_t)n) + (uint32_t)n) >> d.shift); }
 
 // one frequency per thread, in double
 __global__ void k_rope_frequencies(uint64_t* turns, int half, sj_rope_scaling s) {
@@ -68,6 +83,8 @@ struct RopeArgs {
   const uint64_t* turns;
   float amplitude, sign;
   int rb;  // rows of a workgroup
+  int rot_units, units, per_row;  // units of a head's rotated part, of a head, of a row
+  Div d_half, d_units, d_row;
 };
 
 // EL elements of T as they lie (element-aligned: the hardware takes
@@ -87,78 +104,78 @@ __device__ __forceinline__ void from_f(float v, bf16_t& o) { o = f2bf(v); }
 // one rounding to the storage type.
 template <typename T, int EL, bool HALF>
 __global__ __launch_bounds__(RT) void k_rope_rows(RopeArgs a) {
+  typedef Pack<T, EL> P;
   __shared__ float2 cs[RPAIRS];
-  const int t = threadIdx.x, half = a.half, D = a.D;
-  const int rot_units = HALF ? half / EL : 2 * half / EL;
-  const int units = rot_units + (D - 2 * half) / EL;
-  // blocks of rows, and within them blocks of pairs where a head has more
-  // than LDS holds (rb is 1 then, and half <= RPAIRS is checked on the host)
+  const int t = threadIdx.x, half = a.half;
+  // blocks of rows; where a row has more units than a workgroup takes, rb is 1
+  // and blockIdx.y counts its parts
   const long r0 = (long)blockIdx.x * a.rb;
   const int nr = (int)(a.rows - r0 < a.rb ? a.rows - r0 : a.rb);
+  const int total = nr * a.per_row, u0 = blockIdx.y * (RT * RU) + t;
+  P lo[RU], hi[RU];
+  T* y[RU];      // where the unit goes; null: nowhere
+  int pair[RU];  // its angles, -1: copied
+#pragma unroll
+  for (int j = 0; j < RU; j++) {
+    const int i = u0 + RT * j;
+    y[j] = nullptr;
+    pair[j] = -1;
+    if (i >= total) continue;
+    const int r = div(i, a.d_row), hu = i - r * a.per_row, head = div(hu, a.d_units), u = hu - head * a.units;
+    const long row = r0 + r;
+    RopeSeg sg = a.seg[0];
+    int h = head;
+    long dst = row;
+    if (a.nseg > 1) {  // q | k | v
+      const int sl = a.slots[row];
+      if (sl < 0 || sl >= a.nslots) continue;  // a padded row: nothing of it is written
+      if (h >= sg.heads) {
+        h -= sg.heads;
+        sg = a.seg[1];
+        if (h >= sg.heads) h -= sg.heads, sg = a.seg[2];
+        dst = sl;
+      }
+    }
+    const T* x = (const T*)sg.x + row * sg.ldx + (long)h * a.D;
+    const int o = !HALF || u < a.rot_units ? u * EL : 2 * half + (u - a.rot_units) * EL;
+    y[j] = (T*)sg.y + dst * sg.ldy + (long)h * a.D + o;
+    lo[j] = *(const P*)(x + o);
+    if (HALF && u < a.rot_units) hi[j] = *(const P*)(x + o + half);
+    if (u < a.rot_units) pair[j] = sg.rotate ? r * half + (HALF ? u * EL : u * (EL / 2)) : HALF ? -2 : -1;
+  }
   for (int i = t; i < nr * half; i += RT) {
-    const int r = i / half, p = i - r * half;
+    const int r = div(i, a.d_half), p = i - r * half;
     const uint64_t ph = (uint64_t)(int64_t)a.positions[r0 + r] * a.turns[p];
     float s, c;
     sincospif((float)(int32_t)(ph >> 32) * 4.656612873077393e-10f, &s, &c);  // half turns: 2^-31
     cs[i] = make_float2(c * a.amplitude, s * a.amplitude * a.sign);
   }
   __syncthreads();
-  const int per_row = a.heads * units;
-  for (int i = t + (int)blockIdx.y * RT; i < nr * per_row; i += RT * (int)gridDim.y) {
-    const int r = i / per_row, hu = i - r * per_row;
-    int h = hu / units;
-    const int u = hu - h * units;
-    const long row = r0 + r;
-    long dst = row;
-    if (a.slots) {
-      const int sl = a.slots[row];
-      if (sl < 0 || sl >= a.nslots) continue;  // a padded row: nothing of it is written
-      dst = sl;
-    }
-    RopeSeg sg = a.seg[0];
-    if (a.nseg > 1) {  // q | k | v
-      if (h >= a.seg[0].heads) {
-        h -= a.seg[0].heads;
-        sg = a.seg[1];
-        if (h >= sg.heads) h -= sg.heads, sg = a.seg[2];
-      }
-      if (!sg.slots) dst = row;
-    }
-    const T* x = (const T*)sg.x + row * sg.ldx + (long)h * D;
-    T* y = (T*)sg.y + dst * sg.ldy + (long)h * D;
-    typedef Pack<T, EL> P;
-    const float2* c = cs + r * half;
-    if (u >= rot_units || !sg.rotate) {
-      if (HALF && u < rot_units) {
-        const P lo = *(const P*)(x + u * EL), hi = *(const P*)(x + half + u * EL);
-        *(P*)(y + u * EL) = lo;
-        *(P*)(y + half + u * EL) = hi;
+#pragma unroll
+  for (int j = 0; j < RU; j++) {
+    if (!y[j]) continue;
+    if (pair[j] >= 0) {
+      const float2* c = cs + pair[j];
+      if constexpr (HALF) {
+#pragma unroll
+        for (int e = 0; e < EL; e++) {
+          const float va = to_f(lo[j].v[e]), vb = to_f(hi[j].v[e]);
+          const float2 q = c[e];
+          from_f(va * q.x - vb * q.y, lo[j].v[e]);
+          from_f(va * q.y + vb * q.x, hi[j].v[e]);
+        }
       } else {
-        const int o = HALF ? 2 * half + (u - rot_units) * EL : u * EL;
-        *(P*)(y + o) = *(const P*)(x + o);
-      }
-    } else if constexpr (HALF) {
-      P lo = *(const P*)(x + u * EL), hi = *(const P*)(x + half + u * EL);
 #pragma unroll
-      for (int e = 0; e < EL; e++) {
-        const float va = to_f(lo.v[e]), vb = to_f(hi.v[e]);
-        const float2 q = c[u * EL + e];
-        from_f(va * q.x - vb * q.y, lo.v[e]);
-        from_f(va * q.y + vb * q.x, hi.v[e]);
+        for (int e = 0; e < EL / 2; e++) {
+          const float va = to_f(lo[j].v[2 * e]), vb = to_f(lo[j].v[2 * e + 1]);
+          const float2 q = c[e];
+          from_f(va * q.x - vb * q.y, lo[j].v[2 * e]);
+          from_f(va * q.y + vb * q.x, lo[j].v[2 * e + 1]);
+        }
       }
-      *(P*)(y + u * EL) = lo;
-      *(P*)(y + half + u * EL) = hi;
-    } else {
-      P v = *(const P*)(x + u * EL);
-#pragma unroll
-      for (int e = 0; e < EL / 2; e++) {
-        const float va = to_f(v.v[2 * e]), vb = to_f(v.v[2 * e + 1]);
-        const float2 q = c[u * (EL / 2) + e];
-        from_f(va * q.x - vb * q.y, v.v[2 * e]);
-        from_f(va * q.y + vb * q.x, v.v[2 * e + 1]);
-      }
-      *(P*)(y + u * EL) = v;
     }
+    *(P*)y[j] = lo[j];
+    if (HALF && pair[j] != -1) *(P*)(y[j] + half) = hi[j];
   }
 }
 
@@ -175,11 +192,20 @@ int launch(hipStream_t s, RopeArgs& a, int dtype) {
   int el = width;  // the widest unit that divides the head, its rotated part and (half layout) each half
   const int part = a.layout == SJ_ROPE_HALF ? a.half : 2 * a.half;
   while (el > 1 && (a.D % el || part % el)) el >>= 1;
-  a.rb = a.half < RPAIRS ? (a.half ? RPAIRS / a.half : 8) : 1;
-  if (a.rb > 8) a.rb = 8;
-  // few rows: fewer of them to a workgroup, down to one, so that they reach more CUs
-  while (a.rb > 1 && (a.rows + a.rb - 1) / a.rb < 512) a.rb >>= 1;
-  const dim3 grid((unsigned)((a.rows + a.rb - 1) / a.rb), 1);
+  const int unit = a.layout == SJ_ROPE_HALF ? 2 * el : el;  // columns of a rotated unit
+  a.rot_units = 2 * a.half / unit;
+  a.units = a.rot_units + (a.D - 2 * a.half) / el;
+  a.per_row = a.heads * a.units;
+  // as many rows as a workgroup has units and angles for, but few enough that
+  // a short call reaches every CU
+  a.rb = RT * RU / a.per_row;
+  if (a.half && a.rb > RPAIRS / a.half) a.rb = RPAIRS / a.half;
+  while (a.rb > 1 && (a.rows + a.rb - 1) / a.rb < 512) a.rb = (a.rb + 1) / 2;
+  if (a.rb < 1) a.rb = 1;
+  a.d_half = make_div(a.half ? a.half : 1);
+  a.d_units = make_div(a.units);
+  a.d_row = make_div(a.per_row);
+  const dim3 grid((unsigned)((a.rows + a.rb - 1) / a.rb), (unsigned)(a.rb > 1 ? 1 : (a.per_row + RT * RU - 1) / (RT * RU)));
   if (dtype == SJ_BF16) {
     if (el == 8) launch_el<bf16_t, 8>(s, a, grid);
     else if (el == 4) launch_el<bf16_t, 4>(s, a, grid);
@@ -224,7 +250,7 @@ extern "C" int sj_rope_rows(void* stream, const void* x, long ldx, void* y, long
   SJ_REQUIRE(dtype == SJ_F32 || dtype == SJ_BF16, "rope rows dtype %d", dtype);
   SJ_REQUIRE(head_ok(head_dim, rotary_dim, layout), "rope rows: head width %ld, rotary width %ld, layout %d", head_dim,
              rotary_dim, layout);
-  SJ_REQUIRE(rows >= 0 && heads > 0 && heads <= 65536 && ldx >= heads * head_dim && ldy >= heads * head_dim,
+  SJ_REQUIRE(rows >= 0 && heads > 0 && heads <= 16384 && ldx >= heads * head_dim && ldy >= heads * head_dim,
              "rope rows dimensions");
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && y && positions && (turns || rotary_dim == 0), "rope rows: null");
@@ -251,7 +277,7 @@ extern "C" int sj_paged_append(void* stream, const void* q, long ldq, const void
   SJ_REQUIRE(dtype == SJ_F32 || dtype == SJ_BF16, "paged append dtype %d", dtype);
   SJ_REQUIRE(head_ok(head_dim, rotary_dim, layout), "paged append: head width %ld, rotary width %ld, layout %d",
              head_dim, rotary_dim, layout);
-  SJ_REQUIRE(rows >= 0 && hq >= 0 && hk > 0 && hq <= 65536 && hk <= 65536 && ldq >= hq * head_dim &&
+  SJ_REQUIRE(rows >= 0 && hq >= 0 && hk > 0 && hq <= 16384 && hk <= 16384 && ldq >= hq * head_dim &&
                  ldqo >= hq * head_dim && ldk >= hk * head_dim && ldv >= hk * head_dim && ldkv >= hk * head_dim &&
                  cache_slots >= 0,
              "paged append dimensions");

@@ -44,7 +44,8 @@ ROPE = dict(stream=None, x=X, ldx=128, y=X, ldy=128, dtype=N.SJ_BF16, rows=4, he
 
 @pytest.mark.parametrize("kw", [dict(dtype=N.SJ_F16), dict(dtype=N.SJ_F64), dict(head_dim=63), dict(rotary_dim=66),
                                 dict(rotary_dim=7), dict(rotary_dim=-2), dict(layout=2), dict(layout=-1), dict(rows=-1),
-                                dict(heads=0), dict(ldx=127), dict(ldy=127), dict(x=None), dict(y=None),
+                                dict(heads=0), dict(rows=2 ** 24 + 1),
+                                dict(heads=2 ** 14 + 1, ldx=2 ** 21, ldy=2 ** 21), dict(ldx=127), dict(ldy=127), dict(x=None), dict(y=None),
                                 dict(positions=None), dict(turns=None), dict(head_dim=1026, ldx=4096, ldy=4096)])
 def test_rope_refusals(kw):
     refused("sj_rope_rows", changed(ROPE, **kw), 1, b"rope rows")
@@ -101,7 +102,7 @@ ATTEND = dict(stream=None, q=X, ldq=256, k_cache=X, v_cache=X, ldkv=128, dtype=N
                                 dict(window=-1), dict(ldq=255), dict(ldo=255), dict(ldkv=127), dict(page_size=0),
                                 dict(pages=0), dict(pages=INT_MAX), dict(ldt=0), dict(ldt=INT_MAX), dict(q=None),
                                 dict(k_cache=None), dict(v_cache=None), dict(table=None), dict(positions=None),
-                                dict(o=None), dict(owners=None, rows=5)])
+                                dict(o=None), dict(owners=None, rows=5), dict(rows=2 ** 22 + 1)])
 def test_attention_refusals(kw):
     refused("sj_paged_attention", changed(ATTEND, **kw), 1, b"paged attention")
 
@@ -111,7 +112,8 @@ SCORE = dict(stream=None, x=X, dtype=N.SJ_F32, ldx=264, rows=4, vocab=257, token
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=N.SJ_F16), dict(rows=-1), dict(vocab=0), dict(ldx=256), dict(top=-1),
-                                dict(top=65), dict(vocab=3, top=4), dict(x=None), dict(tokens=None), dict(top_ids=None),
+                                dict(top=65), dict(vocab=3, top=4), dict(x=None), dict(rows=2 ** 24 + 1),
+                                dict(vocab=2 ** 24 + 1, ldx=2 ** 25), dict(vocab=100000, ldx=100000, rows=2 ** 21), dict(tokens=None), dict(top_ids=None),
                                 dict(top_logprob=None)])
 def test_score_refusals(kw):
     refused("sj_token_logprobs", changed(SCORE, **kw), 1, b"token log probabilities")
