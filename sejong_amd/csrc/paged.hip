@@ -288,7 +288,9 @@ template <typename T, int DC>
 struct Walk {
   static constexpr bool BF = sizeof(T) == 2;
   static constexpr int DP = 32 * DC, E = BF ? 8 : 4;
-  static constexpr int KT = BF ? (DC <= 2 ? 64 : 32) : (DC <= 2 ? 32 : 16), KS = KT / 16;
+  // 8 KB of keys a tile, and as much of values; wide heads by what the
+  // products take at least (32 keys in bf16, 16 in fp32)
+  static constexpr int KT = BF ? (DC == 1 ? 128 : DC == 2 ? 64 : 32) : (DC == 1 ? 64 : DC == 2 ? 32 : 16), KS = KT / 16;
   static constexpr int NC = DP / (4 * E);
   // fp32 V: a lane takes VW columns of a key, 16 lanes NV blocks of them
   static constexpr int VW = BF ? 1 : (DC == 1 ? 2 : 4), NV = BF ? 1 : DP / (16 * VW);
@@ -628,15 +630,12 @@ __global__ __launch_bounds__(256) void k_paged_stream(PagedArgs a) {
     if (i < per && r < a.rows && row_range(a, r, owner, lo, hi)) n[i] = (hi - lo + W::KT - 1) / W::KT;
     mine += n[i];
   }
-  int at = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(at, o, 64);
-    if (lane >= o) at += u;
-  }
+  int at = (int)scan_add((uint32_t)mine);
   if (lane == 63) ws[w] = at;
   __syncthreads();
-  for (int i = 0; i < w; i++) at += ws[i];
+#pragma unroll
+  for (int i = 0; i < 3; i++)
+    if (i < w) at += ws[i];
   at -= mine;
 #pragma unroll
   for (int i = 0; i < MOST; i++) {
@@ -662,14 +661,11 @@ __global__ __launch_bounds__(256) void k_paged_stream(PagedArgs a) {
   bf16_t* tile = (bf16_t*)(lds + w * W::LDS);
   W wk;
   while (x < e) {
-    // the row that holds tile x: the last whose tiles begin at or before it
-    int r0 = 0, r1 = a.rows;
+    // the row that holds tile x, the last whose tiles begin at or before it:
+    // counted by 32s, then within
     const int y = x / nb;
-    while (r1 - r0 > 1) {
-      const int mid = (r0 + r1) >> 1;
-      if (pre[mid] <= y) r0 = mid; else r1 = mid;
-    }
-    const int row = __builtin_amdgcn_readfirstlane(r0);
+    const int r32 = 32 * (__popcll(__ballot(32 * lane < a.rows && pre[min(32 * lane, a.rows)] <= y)) - 1);
+    const int row = r32 + __popcll(__ballot(lane < 32 && r32 + lane < a.rows && pre[min(r32 + lane, a.rows)] <= y)) - 1;
     const int first = __builtin_amdgcn_readfirstlane(pre[row]);
     const int nt = __builtin_amdgcn_readfirstlane(pre[row + 1]) - first;
     const int in = x - first * nb, hb = in / nt, t0 = in - hb * nt, t1 = min(nt, t0 + e - x);
@@ -709,42 +705,46 @@ __global__ __launch_bounds__(256) void k_paged_stream(PagedArgs a) {
 // i, in the order of the keys.  Threads own columns and share the partials.
 template <typename T>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
-  __shared__ float red[2][4];
   __shared__ f32x4 acc[256];
-  const int row = blockIdx.x, h = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
+  __shared__ float2 sums[256];
+  const int row = blockIdx.x, h = blockIdx.y, t = threadIdx.x;
   const int piece = a.plan[0], p0 = a.plan[1 + row], nt = a.plan[2 + row] - p0;
   if (nt == 0) return;
   const int kh = h / a.G, hg = h - kh * a.G, qt = hg >> 4, q = hg & 15, nb = a.HK * a.QT;
   const int x0 = p0 * nb + (kh * a.QT + qt) * nt, w0 = x0 / piece, w1 = (x0 + nt - 1) / piece, n = w1 - w0 + 1;
   if (n == 1) return;
-  auto slot = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0)) * a.slot; };
-  float M = -INFINITY;
-  for (int i = t; i < n; i += 256) M = fmaxf(M, slot(i)[q]);
-  M = wave_max(M);
-  if (lane == 0) red[0][w] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const int quads = a.D / 4, groups = 256 / quads, gr = t / quads, d = 4 * (t - gr * quads);
+  // one look at the partials, four at a time, with a running maximum per group
+  float M = -INFINITY, L = 0.f;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
+  auto scaled = [&](float m, float M) { return M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - M) * a.scale); };
+  auto add = [&](float m, float l, const f32x4& x) {
+    if (l == 0.f) return;  // no key with a share
+    const float mn = fmaxf(M, m), f0 = L == 0.f ? 0.f : scaled(M, mn), f1 = scaled(m, mn);
+    s = s * f0 + x * f1;
+    L = L * f0 + l * f1;
+    M = mn;
+  };
   if (gr < groups)
-    for (int i = gr; i < n; i += groups) {
-      const float* p = slot(i);
-      const float l = p[16 + q];
-      if (l == 0.f) continue;
-      const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((p[q] - M) * a.scale);
-      s += *(const f32x4*)(p + 32 + q * a.D + d) * f;
-      L += l * f;
+    for (int i = gr; i < n; i += 4 * groups) {
+      float m[4], l[4];
+      f32x4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int k = i + u * groups;
+        const float* p = a.part + (2L * (w0 + min(k, n - 1)) + (min(k, n - 1) == 0)) * a.slot;
+        m[u] = p[q];
+        l[u] = k < n ? p[16 + q] : 0.f;
+        x[u] = *(const f32x4*)(p + 32 + q * a.D + d);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) add(m[u], l[u], x[u]);
     }
   acc[t] = s;
-  __shared__ float ls[256];
-  ls[t] = L;
+  sums[t] = make_float2(M, L);
   __syncthreads();
   if (gr) return;
-  for (int i = 1; i < groups; i++) {
-    s += acc[i * quads + t];
-    L += ls[i * quads + t];
-  }
+  for (int i = 1; i < groups; i++) add(sums[i * quads + t].x, sums[i * quads + t].y, acc[i * quads + t]);
   put4((T*)a.o + (long)row * a.ldo + (long)h * a.D + d, s, L == 0.f ? 0.f : 1.f / L);
   if (a.lse && t == 0) a.lse[(long)row * a.HQ + h] = natural_lse(M, L, a.scale);
 }
