@@ -3,6 +3,10 @@
 // of the step's tokens over the pages (no counterpart in the reference, whose
 // cache holds one sequence: model lib.rs:36-50, architecture.rs:428-533).
 #include <math.h>
+#include <time.h>
+#include <unistd.h>
+
+#include <atomic>
 
 #include "common.h"
 
@@ -225,6 +229,13 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
 // The loads of a tile are in flight while the one before is computed, its page
 // ids one tile earlier still.
 
+// n / d for n < 2^31 by multiplication: mul = floor(2^32 (2^shift - d) / d) + 1
+// with 2^shift >= d; the added n is the 33rd bit of 2^32 + mul
+struct Div {
+  uint32_t mul, shift;
+};
+__device__ __forceinline__ int div(int n, Div d) { return (int)((__umulhi(d.mul, (uint32_t)n) + (uint32_t)n) >> d.shift); }
+
 struct PagedArgs {
   const void* q;
   long ldq;
@@ -238,14 +249,15 @@ struct PagedArgs {
   float* lse;
   int requests, rows, HQ, HK, D;
   int pages, P;
-  uint32_t pmul, pshift;  // division by P (page_col)
+  Div d_page, d_heads, d_tiles, d_quads;  // by P, by HK QT, by QT, by D / 4
   long window;
   float scale;  // log2(e) / sqrt(D): the softmax in powers of two
   int G, QT;    // query heads of a KV head, and their tiles of 16
   // split walks
-  float* part;    // [2 * waves][slot]
-  int32_t* plan;  // tiles of a wave, then the rows' exclusive tile counts
-  int slot;       // floats of a partial: 16 maxima, 16 sums, min(G, 16) rows of D
+  unsigned long long* flag;  // [2 * workgroups]: mark where a part's totals are complete
+  unsigned long long mark;
+  float* part;  // [2 * workgroups][slot]
+  int slot;     // floats of a walk's totals: 16 maxima and sums of shares, min(G, 16) rows of D
 };
 
 // the keys a row sees, [lo, hi), and its request; false for a padded row
@@ -260,15 +272,12 @@ __device__ __forceinline__ bool row_range(const PagedArgs& a, int row, int& owne
   return true;
 }
 
-// n / P for n < 2^31: the multiplier is floor(2^32 (2^shift - P) / P) + 1
-// with 2^shift >= P, and the 33rd bit of 2^32 + multiplier is the added n
-__device__ __forceinline__ int page_col(const PagedArgs& a, int n) {
-  return (int)((__umulhi(a.pmul, (uint32_t)n) + (uint32_t)n) >> a.pshift);
-}
-
 // 16 bytes at any alignment
 struct __attribute__((packed, aligned(2))) Raw16 {
   u32x4 v;
+};
+struct __attribute__((packed, aligned(2))) Raw8 {
+  u32x2 v;
 };
 __device__ __forceinline__ u32x4 load16(const void* p) { return ((const Raw16*)p)->v; }
 
@@ -306,6 +315,7 @@ struct Walk {
   f32x4 o[NO];
   float m, l;
   int pid[KS], sl[KS];
+  uint32_t absent;  // fp32: of the lane's V keys (4g + i of each 16), those without a slot
 
   __device__ __forceinline__ void start(const PagedArgs& a, int row, int kh, int qt, int lane) {
     const int col = lane & 15, g = lane >> 4, h = qt * 16 + col;
@@ -325,7 +335,7 @@ struct Walk {
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       const int j = base + 16 * s + (lane & 15);
-      pid[s] = j < hi ? pages[page_col(a, j)] : -1;
+      pid[s] = j < hi ? pages[div(j, a.d_page)] : -1;
     }
   }
   __device__ __forceinline__ void place(const PagedArgs& a, int base, int lane) {
@@ -333,7 +343,7 @@ struct Walk {
     for (int s = 0; s < KS; s++) {
       const int j = base + 16 * s + (lane & 15);
       const bool in = (uint32_t)pid[s] < (uint32_t)a.pages;
-      sl[s] = in ? pid[s] * a.P + (j - page_col(a, j) * a.P) : -1;
+      sl[s] = in ? pid[s] * a.P + (j - div(j, a.d_page) * a.P) : -1;
     }
   }
   // a key without a slot reads slot 0 and is masked in scores() and store_v()
@@ -372,13 +382,11 @@ struct Walk {
             for (int b = 0; b < NV; b++) {
               const int d = 64 * b + 4 * (lane & 15);
               v[4 * s + i][b] = load16(x + (d < a.D ? d : 0));
-              if (slot < 0) v[4 * s + i][b] = u32x4{0u, 0u, 0u, 0u};
             }
           } else {
             const int d = 2 * (lane & 15);
-            const uint32_t* y = (const uint32_t*)(x + (d < a.D ? d : 0));
-            const uint32_t y0 = y[0], y1 = y[1];
-            v[4 * s + i][0] = slot < 0 ? u32x4{0u, 0u, 0u, 0u} : u32x4{y0, y1, 0u, 0u};
+            const u32x2 y = ((const Raw8*)(x + (d < a.D ? d : 0)))->v;
+            v[4 * s + i][0] = u32x4{y[0], y[1], 0u, 0u};
           }
         }
       }
@@ -387,6 +395,7 @@ struct Walk {
   // S^T of the tile, the running maximum, and P in place of S
   __device__ __forceinline__ void scores(const PagedArgs& a, f32x4 (&p)[KS], int lane) {
     const int g = lane >> 4;
+    absent = 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -405,6 +414,7 @@ struct Walk {
       }
       const uint64_t good = __ballot(sl[s] >= 0);
       if ((good & 0xffffu) != 0xffffu) {
+        absent |= ((uint32_t)(~good >> (4 * g)) & 15u) << (4 * s);
 #pragma unroll
         for (int i = 0; i < 4; i++)
           if (!((good >> (4 * g + i)) & 1)) acc[i] = -INFINITY;
@@ -477,6 +487,13 @@ struct Walk {
         }
       }
     } else {
+      if (__any(absent)) {  // whatever such a slot holds, it counts 0 times 0
+#pragma unroll
+        for (int i = 0; i < 4 * KS; i++)
+          if ((absent >> i) & 1)
+#pragma unroll
+            for (int b = 0; b < NV; b++) v[i][b] = u32x4{0u, 0u, 0u, 0u};
+      }
 #pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -559,26 +576,19 @@ __device__ __forceinline__ void put4(T* y, const f32x4& x, float inv) {
   }
 }
 
-// One workgroup per row, KV head and tile of 16 query heads: its waves take
-// the key tiles in turn and join in LDS.  For walks that are short, or rows
-// that are many.
 constexpr int direct_waves(int dc) { return dc == 8 ? 4 : 8; }  // 256 registers a lane at most hold 8
+
+// The waves of a workgroup join what each summed of one walk: rows of sums in
+// each wave's LDS part, maxima and sums of shares beside.  NW: as many waves
+// as there can be, nw of them here.
+struct Shares {
+  float m[8][16], l[8][16];
+};
 template <typename T, int DC>
-__global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArgs a) {
+__device__ __forceinline__ void leave(const Walk<T, DC>& wk, Shares& sh, uint8_t* lds, int n, int w, int lane) {
   typedef Walk<T, DC> W;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ float wm[8][16], wl[8][16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int nb = a.HK * a.QT, row = blockIdx.x / nb, hb = blockIdx.x - row * nb, kh = hb / a.QT, qt = hb - kh * a.QT;
-  int owner, lo, hi;
-  if (!row_range(a, row, owner, lo, hi)) return;
-  W wk;
-  wk.start(a, row, kh, qt, lane);
-  const int tiles = (hi - lo + W::KT - 1) / W::KT;
-  bf16_t* tile = (bf16_t*)(lds + w * W::LDS);
-  wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, w, tiles, nw, tile, lane);
-  const int q = lane & 15, n = min(16, a.G - qt * 16);
-  if (lane < 16) wm[w][lane] = wk.m, wl[w][lane] = wk.l;
+  const int q = lane & 15;
+  if (lane < 16) sh.m[w][lane] = wk.m, sh.l[w][lane] = wk.l;
   float* mine = (float*)(lds + w * W::LDS);
 #pragma unroll
   for (int i = 0; i < W::QUADS; i++) {
@@ -586,38 +596,106 @@ __global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArg
     const int d = wk.quad(i, lane, x);
     if (q < n) *(f32x4*)(mine + q * W::DP + d) = x;
   }
+}
+// running totals of one query: the largest maximum M, the sum of shares L and
+// four columns s relative to it
+struct Total {
+  float M = -INFINITY, L = 0.f;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float m, float l, const f32x4& x, float scale) {
+    if (l == 0.f) return;  // no key with a share
+    // with NaN scores alone there is no maximum: the NaN is in l and x
+    const float mn = fmaxf(M, m), f0 = L == 0.f ? 0.f : mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((M - mn) * scale);
+    const float f1 = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * scale);
+    s = s * f0 + x * f1;
+    L = L * f0 + l * f1;
+    M = mn;
+  }
+};
+template <typename T, int DC, int NW>
+__device__ __forceinline__ Total joined(const PagedArgs& a, const Shares& sh, const uint8_t* lds, int nw, int r, int d) {
+  typedef Walk<T, DC> W;
+  float m[NW], l[NW];
+  f32x4 x[NW];
+#pragma unroll
+  for (int i = 0; i < NW; i++) {
+    const int k = i < nw ? i : 0;
+    m[i] = sh.m[k][r];
+    l[i] = i < nw ? sh.l[k][r] : 0.f;
+    x[i] = *(const f32x4*)((const float*)(lds + k * W::LDS) + r * W::DP + d);
+  }
+  Total t;
+#pragma unroll
+  for (int i = 0; i < NW; i++) t.add(m[i], l[i], x[i], a.scale);
+  return t;
+}
+template <typename T>
+__device__ __forceinline__ void put_result(const PagedArgs& a, int row, int h, int d, const Total& t) {
+  put4((T*)a.o + (long)row * a.ldo + (long)h * a.D + d, t.s, t.L == 0.f ? 0.f : 1.f / t.L);
+  if (a.lse && d == 0) a.lse[(long)row * a.HQ + h] = natural_lse(t.M, t.L, a.scale);
+}
+
+// One workgroup per row, KV head and tile of 16 query heads: its waves take
+// the key tiles in turn.  For walks that are short, and rows that are many.
+template <typename T, int DC>
+__global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArgs a) {
+  typedef Walk<T, DC> W;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ Shares sh;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int nb = a.HK * a.QT, row = div(blockIdx.x, a.d_heads), hb = blockIdx.x - row * nb;
+  const int kh = div(hb, a.d_tiles), qt = hb - kh * a.QT;
+  int owner, lo, hi;
+  if (!row_range(a, row, owner, lo, hi)) return;
+  W wk;
+  wk.start(a, row, kh, qt, lane);
+  const int tiles = (hi - lo + W::KT - 1) / W::KT, n = min(16, a.G - qt * 16);
+  wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, w, tiles, nw, (bf16_t*)(lds + w * W::LDS), lane);
+  leave(wk, sh, lds, n, w, lane);
   __syncthreads();
   const int quads = a.D / 4;
   for (int u = threadIdx.x; u < n * quads; u += blockDim.x) {
-    const int r = u / quads, d = 4 * (u - r * quads);
-    float M = -INFINITY, L = 0.f;
-    for (int i = 0; i < nw; i++) M = fmaxf(M, wm[i][r]);
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < nw; i++) {
-      const float li = wl[i][r];
-      if (li == 0.f) continue;
-      const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((wm[i][r] - M) * a.scale);
-      L += li * f;
-      s += *(const f32x4*)((const float*)(lds + i * W::LDS) + r * W::DP + d) * f;
-    }
-    const long h = (long)kh * a.G + qt * 16 + r;
-    put4((T*)a.o + (long)row * a.ldo + h * a.D + d, s, L == 0.f ? 0.f : 1.f / L);
-    if (a.lse && d == 0) a.lse[(long)row * a.HQ + h] = natural_lse(M, L, a.scale);
+    const int r = div(u, a.d_quads), d = 4 * (u - r * quads);
+    put_result<T>(a, row, kh * a.G + qt * 16 + r, d, joined<T, DC, direct_waves(DC)>(a, sh, lds, nw, r, d));
   }
 }
 
-// Long walks, or few: all the tiles of all rows and heads in one line, and
-// every wave an equal piece of it, whatever the rows' lengths.  A piece that
-// holds a whole walk writes its result; a walk that is cut leaves partial
-// maxima, sums and rows, which k_paged_join joins in the order of the keys.
-// A wave has at most two of them: the end of one walk and the beginning of
-// another.  Each workgroup sums the rows' tiles itself (one block scan).
+// Walks of any lengths: the tiles of all rows and heads in one line, four by
+// four (one per wave), and every workgroup an equal piece of the line.  Each
+// workgroup sums the rows' tiles itself (one block scan).  A walk that lies in
+// one piece is written as it is; of a walk that is cut, each workgroup leaves
+// its totals in the workspace, and the one that counts last joins them in the
+// order of the keys.  A workgroup has at most two cut walks, the end of one
+// and the beginning of another.
+//
+// Totals pass between workgroups (on different XCDs, each with its own L2)
+// through relaxed atomics at agent scope, which are coherent by themselves.
+// A part's totals are complete (vmcnt 0) before its flag is set, and its flag
+// (vmcnt 0 again) before it looks at the flags of the walk's other parts; so
+// the part whose flag is set last finds all of them.  Two parts may both find
+// them: they write the same bits.  Nobody waits for anybody.  The workspace is
+// the caller's and not cleared, so a set flag is a number of 64 bits that no
+// other call has; whoever finds all flags clears them, and a replayed graph,
+// which keeps its number, starts from cleared flags again.
 constexpr int STREAM_ROWS = 2048;
+// workgroups: as many as 256 CUs hold at once (by registers), at most 768
+constexpr int split_per_cu(int dc) { return dc == 8 ? 1 : dc == 2 || dc == 3 ? 3 : 2; }
+constexpr int STREAM_GROUPS = 1024;
+
+__device__ __forceinline__ void share_put(float* p, float x, float y) {
+  __hip_atomic_store((unsigned long long*)p, ((unsigned long long)__float_as_uint(y) << 32) | __float_as_uint(x),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 share_get(const float* p) {
+  const unsigned long long v = __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
 template <typename T, int DC>
-__global__ __launch_bounds__(256) void k_paged_stream(PagedArgs a) {
+__global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs a) {
   typedef Walk<T, DC> W;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ int pre[STREAM_ROWS + 1], ws[4];
+  __shared__ Shares sh;
+  __shared__ int pre[STREAM_ROWS + 1], ws[4], complete;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, nb = a.HK * a.QT;
   constexpr int MOST = STREAM_ROWS / 256;
   const int per = (a.rows + 255) / 256;
@@ -627,7 +705,7 @@ __global__ __launch_bounds__(256) void k_paged_stream(PagedArgs a) {
     n[i] = 0;
     const int r = t * per + i;
     int owner, lo, hi;
-    if (i < per && r < a.rows && row_range(a, r, owner, lo, hi)) n[i] = (hi - lo + W::KT - 1) / W::KT;
+    if (i < per && r < a.rows && row_range(a, r, owner, lo, hi)) n[i] = (hi - lo + 4 * W::KT - 1) / (4 * W::KT);
     mine += n[i];
   }
   int at = (int)scan_add((uint32_t)mine);
@@ -642,111 +720,111 @@ __global__ __launch_bounds__(256) void k_paged_stream(PagedArgs a) {
     const int r = t * per + i;
     if (i < per && r < a.rows) {
       pre[r] = at;
-      if (blockIdx.x == 0) a.plan[1 + r] = at;
       at += n[i];
     }
   }
   const int all = ws[0] + ws[1] + ws[2] + ws[3];
-  const int total = all * nb, waves = gridDim.x * 4;
-  const int piece = max(1, (int)(((long)total + waves - 1) / waves));
-  if (t == 0) {
-    pre[a.rows] = all;
-    if (blockIdx.x == 0) a.plan[0] = piece, a.plan[1 + a.rows] = all;
-  }
+  const int total = all * nb, piece = (int)(((long)total + gridDim.x - 1) / gridDim.x);
+  if (t == 0) pre[a.rows] = all;
   __syncthreads();
-  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + w);
-  if ((long)wave * piece >= total) return;
-  int x = wave * piece;
+  if ((long)blockIdx.x * piece >= total) return;
+  int x = blockIdx.x * piece;
   const int e = (int)min((long)total, (long)x + piece);
-  bf16_t* tile = (bf16_t*)(lds + w * W::LDS);
   W wk;
   while (x < e) {
-    // the row that holds tile x, the last whose tiles begin at or before it:
-    // counted by 32s, then within
-    const int y = x / nb;
+    // the row that holds place x, the last whose places begin at or before
+    // it: counted by 32s, then within
+    const int y = div(x, a.d_heads);
     const int r32 = 32 * (__popcll(__ballot(32 * lane < a.rows && pre[min(32 * lane, a.rows)] <= y)) - 1);
     const int row = r32 + __popcll(__ballot(lane < 32 && r32 + lane < a.rows && pre[min(r32 + lane, a.rows)] <= y)) - 1;
     const int first = __builtin_amdgcn_readfirstlane(pre[row]);
-    const int nt = __builtin_amdgcn_readfirstlane(pre[row + 1]) - first;
-    const int in = x - first * nb, hb = in / nt, t0 = in - hb * nt, t1 = min(nt, t0 + e - x);
-    const int kh = hb / a.QT, qt = hb - kh * a.QT;
+    const int places = __builtin_amdgcn_readfirstlane(pre[row + 1]) - first;
+    // the walk of the row's: fewer than 2^16, so the fp32 quotient is off by
+    // one at most
+    const int in = x - first * nb;
+    int hb = (int)((float)in * __builtin_amdgcn_rcpf((float)places));
+    hb -= in - hb * places < 0;
+    hb += in - hb * places >= places;
+    const int c0 = in - hb * places, c1 = min(places, c0 + e - x);
+    const int kh = div(hb, a.d_tiles), qt = hb - kh * a.QT, nq = min(16, a.G - qt * 16);
     int owner, lo, hi;
     row_range(a, row, owner, lo, hi);
     owner = __builtin_amdgcn_readfirstlane(owner);
     wk.start(a, row, kh, qt, lane);
-    wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, t0, t1, 1, tile, lane);
-    const int q = lane & 15, nq = min(16, a.G - qt * 16);
-    if (t0 == 0 && t1 == nt) {
-      const long h = (long)kh * a.G + qt * 16 + q;
-      T* y = (T*)a.o + (long)row * a.ldo + h * a.D;
-      const float inv = wk.l == 0.f ? 0.f : 1.f / wk.l;
-#pragma unroll
-      for (int i = 0; i < W::QUADS; i++) {
-        f32x4 v;
-        const int d = wk.quad(i, lane, v);
-        if (q < nq && d < a.D) put4(y + d, v, inv);
+    wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, 4 * c0 + w, min(4 * c1, (hi - lo + W::KT - 1) / W::KT), 4,
+           (bf16_t*)(lds + w * W::LDS), lane);
+    leave(wk, sh, lds, nq, w, lane);
+    __syncthreads();
+    const int quads = a.D / 4, items = nq * quads, h0 = kh * a.G + qt * 16;
+    if (c0 == 0 && c1 == places) {
+      for (int u = t; u < items; u += 256) {
+        const int r = div(u, a.d_quads), d = 4 * (u - r * quads);
+        put_result<T>(a, row, h0 + r, d, joined<T, DC, 4>(a, sh, lds, 4, r, d));
       }
-      if (a.lse && lane < nq) a.lse[(long)row * a.HQ + h] = natural_lse(wk.m, wk.l, a.scale);
     } else {
-      float* s = a.part + ((long)2 * wave + (t0 == 0)) * a.slot;
-      if (lane < 16) s[lane] = wk.m, s[16 + lane] = wk.l;
+      // part i of the walk is workgroup g0 + i's
+      const int x0 = x - c0, g0 = x0 / piece, parts = (x0 + places - 1) / piece - g0 + 1;
+      auto slot = [&](int i) { return a.part + (2L * (g0 + i) + (i == 0)) * a.slot; };
+      float* s = slot(blockIdx.x - g0);
+      for (int u = t; u < items; u += 256) {
+        const int r = div(u, a.d_quads), q = u - r * quads;
+        const Total v = joined<T, DC, 4>(a, sh, lds, 4, r, 4 * q);
+        if (q == 0) share_put(s + 2 * r, v.M, v.L);
+        share_put(s + 32 + 2 * u, v.s[0], v.s[1]);
+        share_put(s + 32 + 2 * (items + u), v.s[2], v.s[3]);
+      }
+      auto flag = [&](int i) { return a.flag + 2L * (g0 + i) + (i == 0); };
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (w == 0) {
+        if (lane == 0) __hip_atomic_store(flag(blockIdx.x - g0), a.mark, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        bool set = true;
+        for (int i = lane; i < parts; i += 64)
+          set &= __hip_atomic_load(flag(i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.mark;
+        set = __all(set);
+        if (lane == 0) complete = set;
+      }
+      __syncthreads();
+      if (complete) {
+        for (int i = t; i < parts; i += 256)
+          __hip_atomic_store(flag(i), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // fewer items than threads: groups of threads share the parts, and
+        // join through LDS
+        const int span = min(items, 256), groups = 256 / span, gr = t / span;
+        f32x4* acc = (f32x4*)lds;             // [256], then their maxima and shares: within the first two waves' parts
+        float2* ml = (float2*)(lds + 256 * 16);
+        for (int u0 = 0; u0 < items; u0 += span) {
+          const int u = u0 + t - gr * span, r = div(u, a.d_quads), q = u - r * quads;
+          const bool live = gr < groups && u < items;
+          Total v;
+          constexpr int MANY = 8;  // parts asked for at once
+          for (int i = gr; live && i < parts; i += MANY * groups) {
+            float2 m[MANY], p0[MANY], p1[MANY];
 #pragma unroll
-      for (int i = 0; i < W::QUADS; i++) {
-        f32x4 v;
-        const int d = wk.quad(i, lane, v);
-        if (q < nq && d < a.D) *(f32x4*)(s + 32 + q * a.D + d) = v;
+            for (int k = 0; k < MANY; k++) {
+              const float* p = slot(min(i + k * groups, parts - 1));
+              m[k] = share_get(p + 2 * r);
+              p0[k] = share_get(p + 32 + 2 * u);
+              p1[k] = share_get(p + 32 + 2 * (items + u));
+            }
+#pragma unroll
+            for (int k = 0; k < MANY; k++)
+              v.add(m[k].x, i + k * groups < parts ? m[k].y : 0.f, f32x4{p0[k].x, p0[k].y, p1[k].x, p1[k].y}, a.scale);
+          }
+          if (groups > 1) {
+            acc[t] = v.s;
+            ml[t] = make_float2(v.M, v.L);
+            __syncthreads();
+            for (int i = 1; gr == 0 && i < groups; i++) v.add(ml[t + i * span].x, ml[t + i * span].y, acc[t + i * span], a.scale);
+          }
+          if (live && gr == 0) put_result<T>(a, row, h0 + r, 4 * q, v);
+        }
       }
     }
-    x += t1 - t0;
+    __syncthreads();  // the next walk's waves write where this one was read
+    x += c1 - c0;
   }
-}
-
-// The cut walks of one row and query head: partial i is that of wave first +
-// i, in the order of the keys.  Threads own columns and share the partials.
-template <typename T>
-__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
-  __shared__ f32x4 acc[256];
-  __shared__ float2 sums[256];
-  const int row = blockIdx.x, h = blockIdx.y, t = threadIdx.x;
-  const int piece = a.plan[0], p0 = a.plan[1 + row], nt = a.plan[2 + row] - p0;
-  if (nt == 0) return;
-  const int kh = h / a.G, hg = h - kh * a.G, qt = hg >> 4, q = hg & 15, nb = a.HK * a.QT;
-  const int x0 = p0 * nb + (kh * a.QT + qt) * nt, w0 = x0 / piece, w1 = (x0 + nt - 1) / piece, n = w1 - w0 + 1;
-  if (n == 1) return;
-  const int quads = a.D / 4, groups = 256 / quads, gr = t / quads, d = 4 * (t - gr * quads);
-  // one look at the partials, four at a time, with a running maximum per group
-  float M = -INFINITY, L = 0.f;
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  auto scaled = [&](float m, float M) { return M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - M) * a.scale); };
-  auto add = [&](float m, float l, const f32x4& x) {
-    if (l == 0.f) return;  // no key with a share
-    const float mn = fmaxf(M, m), f0 = L == 0.f ? 0.f : scaled(M, mn), f1 = scaled(m, mn);
-    s = s * f0 + x * f1;
-    L = L * f0 + l * f1;
-    M = mn;
-  };
-  if (gr < groups)
-    for (int i = gr; i < n; i += 4 * groups) {
-      float m[4], l[4];
-      f32x4 x[4];
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const int k = i + u * groups;
-        const float* p = a.part + (2L * (w0 + min(k, n - 1)) + (min(k, n - 1) == 0)) * a.slot;
-        m[u] = p[q];
-        l[u] = k < n ? p[16 + q] : 0.f;
-        x[u] = *(const f32x4*)(p + 32 + q * a.D + d);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; u++) add(m[u], l[u], x[u]);
-    }
-  acc[t] = s;
-  sums[t] = make_float2(M, L);
-  __syncthreads();
-  if (gr) return;
-  for (int i = 1; i < groups; i++) add(sums[i * quads + t].x, sums[i * quads + t].y, acc[i * quads + t]);
-  put4((T*)a.o + (long)row * a.ldo + (long)h * a.D + d, s, L == 0.f ? 0.f : 1.f / L);
-  if (a.lse && t == 0) a.lse[(long)row * a.HQ + h] = natural_lse(M, L, a.scale);
 }
 
 // Heads that are no whole 16-byte chunks: one workgroup per row and query
@@ -855,11 +933,32 @@ extern "C" int sj_paged_plan(void* stream, const int32_t* lengths, const int32_t
 
 namespace {
 
-// waves of the split walks: as many as the chip holds at once
-constexpr int STREAM_GROUPS = 1024;
+// a number that no other call has, as far as 64 bits go: the process's calls
+// counted from a point of its own (time, process, an address), and mixed
+unsigned long long mix(unsigned long long z) {
+  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+  z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+  return z ^ (z >> 31);
+}
+unsigned long long new_mark() {
+  static std::atomic<unsigned long long> calls{[] {
+    timespec now = {};
+    clock_gettime(CLOCK_REALTIME, &now);
+    return mix((unsigned long long)now.tv_sec * 1000000007ull + now.tv_nsec) ^ mix((unsigned long long)getpid()) ^
+           mix((unsigned long long)(uintptr_t)&now);
+  }()};
+  return mix(calls.fetch_add(1) * 0x9e3779b97f4a7c15ull) | 1;  // not 0: that is a cleared flag
+}
 
-// whether sj_paged_attention splits: a rule on sizes alone, so that the
-// workspace query knows it too
+Div make_div(uint32_t d) {
+  Div r = {0, 0};
+  while ((1ul << r.shift) < d) r.shift++;
+  r.mul = (uint32_t)((((1ul << r.shift) - d) << 32) / d + 1);
+  return r;
+}
+
+// whether sj_paged_attention may split: by sizes alone, so that the workspace
+// query knows it too
 bool split_ok(long rows, long head_dim) { return rows <= STREAM_ROWS && head_dim % 4 == 0; }
 long slot_floats(long g, long head_dim) { return 32 + (g < 16 ? g : 16) * head_dim; }
 
@@ -886,16 +985,20 @@ int launch_direct(hipStream_t s, const PagedArgs& a, int waves, Walk<T, DC>) {
   return SJ_OK;
 }
 template <typename T, int DC>
-int launch_stream(hipStream_t s, const PagedArgs& a, Walk<T, DC>) {
+int launch_split(hipStream_t s, const PagedArgs& a, long most, Walk<T, DC>) {
   static sj::OncePerDevice once;
   if (int st = sjh::once_per_device(once, [] {
-        SJ_HIP(hipFuncSetAttribute((const void*)k_paged_stream<T, DC>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        SJ_HIP(hipFuncSetAttribute((const void*)k_paged_split<T, DC>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                    4 * Walk<T, DC>::LDS));
         return SJ_OK;
       }))
     return st;
-  k_paged_stream<T, DC><<<STREAM_GROUPS, 256, 4 * Walk<T, DC>::LDS, s>>>(a);
-  k_paged_join<T><<<dim3((unsigned)a.rows, (unsigned)a.HQ), 256, 0, s>>>(a);
+  // A short line of places (at the most that the tables hold) goes over as many
+  // workgroups as the chip holds at once, so that none begins behind another;
+  // a long one over more of them, so that they end together
+  constexpr int at_once = 256 * split_per_cu(DC);
+  const long places = (long)a.rows * a.HK * a.QT * ((most + 4 * Walk<T, DC>::KT - 1) / (4 * Walk<T, DC>::KT));
+  k_paged_split<T, DC><<<places < 8 * at_once ? at_once : STREAM_GROUPS, 256, 4 * Walk<T, DC>::LDS, s>>>(a);
   return SJ_OK;
 }
 
@@ -906,20 +1009,26 @@ int attend(hipStream_t s, PagedArgs& a, long most, void* workspace) {
     return SJ_OK;
   }
   const long units = (long)a.rows * a.HK * a.QT;
-  // a direct walk's waves take a tile each in turn; past 2048 keys a row the
-  // split walks pay for their second launch
-  const bool direct = most <= 2048 || !split_ok(a.rows, a.D) || (most / 16 + 1) * units > 0x7fffffffL;
   int st = SJ_OK;
-  if (direct) {
-    int waves = units >= 1024 ? 4 : 8;
-    if (most <= 256) waves = 4;
-    by_width<T>(a.D, [&](auto w) { st = launch_direct(s, a, waves, w); });
-    return st;
-  }
+  bool direct = !split_ok(a.rows, a.D) || (most / 16 + 1) * units > 0x7fffffffL;
+  by_width<T>(a.D, [&](auto w) {
+    const long tiles = (most + decltype(w)::KT - 1) / decltype(w)::KT;
+    // The direct form, which sums no rows and joins in LDS alone, where a wave
+    // has one tile, and where the workgroups are many and the walks, however
+    // uneven, not long.  us, direct / split, bf16: heads of 64, 1 request x 2
+    // of 512 keys 7.8 / 10.1, of 1024 11.6 / 10.6, of 8192 62 / 11.6; 64 x 2 of
+    // 1024 12.8 / 14.9, of 4096 40 / 39; 64 x 8 of 1024 34 / 42, of 4096 117 /
+    // 127, of 8192 228 / 243 (but 45 x 4 of 1 to 6000 32 / 17); heads of 128,
+    // 256 x 8 of 1024 200 / 188
+    direct = direct || tiles <= 8 || (units >= 128 && tiles <= 16) || (units >= 512 && units < 2048 && tiles <= 64);
+    if (direct) st = launch_direct(s, a, tiles <= 4 || units >= 1024 ? 4 : 8, w);
+  });
+  if (direct) return st;
   a.slot = (int)slot_floats(a.G, a.D);
-  a.plan = (int32_t*)workspace;
-  a.part = (float*)((uint8_t*)workspace + 4 * (STREAM_ROWS + 8));
-  by_width<T>(a.D, [&](auto w) { st = launch_stream(s, a, w); });
+  a.flag = (unsigned long long*)workspace;
+  a.part = (float*)((uint8_t*)workspace + 16 * STREAM_GROUPS);
+  a.mark = new_mark();
+  by_width<T>(a.D, [&](auto w) { st = launch_split(s, a, most, w); });
   return st;
 }
 
@@ -927,7 +1036,7 @@ int attend(hipStream_t s, PagedArgs& a, long most, void* workspace) {
 
 extern "C" size_t sj_paged_attention_workspace_bytes(long rows, long hq, long hk, long head_dim) {
   if (rows <= 0 || hq <= 0 || hk <= 0 || head_dim <= 0 || hq % hk || !split_ok(rows, head_dim)) return 0;
-  return 4 * (STREAM_ROWS + 8) + 8 * STREAM_GROUPS * (size_t)slot_floats(hq / hk, head_dim) * sizeof(float);
+  return 16 * STREAM_GROUPS + 2 * STREAM_GROUPS * (size_t)slot_floats(hq / hk, head_dim) * sizeof(float);
 }
 
 extern "C" int sj_paged_attention(void* stream, const void* q, long ldq, const void* k_cache, const void* v_cache,
@@ -959,9 +1068,11 @@ extern "C" int sj_paged_attention(void* stream, const void* q, long ldq, const v
   a.scale = (float)(1.4426950408889634 / sqrt((double)head_dim));
   a.G = (int)(hq / hk);
   a.QT = (a.G + 15) / 16;
-  while ((1UL << a.pshift) < (unsigned long)page_size) a.pshift++;
-  a.pmul = (uint32_t)((((1UL << a.pshift) - (unsigned long)page_size) << 32) / (unsigned long)page_size + 1);
   SJ_REQUIRE(rows <= (1L << 23) / (hk * a.QT), "paged attention: %ld rows of %ld heads", rows, hk);
+  a.d_page = make_div((uint32_t)page_size);
+  a.d_heads = make_div((uint32_t)(hk * a.QT));
+  a.d_tiles = make_div((uint32_t)a.QT);
+  a.d_quads = make_div((uint32_t)(head_dim / 4 > 0 ? head_dim / 4 : 1));
   long most = ldt * page_size;
   if (window > 0 && window < most) most = window;
   hipStream_t s = (hipStream_t)stream;

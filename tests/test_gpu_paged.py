@@ -335,7 +335,9 @@ def test_attention_windows(dtype, window):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("lengths,hq,hk,D,P", [([20000], 6, 2, 64, 16), ([9000, 3], 8, 8, 128, 64), ([1] * 500, 4, 2, 64, 16),
                                                ([5000] + [40] * 60, 16, 4, 64, 24), ([3000, 3001], 2, 1, 32, 16),
-                                               ([70000], 2, 1, 16, 256), (list(range(0, 900, 9)), 6, 2, 64, 16)])
+                                               ([70000], 2, 1, 16, 256), (list(range(0, 900, 9)), 6, 2, 64, 16),
+                                               ([3] * 2100 + [200], 2, 1, 32, 16), ([700] + [9] * 2047, 1, 1, 16, 16),
+                                               ([600] * 12, 68, 2, 64, 16)])
 def test_attention_long_and_ragged_batches(dtype, lengths, hq, hk, D, P):
     """Few long rows are split over the workgroups and joined; many short ones share them."""
     Attend(len(lengths) + D, dtype, hq, hk, D, P, lengths).upload().run().check()
