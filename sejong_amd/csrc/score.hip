@@ -30,8 +30,8 @@ namespace {
 // an exponential.
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int CAP = 1024;   // entries at or above the threshold that LDS holds
-constexpr int SLICE = 8192; // entries of a workgroup's slice
+constexpr int CAP_SLICE = 1024;  // entries at or above the threshold that LDS holds of a slice
+constexpr int SLICE = 8192;  // entries of a workgroup's slice where the slices are few; twice as many where they are not
 
 typedef unsigned long long u64;
 
@@ -109,7 +109,7 @@ struct ScoreArgs {
   const void* x;
   long ldx;
   long rows;
-  int V, top, slices;
+  int V, top, slices, width;  // width: entries of a slice, a multiple of 8
   const int32_t* tokens;
   float *logprob, *entropy, *stats;
   int32_t* ids;
@@ -157,7 +157,7 @@ __device__ __forceinline__ void write_alternative(const ScoreArgs& a, long row, 
 template <typename T, int NT, int EV>
 __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   typedef Unit<T> U;
-  constexpr int E = U::E, NU = EV / E, NW = NT / 64, GROUPS = 256 / NT;
+  constexpr int E = U::E, NU = EV / E, NW = NT / 64, GROUPS = 256 / NT, CAP = NT == 64 ? 64 * EV : CAP_SLICE;
   __shared__ __attribute__((aligned(16))) float s_best[256];
   __shared__ u64 s_cand[GROUPS][CAP], s_last[4];
   __shared__ float s_max[4], s_sum[2][2][4], s_T[GROUPS];
@@ -169,12 +169,12 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     else
       __syncthreads();
   };
-  const long g = (long)blockIdx.x * GROUPS + gt;
-  const long row = NT == 64 ? g : g / a.slices;
+  const int g = blockIdx.x * GROUPS + gt;
+  const int row = NT == 64 ? g : g / a.slices;
   if (row >= a.rows) return;  // a whole wave, or nobody
-  const int slice = NT == 64 ? 0 : (int)(g - row * a.slices);
-  const int base = slice * (NT * EV), end = min(a.V, base + NT * EV), top = a.top;
-  const T* x = (const T*)a.x + row * a.ldx;
+  const int slice = NT == 64 ? 0 : g - row * a.slices;
+  const int base = slice * a.width, end = min(a.V, base + a.width), top = a.top;
+  const T* x = (const T*)a.x + (long)row * a.ldx;
   auto index = [&](int i) { return base + E * (t + NT * (i / E)) + i % E; };
   U u[NU];
 #pragma unroll
@@ -183,20 +183,28 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     if (v + E <= end) u[i].r = *(const typename U::Raw*)(x + v);
   }
   const Token tk = token_of<T>(a, row);
-  float f[EV], best = -INFINITY;
+  // units past the end are left out everywhere; one that crosses it is filled
+  // with -inf
+  constexpr int PART = 4, PARTS = EV / PART;  // maxima of parts: the search below passes those without
+  float f[EV], pm[PARTS], best = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NU; i++) {
     const int v = base + E * (t + NT * i);
-    if (v + E <= end) {
+    if (v < end) {
+      if (v + E <= end) {
 #pragma unroll
-      for (int e = 0; e < E; e++) f[i * E + e] = u[i].get(e);
-    } else {
+        for (int e = 0; e < E; e++) f[i * E + e] = u[i].get(e);
+      } else {
 #pragma unroll
-      for (int e = 0; e < E; e++) f[i * E + e] = v + e < end ? at_f32(x, v + e) : -INFINITY;
+        for (int e = 0; e < E; e++) f[i * E + e] = v + e < end ? at_f32(x, v + e) : -INFINITY;
+      }
+#pragma unroll
+      for (int j = i * E / PART; j < (i + 1) * E / PART; j++) {
+        pm[j] = fmaxf(fmaxf(f[PART * j], f[PART * j + 1]), fmaxf(f[PART * j + 2], f[PART * j + 3]));
+        best = fmaxf(best, pm[j]);
+      }
     }
   }
-#pragma unroll
-  for (int i = 0; i < EV; i++) best = fmaxf(best, f[i]);
   float m = all_max(best);
   if (t == 0) s_n[gt] = 0;
   if (NT > 64) {
@@ -223,12 +231,51 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   }
   const float ref = m == -INFINITY ? 0.f : m;
   float rest = 0.f, xs = 0.f;
+  // Terms 2^(x log2e - c) with c = ref log2e rounded: one fused step and the
+  // exponential.  c stands for a reference that is off by delta / log2e, known
+  // exactly, so the sums come back to ref by one factor.
+  const float c = ref * LOG2E, delta = fmaf(ref, LOG2E, -c);
 #pragma unroll
-  for (int i = 0; i < EV; i++) {
-    const float d = f[i] - ref, e = __builtin_amdgcn_exp2f(d * LOG2E);
-    rest += e;
-    xs = fmaf(e, fmaxf(d, -1e30f), xs);  // a share of 0 has no entropy; a NaN is in e
+  for (int i = 0; i < NU; i++) {
+    const int v = base + E * (t + NT * i);
+    if (v < end) {
+      if (v + E > end && ref > -1e20f) {  // the filling: a share of 0 and no NaN
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (v + e >= end) f[i * E + e] = -1e30f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float d = fmaf(f[i * E + e], LOG2E, -c), y = __builtin_amdgcn_exp2f(d);
+        rest += y;
+        xs = fmaf(y, d, xs);
+      }
+    }
   }
+  const float back = __builtin_amdgcn_exp2f(-delta);
+  rest *= back;
+  xs = fmaf(xs * back, 0.6931471805599453f, -rest * (delta * 0.6931471805599453f));
+  // The sums with the difference first, and without one entry that equals
+  // `skip`: entries of -inf have a share of 0 and no entropy, a NaN stays
+  auto slowly = [&](float skip) {
+    rest = xs = 0.f;
+    bool left = skip != skip;
+#pragma unroll
+    for (int i = 0; i < NU; i++)
+      if (base + E * (t + NT * i) < end)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const float y = f[i * E + e];
+          const bool out = !left && y == skip;
+          left |= out;
+          const float d = y - ref, p = out ? 0.f : __builtin_amdgcn_exp2f(d * LOG2E);
+          rest += p;
+          xs = fmaf(p, fmaxf(d, -1e30f), xs);
+        }
+  };
+  // -inf or NaN among the entries, or a reference whose rounding leaves the
+  // powers' range
+  if (__any(!(fabsf(xs) < INFINITY)) || fabsf(ref) > 1e6f) slowly(NAN);
   auto total = [&](float& r, float& y, int k) {
     r = all_sum(r);
     y = all_sum(y);
@@ -245,20 +292,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     int first = 0;
     if (NT > 64) while (first < NW - 1 && s_max[first] != m) first++;
     const u64 mask = __ballot(best == m);
-    if (w == first && mask && lane == __ffsll(mask) - 1) {
-      rest = xs = 0.f;
-      bool left = false;
-      float r = ref;
-      asm volatile("" : "+v"(r));  // or the terms above would be kept for here, in registers of their own
-#pragma unroll
-      for (int i = 0; i < EV; i++) {
-        const bool out = !left && f[i] == m;
-        left |= out;
-        const float d = f[i] - r, e = out ? 0.f : __builtin_amdgcn_exp2f(d * LOG2E);
-        rest += e;
-        xs = fmaf(e, fmaxf(d, -1e30f), xs);
-      }
-    }
+    if (w == first && mask && lane == __ffsll(mask) - 1) slowly(m);
     total(rest, xs, 1);
   } else {
     rest = l - 1.f;
@@ -281,14 +315,16 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   };
   sync();
   const float T0 = s_T[gt];
-  if (best >= T0) {
 #pragma unroll
-    for (int i = 0; i < EV; i++)
-      if (f[i] >= T0 && index(i) < end) {
-        const int n = atomicAdd(&s_n[gt], 1);
-        if (n < CAP) s_cand[gt][n] = order_key(f[i], index(i));
-      }
-  }
+  for (int j = 0; j < PARTS; j++)
+    if (index(PART * j) < end && pm[j] >= T0) {
+#pragma unroll
+      for (int i = PART * j; i < PART * (j + 1); i++)
+        if (f[i] >= T0 && index(i) < end) {
+          const int n = atomicAdd(&s_n[gt], 1);
+          if (n < CAP) s_cand[gt][n] = order_key(f[i], index(i));
+        }
+    }
   sync();
   int n = s_n[gt];
   const int held = min(top, end - base);  // a row's last slice may have fewer entries
@@ -317,6 +353,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     for (int i = t; i < n; i += NT) {
       const u64 k = s_cand[gt][i];
       int place = 0;
+#pragma unroll 4
       for (int c = 0; c < n; c++) place += s_cand[gt][c] > k;
       if (place < top) put(place, k);
     }
@@ -351,11 +388,12 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
 __device__ __forceinline__ u64 larger_of(u64 a, u64 b) { return a > b ? a : b; }
 template <typename T>
 __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a) {
+  constexpr int CAP = CAP_SLICE;
   __shared__ u64 cand[CAP], s_key[4];
   __shared__ float s_max[4], s_sum[2][4];
   __shared__ int s_n, s_first;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const long row = blockIdx.x;
+  const int row = blockIdx.x;
   const int S = a.slices, top = a.top, all = S * top;
   const f32x4* sums = (const f32x4*)part_sums(a, row);
   const u64* keys = part_keys(a, row);
@@ -415,6 +453,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a) {
     for (int i = t; i < n; i += 256) {
       const u64 key = cand[i];
       int place = 0;
+#pragma unroll 4
       for (int c = 0; c < n; c++) place += cand[c] > key;
       if (place < top) write_alternative(a, row, place, key, ref, ll);
     }
@@ -508,20 +547,30 @@ __global__ __launch_bounds__(256) void k_score_bwd(ScoreBwdArgs a) {
   }
 }
 
+// the slices of a row, at most: what the workspace holds
 long slices_of(long vocab) { return (vocab + SLICE - 1) / SLICE; }
 
 template <typename T>
-void launch_score(hipStream_t s, const ScoreArgs& a) {
-  const unsigned waves = (unsigned)((a.rows + 3) / 4);
+void launch_score(hipStream_t s, ScoreArgs& a) {
+  const unsigned waves = (unsigned)((a.rows + 3) / 4), rows = (unsigned)a.rows;
+  a.slices = 1;
+  a.width = (a.V + 7) / 8 * 8;
   if (a.V <= 512) {
     k_score<T, 64, 8><<<waves, 256, 0, s>>>(a);
   } else if (a.V <= 1024) {
     k_score<T, 64, 16><<<waves, 256, 0, s>>>(a);
   } else if (a.V <= 4096) {
-    k_score<T, 256, 16><<<(unsigned)a.rows, 256, 0, s>>>(a);
+    k_score<T, 256, 16><<<rows, 256, 0, s>>>(a);
   } else {
-    k_score<T, 256, 32><<<(unsigned)(a.rows * a.slices), 256, 0, s>>>(a);
-    if (a.slices > 1) k_score_join<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
+    const bool few = a.V <= SLICE || a.rows * slices_of(a.V) < 2048;
+    const int most = few ? SLICE : 2 * SLICE;
+    a.slices = (a.V + most - 1) / most;
+    a.width = ((a.V + a.slices - 1) / a.slices + 7) / 8 * 8;  // alike, so that they end together
+    if (few)
+      k_score<T, 256, 32><<<rows * a.slices, 256, 0, s>>>(a);
+    else
+      k_score<T, 256, 64><<<rows * a.slices, 256, 0, s>>>(a);
+    if (a.slices > 1) k_score_join<T><<<rows, 256, 0, s>>>(a);
   }
 }
 template <typename T>
@@ -559,7 +608,7 @@ extern "C" int sj_token_logprobs(void* stream, const void* x, int dtype, long ld
     return sjh::fail(SJ_ERR_CAPACITY, "token log probabilities workspace: required %zu bytes, available %zu bytes", need,
                      workspace ? workspace_bytes : 0);
   ScoreArgs a = {};
-  a.x = x; a.ldx = ldx; a.rows = rows; a.V = (int)vocab; a.top = (int)top; a.slices = (int)slices_of(vocab);
+  a.x = x; a.ldx = ldx; a.rows = rows; a.V = (int)vocab; a.top = (int)top;
   a.tokens = tokens; a.logprob = logprob; a.entropy = entropy; a.stats = stats; a.ids = top_ids; a.alt = top_logprob;
   a.part = (uint8_t*)workspace;
   if (dtype == SJ_BF16)
