@@ -5,8 +5,12 @@
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
+#include <time.h>
+#include <unistd.h>
 
-#include "common.h"
+#include <atomic>
+
+#include "lanes.h"
 
 static thread_local char g_last_error[1024] = "";
 
@@ -25,6 +29,22 @@ int fail(int status, const char* fmt, ...) {
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
   va_end(ap);
   return status;
+}
+// the process's calls counted from a point of its own (time, process, an
+// address), and mixed
+static unsigned long long mix(unsigned long long z) {
+  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+  z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+  return z ^ (z >> 31);
+}
+unsigned long long call_number() {
+  static std::atomic<unsigned long long> calls{[] {
+    timespec now = {};
+    clock_gettime(CLOCK_REALTIME, &now);
+    return mix((unsigned long long)now.tv_sec * 1000000007ull + now.tv_nsec) ^ mix((unsigned long long)getpid()) ^
+           mix((unsigned long long)(uintptr_t)&now);
+  }()};
+  return mix(calls.fetch_add(1) * 0x9e3779b97f4a7c15ull) | 1;
 }
 int hip_check(hipError_t e, const char* what) {
   return fail(SJ_ERR_HIP, "%s: HIP %d: %s", what, (int)e, hipGetErrorString(e));

@@ -3,12 +3,8 @@
 // of the step's tokens over the pages (no counterpart in the reference, whose
 // cache holds one sequence: model lib.rs:36-50, architecture.rs:428-533).
 #include <math.h>
-#include <time.h>
-#include <unistd.h>
 
-#include <atomic>
-
-#include "common.h"
+#include "lanes.h"
 
 using namespace sj;
 
@@ -36,30 +32,6 @@ struct PlanArgs {
 };
 
 __device__ __forceinline__ uint32_t ceil_div(uint32_t n, uint32_t d) { return n / d + (n % d != 0); }
-
-// inclusive scan over the wave: four steps within rows of 16 lanes, then the
-// rows' last values into the rows behind
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_or0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
-__device__ __forceinline__ uint32_t scan_add(uint32_t v) {
-  v += dpp_or0<0x111, 0xf>(v);  // from 1, 2, 4, 8 lanes before
-  v += dpp_or0<0x112, 0xf>(v);
-  v += dpp_or0<0x114, 0xf>(v);
-  v += dpp_or0<0x118, 0xf>(v);
-  v += dpp_or0<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
-  v += dpp_or0<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
-  return v;
-}
-// of values >= 0
-__device__ __forceinline__ int scan_max(int v) {
-  v = max(v, dpp_or0<0x111, 0xf>(v));
-  v = max(v, dpp_or0<0x112, 0xf>(v));
-  v = max(v, dpp_or0<0x114, 0xf>(v));
-  v = max(v, dpp_or0<0x118, 0xf>(v));
-  v = max(v, dpp_or0<0x142, 0xa>(v));
-  v = max(v, dpp_or0<0x143, 0xc>(v));
-  return v;
-}
 
 __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
   __shared__ uint32_t w_tok[4], w_need[4], w_want[4], w_long[4], w_bad[4];
@@ -254,8 +226,8 @@ struct PagedArgs {
   float scale;  // log2(e) / sqrt(D): the softmax in powers of two
   int G, QT;    // query heads of a KV head, and their tiles of 16
   // split walks
-  unsigned long long* flag;  // [2 * workgroups]: mark where a part's totals are complete
-  unsigned long long mark;
+  unsigned long long* flag;  // [2 * workgroups], of the meetings
+  unsigned long long number;
   float* part;  // [2 * workgroups][slot]
   int slot;     // floats of a walk's totals: 16 maxima and sums of shares, min(G, 16) rows of D
 };
@@ -664,32 +636,15 @@ __global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArg
 // four (one per wave), and every workgroup an equal piece of the line.  Each
 // workgroup sums the rows' tiles itself (one block scan).  A walk that lies in
 // one piece is written as it is; of a walk that is cut, each workgroup leaves
-// its totals in the workspace, and the one that counts last joins them in the
+// its totals in the workspace, and the last (meet, lanes.h) joins them in the
 // order of the keys.  A workgroup has at most two cut walks, the end of one
 // and the beginning of another.
 //
-// Totals pass between workgroups (on different XCDs, each with its own L2)
-// through relaxed atomics at agent scope, which are coherent by themselves.
-// A part's totals are complete (vmcnt 0) before its flag is set, and its flag
-// (vmcnt 0 again) before it looks at the flags of the walk's other parts; so
-// the part whose flag is set last finds all of them.  Two parts may both find
-// them: they write the same bits.  Nobody waits for anybody.  The workspace is
-// the caller's and not cleared, so a set flag is a number of 64 bits that no
-// other call has; whoever finds all flags clears them, and a replayed graph,
-// which keeps its number, starts from cleared flags again.
 constexpr int STREAM_ROWS = 2048;
 // workgroups: as many as 256 CUs hold at once (by registers), at most 768
 constexpr int split_per_cu(int dc) { return dc == 8 ? 1 : dc == 2 || dc == 3 ? 3 : 2; }
 constexpr int STREAM_GROUPS = 1024;
 
-__device__ __forceinline__ void share_put(float* p, float x, float y) {
-  __hip_atomic_store((unsigned long long*)p, ((unsigned long long)__float_as_uint(y) << 32) | __float_as_uint(x),
-                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 share_get(const float* p) {
-  const unsigned long long v = __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
-}
 template <typename T, int DC>
 __global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs a) {
   typedef Walk<T, DC> W;
@@ -769,26 +724,12 @@ __global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs
       for (int u = t; u < items; u += 256) {
         const int r = div(u, a.d_quads), q = u - r * quads;
         const Total v = joined<T, DC, 4>(a, sh, lds, 4, r, 4 * q);
-        if (q == 0) share_put(s + 2 * r, v.M, v.L);
-        share_put(s + 32 + 2 * u, v.s[0], v.s[1]);
-        share_put(s + 32 + 2 * (items + u), v.s[2], v.s[3]);
+        if (q == 0) part_put(s + 2 * r, v.M, v.L);
+        part_put(s + 32 + 2 * u, v.s[0], v.s[1]);
+        part_put(s + 32 + 2 * (items + u), v.s[2], v.s[3]);
       }
       auto flag = [&](int i) { return a.flag + 2L * (g0 + i) + (i == 0); };
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (w == 0) {
-        if (lane == 0) __hip_atomic_store(flag(blockIdx.x - g0), a.mark, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        bool set = true;
-        for (int i = lane; i < parts; i += 64)
-          set &= __hip_atomic_load(flag(i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.mark;
-        set = __all(set);
-        if (lane == 0) complete = set;
-      }
-      __syncthreads();
-      if (complete) {
-        for (int i = t; i < parts; i += 256)
-          __hip_atomic_store(flag(i), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (meet(flag, blockIdx.x - g0, parts, a.number, &complete)) {
         // fewer items than threads: groups of threads share the parts, and
         // join through LDS
         const int span = min(items, 256), groups = 256 / span, gr = t / span;
@@ -804,9 +745,9 @@ __global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs
 #pragma unroll
             for (int k = 0; k < MANY; k++) {
               const float* p = slot(min(i + k * groups, parts - 1));
-              m[k] = share_get(p + 2 * r);
-              p0[k] = share_get(p + 32 + 2 * u);
-              p1[k] = share_get(p + 32 + 2 * (items + u));
+              m[k] = part_get(p + 2 * r);
+              p0[k] = part_get(p + 32 + 2 * u);
+              p1[k] = part_get(p + 32 + 2 * (items + u));
             }
 #pragma unroll
             for (int k = 0; k < MANY; k++)
@@ -933,23 +874,6 @@ extern "C" int sj_paged_plan(void* stream, const int32_t* lengths, const int32_t
 
 namespace {
 
-// a number that no other call has, as far as 64 bits go: the process's calls
-// counted from a point of its own (time, process, an address), and mixed
-unsigned long long mix(unsigned long long z) {
-  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
-  z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
-  return z ^ (z >> 31);
-}
-unsigned long long new_mark() {
-  static std::atomic<unsigned long long> calls{[] {
-    timespec now = {};
-    clock_gettime(CLOCK_REALTIME, &now);
-    return mix((unsigned long long)now.tv_sec * 1000000007ull + now.tv_nsec) ^ mix((unsigned long long)getpid()) ^
-           mix((unsigned long long)(uintptr_t)&now);
-  }()};
-  return mix(calls.fetch_add(1) * 0x9e3779b97f4a7c15ull) | 1;  // not 0: that is a cleared flag
-}
-
 Div make_div(uint32_t d) {
   Div r = {0, 0};
   while ((1ul << r.shift) < d) r.shift++;
@@ -1027,7 +951,7 @@ int attend(hipStream_t s, PagedArgs& a, long most, void* workspace) {
   a.slot = (int)slot_floats(a.G, a.D);
   a.flag = (unsigned long long*)workspace;
   a.part = (float*)((uint8_t*)workspace + 16 * STREAM_GROUPS);
-  a.mark = new_mark();
+  a.number = sjh::call_number();
   by_width<T>(a.D, [&](auto w) { st = launch_split(s, a, most, w); });
   return st;
 }

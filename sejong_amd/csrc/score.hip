@@ -11,7 +11,7 @@
 // holds beside its peak (in fp32 1 + 1e-8 is 1, and the log 0).
 #include <math.h>
 
-#include "common.h"
+#include "lanes.h"
 
 using namespace sj;
 
@@ -58,52 +58,27 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 
 // E entries at any element alignment, as fp32
-template <typename T>
+template <typename T, int EE>
 struct Unit;
-template <>
-struct Unit<float> {
-  static constexpr int E = 4;
-  struct __attribute__((packed, aligned(4))) Raw { float v[4]; } r;
+template <int EE>
+struct Unit<float, EE> {
+  static constexpr int E = EE;
+  struct __attribute__((packed, aligned(4))) Raw { float v[E]; } r;
   __device__ __forceinline__ float get(int i) const { return r.v[i]; }
 };
-template <>
-struct Unit<bf16_t> {
-  static constexpr int E = 8;
-  struct __attribute__((packed, aligned(2))) Raw { u32x4 v; } r;
+template <int EE>
+struct Unit<bf16_t, EE> {
+  static constexpr int E = EE;
+  struct __attribute__((packed, aligned(2))) Raw { uint32_t v[E / 2]; } r;
   __device__ __forceinline__ float get(int i) const {
     const uint32_t w = r.v[i >> 1];
     return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
   }
 };
+template <typename T>
+constexpr int WIDE = 16 / (int)sizeof(T);  // entries of 16 bytes
 __device__ __forceinline__ float at_f32(const float* x, long i) { return x[i]; }
 __device__ __forceinline__ float at_f32(const bf16_t* x, long i) { return bf2f(x[i]); }
-
-// sums and maxima over a wave without LDS: four steps within rows of 16
-// lanes, then the four rows' values as scalars, in a fixed order
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-template <class F>
-__device__ __forceinline__ float wave_all(float v, F f) {
-  v = f(v, dpp<0xB1>(v));   // lanes 1, 0, 3, 2
-  v = f(v, dpp<0x4E>(v));   // lanes 2, 3, 0, 1
-  v = f(v, dpp<0x141>(v));  // mirrored within 8
-  v = f(v, dpp<0x140>(v));  // mirrored within 16
-  const int b = __float_as_int(v);
-  const float r0 = __int_as_float(__builtin_amdgcn_readlane(b, 0)), r1 = __int_as_float(__builtin_amdgcn_readlane(b, 16)),
-              r2 = __int_as_float(__builtin_amdgcn_readlane(b, 32)), r3 = __int_as_float(__builtin_amdgcn_readlane(b, 48));
-  return f(f(r0, r1), f(r2, r3));
-}
-__device__ __forceinline__ float all_max(float v) {
-  return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float all_min(float v) {
-  return wave_all(v, [](float a, float b) { return fminf(a, b); });
-}
-__device__ __forceinline__ float all_sum(float v) {
-  return wave_all(v, [](float a, float b) { return a + b; });
-}
 
 struct ScoreArgs {
   const void* x;
@@ -114,6 +89,8 @@ struct ScoreArgs {
   float *logprob, *entropy, *stats;
   int32_t* ids;
   float* alt;
+  u64* flag;      // [rows][slices], of the meetings
+  u64 number;
   uint8_t* part;  // per row: (m, rest, xs, -) of each slice, then each slice's `top` keys
 };
 __device__ __forceinline__ float* part_sums(const ScoreArgs& a, long row) {
@@ -152,12 +129,141 @@ __device__ __forceinline__ void write_alternative(const ScoreArgs& a, long row, 
   a.alt[row * a.top + place] = key_value(k) - ref - ll;
 }
 
+// The place of each of the n keys of `keys` (LDS) among them, f(place, key) for
+// the first `top`: four lanes of a group's NT threads count for one key.
+template <int NT, class F>
+__device__ __forceinline__ void rank(const u64* keys, int n, int top, int t, F f) {
+  for (int i = t >> 2; i < n; i += NT / 4) {
+    const u64 k = keys[i];
+    uint32_t place = 0;
+#pragma unroll 4
+    for (int c = t & 3; c < n; c += 4) place += keys[c] > k;
+    place += dpp<0xB1>(place);
+    place += dpp<0x4E>(place);
+    if ((t & 3) == 0 && (int)place < top) f((int)place, k);
+  }
+}
+__device__ __forceinline__ u64 larger_of(u64 a, u64 b) { return a > b ? a : b; }
+
+// The slices of a row, by one workgroup: the sums relative to the row's
+// maximum (slice s holds e^(m_s - m) (1 + rest_s) of them), and the largest of
+// the slices' lists.  MEET: the slices were written by workgroups of this
+// launch.
+struct JoinShared {
+  u64 cand[CAP_SLICE], key[64], last[4];
+  float max[4], sum[2][4];
+  int n, first;
+};
+template <bool MEET>
+__device__ __forceinline__ void join_row(const ScoreArgs& a, int row, const Token& tk, JoinShared& sh) {
+  constexpr int CAP = CAP_SLICE;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int S = a.slices, top = a.top, all = S * top;
+  const float* sums = part_sums(a, row);
+  const u64* keys = part_keys(a, row);
+  auto key = [&](int i) { return MEET ? part_get(keys + i) : keys[i]; };
+  auto sum_of = [&](int s) {
+    if (!MEET) return *(const f32x4*)(sums + 4 * s);
+    const float2 p = part_get(sums + 4 * s), q = part_get(sums + 4 * s + 2);
+    return f32x4{p.x, p.y, q.x, q.y};
+  };
+  constexpr int HELD = 4;  // keys a thread keeps from the first look at them
+  u64 k[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; i++) k[i] = t + 256 * i < all ? key(t + 256 * i) : 0;
+  const f32x4 mine = t < S ? sum_of(t) : f32x4{-INFINITY, 0.f, 0.f, 0.f};
+  // The threshold: of the slices' j-th keys the i-th largest, i j >= top, has
+  // i slices with j keys each at or above it (64 lanes take the slices in
+  // turn and keep their largest)
+  const int lanes = min(S, 64), j = min(top, 2 * ((top + lanes - 1) / lanes)), i = top ? (top + j - 1) / j : 0;
+  u64 col = 0;
+  if (w == 0 && top)
+    for (int s = lane; s < S; s += 64) col = larger_of(col, key(s * top + j - 1));
+  float m = mine[0];
+  for (int s = t + 256; s < S; s += 256) m = fmaxf(m, sum_of(s)[0]);
+  if (t == 0) sh.n = 0, sh.first = 0x7fffffff;
+  m = all_max(m);
+  if (lane == 0) sh.max[w] = m;
+  if (w == 0) sh.key[lane] = col;
+  __syncthreads();
+  m = fmaxf(fmaxf(sh.max[0], sh.max[1]), fmaxf(sh.max[2], sh.max[3]));
+  u64 T0 = 1;  // fewer than i slices with j keys: every key counts
+  if (top) {
+    const u64 mine = sh.key[lane];
+    int larger = 0;
+    for (int c = 0; c < lanes; c++) larger += sh.key[c] > mine;
+    const u64 at = __ballot(mine && larger == i - 1);
+    if (at) T0 = sh.key[__ffsll(at) - 1];
+  }
+  if (t < S && mine[0] == m) atomicMin(&sh.first, t);  // the slice that leaves its maximum out
+  for (int s = t + 256; s < S; s += 256)
+    if (sum_of(s)[0] == m) atomicMin(&sh.first, s);
+  auto collect = [&](u64 key) {
+    if (key >= T0) {
+      const int n = atomicAdd(&sh.n, 1);
+      if (n < CAP) sh.cand[n] = key;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; i++) collect(k[i]);
+  for (int i = t + 256 * HELD; i < all; i += 256) collect(key(i));
+  __syncthreads();
+  const float ref0 = m == -INFINITY ? 0.f : m;
+  float rest = 0.f, xs = 0.f;
+  auto add = [&](int s, const f32x4& q) {
+    if (s == sh.first || q[0] == -INFINITY) {  // without an entry of its own there is nothing to leave out
+      rest += q[1];
+      xs += q[2];
+    } else {
+      const float d = q[0] - ref0, f = __builtin_amdgcn_exp2f(d * LOG2E);
+      rest += f * (1.f + q[1]);
+      xs += f > 0.f ? f * fmaf(d, 1.f + q[1], q[2]) : f;
+    }
+  };
+  if (t < S) add(t, mine);
+  for (int s = t + 256; s < S; s += 256) add(s, sum_of(s));
+  rest = all_sum(rest);
+  xs = all_sum(xs);
+  if (lane == 0) sh.sum[0][w] = rest, sh.sum[1][w] = xs;
+  __syncthreads();
+  rest = (sh.sum[0][0] + sh.sum[0][1]) + (sh.sum[0][2] + sh.sum[0][3]);
+  xs = (sh.sum[1][0] + sh.sum[1][1]) + (sh.sum[1][2] + sh.sum[1][3]);
+  float ref;
+  const float ll = write_row(a, row, m, rest, xs, tk, ref, t == 0);
+  if (!top) return;
+  const int n = sh.n;
+  if (n <= CAP) {
+    rank<256>(sh.cand, n, top, t, [&](int place, u64 k) { write_alternative(a, row, place, k, ref, ll); });
+    return;
+  }
+  u64 last = ~0ull;
+  for (int j = 0; j < top; j++) {
+    u64 k0 = 0;
+    for (int i = t; i < all; i += 256) {
+      const u64 k = key(i);
+      if (k < last && k > k0) k0 = k;
+    }
+    k0 = all_max(k0);
+    __syncthreads();
+    if (lane == 0) sh.last[w] = k0;
+    __syncthreads();
+    last = k0 = larger_of(larger_of(sh.last[0], sh.last[1]), larger_of(sh.last[2], sh.last[3]));
+    if (t == 0) write_alternative(a, row, j, k0, ref, ll);
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_score_join(ScoreArgs a) {
+  __shared__ JoinShared sh;
+  join_row<false>(a, blockIdx.x, token_of<T>(a, blockIdx.x), sh);
+}
+
 // One wave per row (NT = 64) or one workgroup per slice (NT = 256); a thread
-// holds EV entries, in units of 16 bytes that interleave over the threads.
-template <typename T, int NT, int EV>
+// holds EV entries, in units of E that interleave over the threads.  MEET: the
+// last of a row's workgroups joins its slices.
+template <typename T, int NT, int EV, int E = WIDE<T>, bool MEET = false>
 __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
-  typedef Unit<T> U;
-  constexpr int E = U::E, NU = EV / E, NW = NT / 64, GROUPS = 256 / NT, CAP = NT == 64 ? 64 * EV : CAP_SLICE;
+  typedef Unit<T, E> U;
+  constexpr int NU = EV / E, NW = NT / 64, GROUPS = 256 / NT, CAP = NT == 64 ? 64 * EV : CAP_SLICE;
   __shared__ __attribute__((aligned(16))) float s_best[256];
   __shared__ u64 s_cand[GROUPS][CAP], s_last[4];
   __shared__ float s_max[4], s_sum[2][2][4], s_T[GROUPS];
@@ -303,26 +409,51 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   if (whole) {
     ll = write_row(a, row, m, rest, xs, tk, rref, t == 0);
   } else if (t == 0) {
-    *(f32x4*)(part_sums(a, row) + 4 * slice) = f32x4{m, rest, xs, 0.f};
+    float* p = part_sums(a, row) + 4 * slice;
+    if constexpr (MEET)
+      part_put(p, m, rest), part_put(p + 2, xs, 0.f);
+    else
+      *(f32x4*)p = f32x4{m, rest, xs, 0.f};
   }
-  if (!top) return;
   u64* list = whole ? nullptr : part_keys(a, row) + (long)slice * top;
   auto put = [&](int place, u64 k) {
     if (whole)
       write_alternative(a, row, place, k, rref, ll);
+    else if constexpr (MEET)
+      part_put(list + place, k);
     else
       list[place] = k;
   };
+  auto done = [&] {
+    if constexpr (MEET) {
+      __shared__ JoinShared sh;
+      __shared__ int complete;
+      if (meet([&](int i) { return a.flag + (long)row * a.slices + i; }, slice, a.slices, a.number, &complete))
+        join_row<true>(a, row, tk, sh);
+    }
+  };
+  if (!top) return done();
   sync();
   const float T0 = s_T[gt];
+  // counted first, so that a wave takes its places in the list at once
+  uint32_t mine = 0;
+#pragma unroll
+  for (int j = 0; j < PARTS; j++)
+    if (index(PART * j) < end && pm[j] >= T0)
+#pragma unroll
+      for (int i = PART * j; i < PART * (j + 1); i++) mine += f[i] >= T0 && index(i) < end;
+  const uint32_t upto = scan_add(mine);
+  int from = 0;
+  if (lane == 63 && upto) from = atomicAdd(&s_n[gt], (int)upto);
+  from = __builtin_amdgcn_readlane(from, 63) + (int)(upto - mine);
 #pragma unroll
   for (int j = 0; j < PARTS; j++)
     if (index(PART * j) < end && pm[j] >= T0) {
 #pragma unroll
       for (int i = PART * j; i < PART * (j + 1); i++)
         if (f[i] >= T0 && index(i) < end) {
-          const int n = atomicAdd(&s_n[gt], 1);
-          if (n < CAP) s_cand[gt][n] = order_key(f[i], index(i));
+          if (from < CAP) s_cand[gt][from] = order_key(f[i], index(i));
+          from++;
         }
     }
   sync();
@@ -350,15 +481,9 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     for (int lo = base; n < held && lo < end; lo += CAP / 4) collect(lo, min(lo + CAP / 4, end), true);
   }
   if (n <= CAP && n >= held) {
-    for (int i = t; i < n; i += NT) {
-      const u64 k = s_cand[gt][i];
-      int place = 0;
-#pragma unroll 4
-      for (int c = 0; c < n; c++) place += s_cand[gt][c] > k;
-      if (place < top) put(place, k);
-    }
+    rank<NT>(s_cand[gt], n, top, t, put);
     for (int i = held + t; i < top; i += NT) put(i, 0);
-    return;
+    return done();
   }
   // more than LDS holds above the threshold, or fewer entries than asked for
   // beside NaN: the largest below the last, `top` times (then none, key 0)
@@ -369,7 +494,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
       const u64 k = order_key(at_f32(x, v), v);
       if (k < last && k > k0) k0 = k;
     }
-    k0 = wave_max(k0);
+    k0 = all_max(k0);
     if (NT > 64) {
       sync();
       if (lane == 0) s_last[w] = k0;
@@ -380,99 +505,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     last = k0;
     if (t == 0) put(j, k0);
   }
-}
-
-// The slices of a row, one workgroup: the sums relative to the row's maximum
-// (slice s holds e^(m_s - m) (1 + rest_s) of them), and the largest of the
-// slices' lists.
-__device__ __forceinline__ u64 larger_of(u64 a, u64 b) { return a > b ? a : b; }
-template <typename T>
-__global__ __launch_bounds__(256) void k_score_join(ScoreArgs a) {
-  constexpr int CAP = CAP_SLICE;
-  __shared__ u64 cand[CAP], s_key[4];
-  __shared__ float s_max[4], s_sum[2][4];
-  __shared__ int s_n, s_first;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int row = blockIdx.x;
-  const int S = a.slices, top = a.top, all = S * top;
-  const f32x4* sums = (const f32x4*)part_sums(a, row);
-  const u64* keys = part_keys(a, row);
-  const Token tk = token_of<T>(a, row);
-  constexpr int HELD = 4;  // keys a thread keeps from the first look at them
-  u64 k[HELD], T0 = 1;
-#pragma unroll
-  for (int i = 0; i < HELD; i++) k[i] = t + 256 * i < all ? keys[t + 256 * i] : 0;
-  float m = -INFINITY;
-  for (int s = t; s < S; s += 256) {
-    m = fmaxf(m, sums[s][0]);
-    if (top) T0 = larger_of(T0, keys[(s + 1) * top - 1]);  // a slice's last: `top` entries are as large
-  }
-  if (t == 0) s_n = 0, s_first = 0x7fffffff;
-  m = all_max(m);
-  T0 = wave_max(T0);
-  if (lane == 0) s_max[w] = m, s_key[w] = T0;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  T0 = larger_of(larger_of(s_key[0], s_key[1]), larger_of(s_key[2], s_key[3]));
-  for (int s = t; s < S; s += 256)
-    if (sums[s][0] == m) atomicMin(&s_first, s);  // the slice that leaves its maximum out
-  auto collect = [&](u64 key) {
-    if (key >= T0) {
-      const int n = atomicAdd(&s_n, 1);
-      if (n < CAP) cand[n] = key;
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < HELD; i++) collect(k[i]);
-  for (int i = t + 256 * HELD; i < all; i += 256) collect(keys[i]);
-  __syncthreads();
-  const float ref0 = m == -INFINITY ? 0.f : m;
-  float rest = 0.f, xs = 0.f;
-  for (int s = t; s < S; s += 256) {
-    const f32x4 q = sums[s];
-    if (s == s_first || q[0] == -INFINITY) {  // without an entry of its own there is nothing to leave out
-      rest += q[1];
-      xs += q[2];
-    } else {
-      const float d = q[0] - ref0, f = __builtin_amdgcn_exp2f(d * LOG2E);
-      rest += f * (1.f + q[1]);
-      xs += f > 0.f ? f * fmaf(d, 1.f + q[1], q[2]) : f;
-    }
-  }
-  rest = all_sum(rest);
-  xs = all_sum(xs);
-  if (lane == 0) s_sum[0][w] = rest, s_sum[1][w] = xs;
-  __syncthreads();
-  rest = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]);
-  xs = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
-  float ref;
-  const float ll = write_row(a, row, m, rest, xs, tk, ref, t == 0);
-  if (!top) return;
-  const int n = s_n;
-  if (n <= CAP) {
-    for (int i = t; i < n; i += 256) {
-      const u64 key = cand[i];
-      int place = 0;
-#pragma unroll 4
-      for (int c = 0; c < n; c++) place += cand[c] > key;
-      if (place < top) write_alternative(a, row, place, key, ref, ll);
-    }
-    return;
-  }
-  u64 last = ~0ull;
-  for (int j = 0; j < top; j++) {
-    u64 k0 = 0;
-    for (int i = t; i < all; i += 256) {
-      const u64 key = keys[i];
-      if (key < last && key > k0) k0 = key;
-    }
-    k0 = wave_max(k0);
-    __syncthreads();
-    if (lane == 0) s_key[w] = k0;
-    __syncthreads();
-    last = k0 = larger_of(larger_of(s_key[0], s_key[1]), larger_of(s_key[2], s_key[3]));
-    if (t == 0) write_alternative(a, row, j, k0, ref, ll);
-  }
+  done();
 }
 
 struct ScoreBwdArgs {
@@ -488,7 +521,7 @@ struct ScoreBwdArgs {
 // A wave takes 4 units of 16 bytes per lane of a row: read, and written once
 template <typename T, typename O>
 __global__ __launch_bounds__(256) void k_score_bwd(ScoreBwdArgs a) {
-  typedef Unit<T> U;
+  typedef Unit<T, WIDE<T>> U;
   constexpr int E = U::E, NU = 4;
   const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -556,7 +589,7 @@ void launch_score(hipStream_t s, ScoreArgs& a) {
   a.slices = 1;
   a.width = (a.V + 7) / 8 * 8;
   if (a.V <= 512) {
-    k_score<T, 64, 8><<<waves, 256, 0, s>>>(a);
+    k_score<T, 64, 8, 4><<<waves, 256, 0, s>>>(a);  // units of 4: the columns of the threshold are alike
   } else if (a.V <= 1024) {
     k_score<T, 64, 16><<<waves, 256, 0, s>>>(a);
   } else if (a.V <= 4096) {
@@ -566,16 +599,21 @@ void launch_score(hipStream_t s, ScoreArgs& a) {
     const int most = few ? SLICE : 2 * SLICE;
     a.slices = (a.V + most - 1) / most;
     a.width = ((a.V + a.slices - 1) / a.slices + 7) / 8 * 8;  // alike, so that they end together
-    if (few)
-      k_score<T, 256, 32><<<rows * a.slices, 256, 0, s>>>(a);
-    else
-      k_score<T, 256, 64><<<rows * a.slices, 256, 0, s>>>(a);
-    if (a.slices > 1) k_score_join<T><<<rows, 256, 0, s>>>(a);
+    if (few && a.slices > 1) {
+      a.number = sjh::call_number();
+      k_score<T, 256, 32, WIDE<T>, true><<<rows * a.slices, 256, 0, s>>>(a);
+    } else {
+      if (few)
+        k_score<T, 256, 32><<<rows, 256, 0, s>>>(a);
+      else
+        k_score<T, 256, 64><<<rows * a.slices, 256, 0, s>>>(a);
+      if (a.slices > 1) k_score_join<T><<<rows, 256, 0, s>>>(a);
+    }
   }
 }
 template <typename T>
 void launch_bwd(hipStream_t s, ScoreBwdArgs& a, int dx_dtype) {
-  const int chunk = 64 * Unit<T>::E * 4;
+  const int chunk = 64 * WIDE<T> * 4;
   a.chunks = (a.V + chunk - 1) / chunk;
   const unsigned blocks = (unsigned)((a.rows * a.chunks + 3) / 4);
   if (dx_dtype == SJ_BF16)
@@ -588,7 +626,7 @@ void launch_bwd(hipStream_t s, ScoreBwdArgs& a, int dx_dtype) {
 
 extern "C" size_t sj_token_logprobs_workspace_bytes(long rows, long vocab, long top) {
   if (rows <= 0 || vocab <= SLICE || top < 0) return 0;
-  return (size_t)rows * slices_of(vocab) * (16 + 8 * (size_t)top);
+  return (size_t)rows * slices_of(vocab) * (24 + 8 * (size_t)top);
 }
 
 extern "C" int sj_token_logprobs(void* stream, const void* x, int dtype, long ldx, long rows, long vocab,
@@ -610,7 +648,8 @@ extern "C" int sj_token_logprobs(void* stream, const void* x, int dtype, long ld
   ScoreArgs a = {};
   a.x = x; a.ldx = ldx; a.rows = rows; a.V = (int)vocab; a.top = (int)top;
   a.tokens = tokens; a.logprob = logprob; a.entropy = entropy; a.stats = stats; a.ids = top_ids; a.alt = top_logprob;
-  a.part = (uint8_t*)workspace;
+  a.flag = (u64*)workspace;
+  a.part = (uint8_t*)workspace + 8 * (size_t)rows * slices_of(vocab);
   if (dtype == SJ_BF16)
     launch_score<bf16_t>((hipStream_t)stream, a);
   else

@@ -38,12 +38,13 @@ class Score:
         self.lp, self.ent, self.stats = (G.dev(np.full(k * self.n + 4, 55.0)) for k in (1, 1, 2))
         self.ids = PU.ints(np.full(self.n * top + 4, 99))
         self.alt = G.dev(np.full(self.n * top + 4, 55.0))
-        self.ws = G.empty(max(lib.sj_token_logprobs_workspace_bytes(self.n, self.V, top), 16), "u8")
+        self.need = lib.sj_token_logprobs_workspace_bytes(self.n, self.V, top)
+        self.ws = G.Dev(max(self.need, 16), "u8").upload(np.full(max(self.need, 16), 0xFF))  # nothing is kept there
 
     def forward(self, stream=None):
         native()[0].api.sj_token_logprobs(stream, self.x.at(self.off), CODE[self.dtype], self.ld, self.n, self.V,
                                           self.tokens.p, self.top, self.lp.p, self.ent.p, self.stats.p, self.ids.p,
-                                          self.alt.p, self.ws.p, self.ws.nbytes)
+                                          self.alt.p, self.ws.p, self.need)
 
     def host(self):
         out = [b.host() for b in (self.lp, self.ent, self.stats, self.ids, self.alt)]
@@ -111,7 +112,7 @@ def logits(rng, n, V, dtype, spread=2.0):
 @pytest.mark.parametrize("n,V,top,dtype,ld,offset", [
     (1, 1, 1, "f32", 0, 0), (3, 2, 2, "bf16", 0, 0), (5, 63, 5, "f32", 64, 1), (70, 257, 5, "f32", 264, 0),
     (33, 257, 20, "bf16", 257, 3), (9, 1000, 64, "f32", 1001, 0), (7, 4099, 8, "bf16", 0, 1), (4, 8193, 32, "f32", 8200, 2),
-    (3, 32768, 20, "bf16", 0, 0), (2, 50001, 1, "bf16", 50008, 0), (2, 131072, 64, "f32", 0, 0), (17, 5000, 0, "f32", 0, 0),
+    (3, 32768, 20, "bf16", 0, 0), (1030, 8300, 3, "bf16", 8301, 0), (690, 16400, 9, "f32", 0, 0), (2, 50001, 1, "bf16", 50008, 0), (2, 131072, 64, "f32", 0, 0), (17, 5000, 0, "f32", 0, 0),
     (1, 200001, 33, "f32", 0, 1), (600, 300, 3, "bf16", 301, 0), (1030, 16, 4, "f32", 0, 0)])
 def test_scores_and_gradient(n, V, top, dtype, ld, offset):
     rng = np.random.default_rng(V + n)
@@ -274,6 +275,25 @@ def test_crowded_rows(V, top):
     s = Score(x, "f32", np.array([1, 2]), top)
     s.forward()
     check_forward(s.host(), x, np.array([1, 2]), top)
+
+
+def test_two_graphs_of_one_workspace():
+    """Rows of several slices meet in a workspace that two captured graphs share, replayed in turn."""
+    rng = np.random.default_rng(5)
+    both = [Score(logits(rng, n, V, "f32"), "f32", rng.integers(0, V, n), 7) for n, V in ((5, 20000), (2, 50000))]
+    need = max(s.need for s in both)
+    shared = G.Dev(need, "u8").upload(np.full(need, 0xFF))
+    for s in both:
+        s.ws = shared
+    graphs = [PU.Graph(s.forward) for s in both]
+    for _ in range(3):
+        for g, s in zip(graphs, both):
+            x = logits(rng, s.n, s.V, "f32")
+            s.x.upload(x)
+            g.replay()
+            check_forward(s.host(), x, s.tokens.host(), 7)
+    for g in graphs:
+        g.close()
 
 
 def test_crowded_slices():
