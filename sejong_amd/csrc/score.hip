@@ -65,6 +65,7 @@ struct Unit<float, EE> {
   static constexpr int E = EE;
   struct __attribute__((packed, aligned(4))) Raw { float v[E]; } r;
   __device__ __forceinline__ float get(int i) const { return r.v[i]; }
+  __device__ __forceinline__ void set(int i, float x) { r.v[i] = x; }
 };
 template <int EE>
 struct Unit<bf16_t, EE> {
@@ -73,6 +74,10 @@ struct Unit<bf16_t, EE> {
   __device__ __forceinline__ float get(int i) const {
     const uint32_t w = r.v[i >> 1];
     return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+  }
+  __device__ __forceinline__ void set(int i, float x) {
+    uint32_t& w = r.v[i >> 1];
+    w = i & 1 ? (w & 0xffffu) | ((uint32_t)f2bf(x) << 16) : (w & 0xffff0000u) | f2bf(x);
   }
 };
 template <typename T>
@@ -292,21 +297,19 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   // units past the end are left out everywhere; one that crosses it is filled
   // with -inf
   constexpr int PART = 4, PARTS = EV / PART;  // maxima of parts: the search below passes those without
-  float f[EV], pm[PARTS], best = -INFINITY;
+  float pm[PARTS], best = -INFINITY;
+  auto f = [&](int i) { return u[i / E].get(i % E); };  // as stored: bf16 entries are widened at each use
 #pragma unroll
   for (int i = 0; i < NU; i++) {
     const int v = base + E * (t + NT * i);
     if (v < end) {
-      if (v + E <= end) {
+      if (v + E > end) {
 #pragma unroll
-        for (int e = 0; e < E; e++) f[i * E + e] = u[i].get(e);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; e++) f[i * E + e] = v + e < end ? at_f32(x, v + e) : -INFINITY;
+        for (int e = 0; e < E; e++) u[i].set(e, v + e < end ? at_f32(x, v + e) : -INFINITY);
       }
 #pragma unroll
       for (int j = i * E / PART; j < (i + 1) * E / PART; j++) {
-        pm[j] = fmaxf(fmaxf(f[PART * j], f[PART * j + 1]), fmaxf(f[PART * j + 2], f[PART * j + 3]));
+        pm[j] = fmaxf(fmaxf(f(PART * j), f(PART * j + 1)), fmaxf(f(PART * j + 2), f(PART * j + 3)));
         best = fmaxf(best, pm[j]);
       }
     }
@@ -348,11 +351,11 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
       if (v + E > end && ref > -1e20f) {  // the filling: a share of 0 and no NaN
 #pragma unroll
         for (int e = 0; e < E; e++)
-          if (v + e >= end) f[i * E + e] = -1e30f;
+          if (v + e >= end) u[i].set(e, -1e30f);
       }
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const float d = fmaf(f[i * E + e], LOG2E, -c), y = __builtin_amdgcn_exp2f(d);
+        const float d = fmaf(f(i * E + e), LOG2E, -c), y = __builtin_amdgcn_exp2f(d);
         rest += y;
         xs = fmaf(y, d, xs);
       }
@@ -371,7 +374,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
       if (base + E * (t + NT * i) < end)
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          const float y = f[i * E + e];
+          const float y = f(i * E + e);
           const bool out = !left && y == skip;
           left |= out;
           const float d = y - ref, p = out ? 0.f : __builtin_amdgcn_exp2f(d * LOG2E);
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   for (int j = 0; j < PARTS; j++)
     if (index(PART * j) < end && pm[j] >= T0)
 #pragma unroll
-      for (int i = PART * j; i < PART * (j + 1); i++) mine += f[i] >= T0 && index(i) < end;
+      for (int i = PART * j; i < PART * (j + 1); i++) mine += f(i) >= T0 && index(i) < end;
   const uint32_t upto = scan_add(mine);
   int from = 0;
   if (lane == 63 && upto) from = atomicAdd(&s_n[gt], (int)upto);
@@ -451,8 +454,8 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     if (index(PART * j) < end && pm[j] >= T0) {
 #pragma unroll
       for (int i = PART * j; i < PART * (j + 1); i++)
-        if (f[i] >= T0 && index(i) < end) {
-          if (from < CAP) s_cand[gt][from] = order_key(f[i], index(i));
+        if (f(i) >= T0 && index(i) < end) {
+          if (from < CAP) s_cand[gt][from] = order_key(f(i), index(i));
           from++;
         }
     }
