@@ -27,11 +27,10 @@ struct PlanArgs {
   const int32_t *lengths, *counts, *free_pages, *head;
   int32_t *table, *after, *starts, *positions, *slots, *owners, *summary;
   long ldt, nfree, cap;
-  int R;
-  uint32_t P, pages;
+  int R, P;
+  Div d_page;
+  uint32_t pages;
 };
-
-__device__ __forceinline__ uint32_t ceil_div(uint32_t n, uint32_t d) { return n / d + (n % d != 0); }
 
 __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
   __shared__ uint32_t w_tok[4], w_need[4], w_want[4], w_long[4], w_bad[4];
@@ -44,25 +43,40 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
   const int per = (a.R + PT - 1) / PT;
   const int r0 = min(t * per, a.R), r1 = min(r0 + per, a.R);
   const int head = a.head ? a.head[0] : 0;
-  const int n0 = r0 < r1 ? a.lengths[r0] : 0, m0 = r0 < r1 ? a.counts[r0] : 0;
+  // the first of a thread's requests stay in registers (all of 2048)
+  constexpr int HELD = 8;
+  int hn[HELD], hm[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    hn[i] = r0 + i < r1 ? a.lengths[r0 + i] : 0;
+    hm[i] = r0 + i < r1 ? a.counts[r0 + i] : 0;
+  }
   // 32-bit sums are exact wherever the sum of the counts, watched in fp32, is
   // below 3e9: there are at most as many pages to take as tokens and requests
   uint32_t tok = 0, need = 0, want = 0, longest = 0, bad = 0;
   float size = 0.f;
-#pragma unroll 1
-  for (int r = r0; r < r1; r++) {
-    const int n = r == r0 ? n0 : a.lengths[r], m = r == r0 ? m0 : a.counts[r];
-    if ((n | m) < 0) {
+  auto pages_of = [&](int n) {
+    const int q = div(n, a.d_page);
+    return (uint32_t)(q + (q * a.P != n));
+  };
+  auto count = [&](int n, int m) {
+    const uint32_t after = (uint32_t)n + (uint32_t)m;
+    if ((n | m) < 0 || (int)after < 0) {
       bad = 1;
     } else {
-      const uint32_t w = ceil_div((uint32_t)n + (uint32_t)m, a.P);
+      const uint32_t w = pages_of((int)after);
       tok += m;
       size += (float)m;
-      need += w - ceil_div((uint32_t)n, a.P);
+      need += w - pages_of(n);
       want = max(want, w);
-      longest = max(longest, (uint32_t)n + (uint32_t)m);
+      longest = max(longest, after);
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; i++)
+    if (i < per) count(hn[i], hm[i]);  // past the last request 0 and 0, which count for nothing
+#pragma unroll 1
+  for (int r = r0 + HELD; r < r1; r++) count(a.lengths[r], a.counts[r]);
   uint32_t st = scan_add(tok), sn = scan_add(need);
   want = wave_max(want);
   longest = wave_max(longest);
@@ -89,7 +103,7 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
   if (head < 0 || huge || (long)head + all_need > a.nfree) status |= SJ_PLAN_NO_PAGES;
   if (want > (unsigned long)a.ldt) status |= SJ_PLAN_TABLE_WIDTH;
   if (huge || all_tok > a.cap) status |= SJ_PLAN_ROWS;
-  if (bad || longest > 0x7fffffffu) status |= SJ_PLAN_LENGTHS;
+  if (bad) status |= SJ_PLAN_LENGTHS;
   const bool ok = status == 0;
 
   // the requests again with their places; a request's page ids are asked for
@@ -97,16 +111,13 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
   const long t0 = (long)blockIdx.x * PTOK;
   uint32_t s = st - tok, f = sn - need;
   const bool lead = blockIdx.x == 0;
-#pragma unroll 1
-  for (int r = r0; r < r1; r++) {
-    const int n = r == r0 ? n0 : a.lengths[r], m = r == r0 ? m0 : a.counts[r];
+  auto mark = [&](int r, int n, int m) {
     if (lead) {
       a.starts[r] = ok ? (int)s : 0;
       if (a.after) a.after[r] = ok ? n + m : n;
     }
-    if (!ok) continue;
-    const uint32_t in = (uint32_t)n / a.P, have = ceil_div((uint32_t)n, a.P);
-    const uint32_t take = ceil_div((uint32_t)n + (uint32_t)m, a.P) - have;
+    if (!ok) return;
+    const uint32_t in = div(n, a.d_page), have = pages_of(n), take = pages_of(n + m) - have;
     if (m > 0 && s < t0 + PTOK && (long)s + m > t0) {
       const int at = s > t0 ? (int)(s - t0) : 0;
       const int tail = in < have ? a.table[(long)r * a.ldt + in] : -1;
@@ -120,13 +131,18 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
     }
     s += m;
     f += take;
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; i++)
+    if (r0 + i < r1) mark(r0 + i, hn[i], hm[i]);
+#pragma unroll 1
+  for (int r = r0 + HELD; r < r1; r++) mark(r, a.lengths[r], a.counts[r]);
   if (lead && t == 0) {
     a.starts[a.R] = ok ? (int)all_tok : 0;
     a.summary[0] = ok ? (int)all_tok : 0;
     a.summary[1] = head + (ok ? (int)all_need : 0);
     a.summary[2] = status;
-    a.summary[3] = longest > 0x7fffffffu ? 0x7fffffff : (int)longest;
+    a.summary[3] = (int)longest;
   }
   __syncthreads();
   // each token's request: the last mark at or before it (places from 1, 0: none)
@@ -154,7 +170,7 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
     owner[i] = h_req[h];
     const int n = h_len[h];
     pos[i] = n + (int)(g - h_start[h]);
-    const uint32_t col = (uint32_t)pos[i] / a.P, off = (uint32_t)pos[i] - col * a.P, have = ceil_div((uint32_t)n, a.P);
+    const uint32_t col = div(pos[i], a.d_page), off = (uint32_t)pos[i] - col * a.P, have = pages_of(n);
     int page = h_tail[h];
     if (col >= have) {
       page = col == have ? h_fresh[h] : a.free_pages[(long)head + h_first[h] + (col - have)];
@@ -200,13 +216,6 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
 // operands are single values, takes V as it lies; nothing is rounded.
 // The loads of a tile are in flight while the one before is computed, its page
 // ids one tile earlier still.
-
-// n / d for n < 2^31 by multiplication: mul = floor(2^32 (2^shift - d) / d) + 1
-// with 2^shift >= d; the added n is the 33rd bit of 2^32 + mul
-struct Div {
-  uint32_t mul, shift;
-};
-__device__ __forceinline__ int div(int n, Div d) { return (int)((__umulhi(d.mul, (uint32_t)n) + (uint32_t)n) >> d.shift); }
 
 struct PagedArgs {
   const void* q;
@@ -790,7 +799,7 @@ __global__ __launch_bounds__(256) void k_paged_rows(PagedArgs a) {
     const long j = base + lane;
     int sl = -1;
     if (j < hi) {
-      const int col = (int)(j / a.P), pg = pages[col];
+      const int col = div((int)j, a.d_page), pg = pages[col];
       if (pg >= 0 && pg < a.pages) sl = pg * a.P + (int)(j - (long)col * a.P);
     }
     float s = -INFINITY;
@@ -865,7 +874,8 @@ extern "C" int sj_paged_plan(void* stream, const int32_t* lengths, const int32_t
   a.table = table; a.after = lengths_after; a.starts = starts; a.positions = positions; a.slots = slots;
   a.owners = owners; a.summary = summary;
   a.ldt = ldt; a.nfree = free_count; a.cap = capacity;
-  a.R = (int)requests; a.P = (uint32_t)page_size; a.pages = (uint32_t)pages;
+  a.R = (int)requests; a.P = (int)page_size; a.pages = (uint32_t)pages;
+  a.d_page = make_div((uint32_t)page_size);
   const long blocks = capacity > PTOK ? (capacity + PTOK - 1) / PTOK : 1;
   k_paged_plan<<<(unsigned)blocks, PT, 0, (hipStream_t)stream>>>(a);
   SJ_LAUNCH_CHECK("paged plan");
@@ -873,13 +883,6 @@ extern "C" int sj_paged_plan(void* stream, const int32_t* lengths, const int32_t
 }
 
 namespace {
-
-Div make_div(uint32_t d) {
-  Div r = {0, 0};
-  while ((1ul << r.shift) < d) r.shift++;
-  r.mul = (uint32_t)((((1ul << r.shift) - d) << 32) / d + 1);
-  return r;
-}
 
 // whether sj_paged_attention may split: by sizes alone, so that the workspace
 // query knows it too

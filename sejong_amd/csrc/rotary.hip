@@ -16,7 +16,7 @@
 // and the write of the rows.
 #include <math.h>
 
-#include "common.h"
+#include "lanes.h"
 
 using namespace sj;
 
@@ -25,19 +25,6 @@ namespace {
 constexpr int RT = 256;
 constexpr int RPAIRS = 1024;  // at most this many (row, pair) angles of a workgroup in LDS
 constexpr int RU = 4;         // units of a thread
-
-// n / d for n < 2^31 by multiplication: mul = floor(2^32 (2^shift - d) / d) + 1
-// with 2^shift >= d
-struct Div {
-  uint32_t mul, shift;
-};
-Div make_div(uint32_t d) {
-  Div r = {0, 0};
-  while ((1ul << r.shift) < d) r.shift++;
-  r.mul = (uint32_t)((((1ul << r.shift) - d) << 32) / d + 1);
-  return r;
-}
-__device__ __forceinline__ int div(int n, Div d) { return (int)((__umulhi(d.mul, (uint32_t)n) + (uint32_t)n) >> d.shift); }
 
 // one frequency per thread, in double
 __global__ void k_rope_frequencies(uint64_t* turns, int half, sj_rope_scaling s) {
