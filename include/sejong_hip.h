@@ -138,7 +138,7 @@ int sj_rope_frequencies(void *stream, uint64_t *turns, long rotary_dim, const sj
  * is good to 2^-22 up to position 2^27.  x and y fp32 or bf16 (stored value in, fp32
  * products, one rounding); y may be x.  head_dim even, at most 1024; any
  * strides and element alignment (16-byte rows are fastest).  turns may be
- * null when rotary_dim is 0; at most 2^24 rows and 2^14 heads. */
+ * null when rotary_dim is 0; below 2^24 rows, at most 2^14 heads. */
 #define SJ_ROPE_INTERLEAVED 0
 #define SJ_ROPE_HALF 1
 int sj_rope_rows(void *stream, const void *x, long ldx, void *y, long ldy, int dtype, long rows, long heads,
@@ -408,7 +408,7 @@ int sj_paged_plan(void *stream, const int32_t *lengths, const int32_t *counts, l
  * keys rotated and values copied into the cache rows of their slots; the
  * rotation as sj_rope_rows.  A row whose slot is not in 0 .. cache_slots - 1
  * is left out whole (q_out too).  The slots of one call are distinct.  q_out
- * may be q; hq may be 0.  Any strides and element alignment; at most 2^24 rows, hq and hk
+ * may be q; hq may be 0.  Any strides and element alignment; below 2^24 rows, hq and hk
  * at most 2^14. */
 int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, int dtype,
                     long rows, long hq, long hk, long head_dim, long rotary_dim, int layout, const int32_t *positions,
@@ -420,13 +420,13 @@ int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long l
  * scale head_dim^-1/2.  Several rows may belong to one request (drafted
  * tokens, chunks of a prompt).  o [rows][ldo] in the q dtype, lse (nullable)
  * fp32 [rows][hq] natural log of the sum of exp(score).  Keys whose page id is
- * not in 0 .. pages - 1, and scores of -inf, have no share; a row without any
+ * not in 0 .. pages - 1, and scores of -inf (of finite values), have no share; a row without any
  * key gives o = 0 and lse = -inf; rows with position or owner below 0 (or an
  * owner past the requests) are left as they were.  Slots past a request's
  * length are never read into a result, whatever they hold.  head_dim at most
  * 256; rows times hk at most 2^23; any strides and element alignment.  Workspace:
- * sj_paged_attention_workspace_bytes, not cleared and not kept; calls that
- * share one must not overlap. */
+ * sj_paged_attention_workspace_bytes, 16-byte aligned, not cleared and not
+ * kept; calls that share one must not overlap. */
 size_t sj_paged_attention_workspace_bytes(long rows, long hq, long hk, long head_dim);
 int sj_paged_attention(void *stream, const void *q, long ldq, const void *k_cache, const void *v_cache, long ldkv,
                        int dtype, long pages, long page_size, const int32_t *table, long ldt, long requests,
@@ -729,10 +729,12 @@ int sj_cross_entropy(void *stream, const float *x, long ldx, const int32_t *targ
  * [rows][top].  logprob (then tokens too), entropy and stats are nullable.
  * Entries of -inf have no share; a row of nothing else has entropy 0, log
  * probabilities -inf and stats (0, 0).  A NaN makes its row's numbers NaN and
- * is ranked behind everything.  top at most SJ_LOGPROBS_MAX_TOP and vocab;
- * vocab at most 2^24, and rows times vocab / 8192 (rounded up) too.
+ * is ranked behind everything; +inf is ranked first, its row's numbers are not
+ * defined.  top at most SJ_LOGPROBS_MAX_TOP and vocab;
+ * vocab at most 2^24; rows times vocab / 8192 (rounded up) below 2^23.
  * Any stride and element alignment.  Workspace:
- * sj_token_logprobs_workspace_bytes, not cleared and not kept. */
+ * sj_token_logprobs_workspace_bytes, 16-byte aligned, not cleared and not
+ * kept; calls that share one must not overlap. */
 #define SJ_LOGPROBS_MAX_TOP 64
 size_t sj_token_logprobs_workspace_bytes(long rows, long vocab, long top);
 int sj_token_logprobs(void *stream, const void *x, int dtype, long ldx, long rows, long vocab, const int32_t *tokens,

@@ -18,7 +18,9 @@ namespace {
 // (a few KB that stay in L2, one block scan) and expands 1024 tokens, four to
 // a thread, so the plan is one launch and needs no workspace: the bound is
 // that launch, the chain of loads lengths -> page ids, and, for prompts, the
-// 12 bytes written per token.
+// 12 bytes written per token.  64 requests of one token 4.4 us (a launch is
+// 3.7), 1500 requests of 395000 tokens 8.1 (with one token a thread and 1024
+// threads a workgroup 5.7 and 16.2).
 
 constexpr int PT = 256;    // threads of a workgroup
 constexpr int PTOK = 1024; // its tokens
@@ -215,7 +217,9 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
 // plane costs matrix time that is free here.  fp32: the fp32 MFMA, whose
 // operands are single values, takes V as it lies; nothing is rounded.
 // The loads of a tile are in flight while the one before is computed, its page
-// ids one tile earlier still.
+// ids one tile earlier still.  64 requests of 4000 to 16384 keys, 8 KV heads of
+// 128, bf16: 2.3 GB in 424 us (5.4 TB/s, above a copy's 5.1); one wave per row
+// and head without the matrix cores took 4748.
 
 struct PagedArgs {
   const void* q;
@@ -647,10 +651,12 @@ __global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArg
 // one piece is written as it is; of a walk that is cut, each workgroup leaves
 // its totals in the workspace, and the last (meet, lanes.h) joins them in the
 // order of the keys.  A workgroup has at most two cut walks, the end of one
-// and the beginning of another.
-//
+// and the beginning of another.  45 requests of 1 to 6000 keys, 4 KV heads of
+// 64: 16.8 us, of which the walks are 6 (32 MB), the rows' sums before them 2.5
+// and the meeting behind them 5; with the join as a launch of its own 16.7 and
+// for one request of 1000 keys 11.6 against 10.4.
 constexpr int STREAM_ROWS = 2048;
-// workgroups: as many as 256 CUs hold at once (by registers), at most 768
+// workgroups that 256 CUs hold at once (by registers), and the most there are
 constexpr int split_per_cu(int dc) { return dc == 8 ? 1 : dc == 2 || dc == 3 ? 3 : 2; }
 constexpr int STREAM_GROUPS = 1024;
 
@@ -669,7 +675,8 @@ __global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs
     n[i] = 0;
     const int r = t * per + i;
     int owner, lo, hi;
-    if (i < per && r < a.rows && row_range(a, r, owner, lo, hi)) n[i] = (hi - lo + 4 * W::KT - 1) / (4 * W::KT);
+    if (i < per && r < a.rows && row_range(a, r, owner, lo, hi))
+      n[i] = max(1, (hi - lo + 4 * W::KT - 1) / (4 * W::KT));  // a row without keys is written too
     mine += n[i];
   }
   int at = (int)scan_add((uint32_t)mine);
@@ -983,6 +990,7 @@ extern "C" int sj_paged_attention(void* stream, const void* q, long ldq, const v
   if (rows == 0 || requests == 0) return SJ_OK;
   SJ_REQUIRE(q && k_cache && v_cache && table && positions && o, "paged attention: null");
   const size_t need = sj_paged_attention_workspace_bytes(rows, hq, hk, head_dim);
+  SJ_REQUIRE(((uintptr_t)workspace & 15) == 0, "paged attention: the workspace is not 16-byte aligned");
   if (need > workspace_bytes || (need && !workspace))
     return sjh::fail(SJ_ERR_CAPACITY, "paged attention workspace: required %zu bytes, available %zu bytes", need,
                      workspace ? workspace_bytes : 0);

@@ -13,7 +13,9 @@
 // its range reduction.  A workgroup asks for all its elements first (up to four
 // units a thread), forms the cosines and sines of its rows once in LDS while
 // they come, and all the heads of those rows read them: the bound is the read
-// and the write of the rows.
+// and the write of the rows.  16384 rows of 20 heads of 64, bf16: 16.5 us (5.1
+// TB/s, a copy's rate; one unit at a time behind the angles 28); 4099 rows of 6
+// heads of 96, fp32: 5.1; 104 rows with the append: 4.0, a launch.
 #include <math.h>
 
 #include "lanes.h"
@@ -241,7 +243,7 @@ extern "C" int sj_rope_rows(void* stream, const void* x, long ldx, void* y, long
              "rope rows dimensions");
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && y && positions && (turns || rotary_dim == 0), "rope rows: null");
-  SJ_REQUIRE(rows <= 1L << 24, "rope rows: %ld rows", rows);
+  SJ_REQUIRE(rows < 1L << 24, "rope rows: %ld rows", rows);
   RopeArgs a = {};
   a.seg[0] = RopeSeg{x, ldx, y, ldy, (int)heads, 1, 0};
   a.nseg = 1;
@@ -271,7 +273,7 @@ extern "C" int sj_paged_append(void* stream, const void* q, long ldq, const void
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(k && v && positions && slots && (turns || rotary_dim == 0) && k_cache && v_cache && (hq == 0 || (q && q_out)),
              "paged append: null");
-  SJ_REQUIRE(rows <= 1L << 24, "paged append: %ld rows", rows);
+  SJ_REQUIRE(rows < 1L << 24, "paged append: %ld rows", rows);
   RopeArgs a = {};
   a.seg[0] = RopeSeg{q, ldq, q_out, ldqo, (int)hq, 1, 0};
   a.seg[1] = RopeSeg{k, ldk, k_cache, ldkv, (int)hk, 1, 1};

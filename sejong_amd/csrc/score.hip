@@ -25,13 +25,19 @@ namespace {
 // (64 disjoint sets of entries) has at least k entries at or above it and
 // rarely many more; those are collected in LDS and each finds its place by
 // counting the larger ones.  Rows longer than a slice are joined from the
-// slices' sums and lists by a second launch.
-// The bound is the read: per entry there are about 12 operations, one of them
-// an exponential.
+// slices' sums and lists: by the last of their workgroups where they are few,
+// by a second launch where they are many and the meeting's waits would cost
+// more than a launch (32 rows of 131072, 20 alternatives: 19.7 us with a
+// second launch, 14.4 without).
+// The bound is the read, and where an entry has 2 bytes the vector units: per
+// entry about 7 operations, one of them an exponential, and as much again per
+// thread for the threshold and the list.  2048 rows of 50001 bf16, 8
+// alternatives: forward 70 us (2.9 TB/s) and join 8, gradient 78 (5.2 TB/s, a
+// copy's rate); 1024 rows of 131072 fp32 97 us (5.5 TB/s).
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int CAP_SLICE = 1024;  // entries at or above the threshold that LDS holds of a slice
-constexpr int SLICE = 8192;  // entries of a workgroup's slice where the slices are few; twice as many where they are not
+constexpr int SLICE = 8192;      // entries of a slice; twice as many where slices of bf16 are many
 
 typedef unsigned long long u64;
 
@@ -379,7 +385,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
           left |= out;
           const float d = y - ref, p = out ? 0.f : __builtin_amdgcn_exp2f(d * LOG2E);
           rest += p;
-          xs = fmaf(p, fmaxf(d, -1e30f), xs);
+          xs = fmaf(p, fmaxf(d, -1e4f), xs);  // below -104 a share is 0
         }
   };
   // -inf or NaN among the entries, or a reference whose rounding leaves the
@@ -546,7 +552,7 @@ __global__ __launch_bounds__(256) void k_score_bwd(ScoreBwdArgs a) {
   auto grad = [&](float y) {
     const float lp = y - m - ll, p = __builtin_amdgcn_exp2f(lp * LOG2E);
     // a share of 0 (lp = -inf) has none of the entropy's part; a NaN is in p
-    return -p * (dlp + dh * (fmaxf(lp, -1e30f) + H));
+    return -p * (dlp + dh * (fmaxf(lp, -1e4f) + H));
   };
 #pragma unroll
   for (int i = 0; i < NU; i++) {
@@ -578,7 +584,7 @@ __global__ __launch_bounds__(256) void k_score_bwd(ScoreBwdArgs a) {
   const int mine = tk - base;
   if (scored && mine >= 0 && mine < 64 * E * NU && (mine / E) % 64 == lane) {
     const float lp = yt - m - ll, p = __builtin_amdgcn_exp2f(lp * LOG2E);
-    const float d = fmaf(dlp, -expm1f(lp), -p * (dh * (fmaxf(lp, -1e30f) + H)));
+    const float d = fmaf(dlp, -expm1f(lp), -p * (dh * (fmaxf(lp, -1e4f) + H)));
     if constexpr (sizeof(O) == 2) dx[tk] = f2bf(d); else dx[tk] = d;
   }
 }
@@ -643,11 +649,12 @@ extern "C" int sj_token_logprobs(void* stream, const void* x, int dtype, long ld
              "token log probabilities: %ld rows of %ld (stride %ld)", rows, vocab, ldx);
   SJ_REQUIRE(top >= 0 && top <= SJ_LOGPROBS_MAX_TOP && top <= vocab, "token log probabilities: %ld alternatives of %ld",
              top, vocab);
-  SJ_REQUIRE(rows <= (1L << 24) / slices_of(vocab), "token log probabilities: %ld rows of %ld", rows, vocab);
+  SJ_REQUIRE(rows < (1L << 23) / slices_of(vocab), "token log probabilities: %ld rows of %ld", rows, vocab);
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && (logprob == nullptr || tokens) && (top == 0 || (top_ids && top_logprob)),
              "token log probabilities: null");
   const size_t need = sj_token_logprobs_workspace_bytes(rows, vocab, top);
+  SJ_REQUIRE(((uintptr_t)workspace & 15) == 0, "token log probabilities: the workspace is not 16-byte aligned");
   if (need > workspace_bytes || (need && !workspace))
     return sjh::fail(SJ_ERR_CAPACITY, "token log probabilities workspace: required %zu bytes, available %zu bytes", need,
                      workspace ? workspace_bytes : 0);
@@ -671,7 +678,7 @@ extern "C" int sj_token_logprobs_bwd(void* stream, const void* x, int dtype, lon
              "token log probabilities backward dtypes %d, %d", dtype, dx_dtype);
   SJ_REQUIRE(rows >= 0 && rows <= 0x7fffffffL && vocab > 0 && vocab <= 1L << 24 && ldx >= vocab && lddx >= vocab,
              "token log probabilities backward: %ld rows of %ld (strides %ld, %ld)", rows, vocab, ldx, lddx);
-  SJ_REQUIRE(rows <= (1L << 24) / slices_of(vocab), "token log probabilities backward: %ld rows of %ld", rows, vocab);
+  SJ_REQUIRE(rows < (1L << 23) / slices_of(vocab), "token log probabilities backward: %ld rows of %ld", rows, vocab);
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && stats && dx && (dlogprob == nullptr || tokens) && (dentropy == nullptr || entropy),
              "token log probabilities backward: null");

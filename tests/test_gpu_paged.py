@@ -370,6 +370,17 @@ def test_attention_bad_pages_and_empty_rows(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lengths,D", [([40, 70, 20], 64), ([40, 7000, 20, 3000], 64), ([40, 70], 20)])
+def test_attention_windows_past_the_table(dtype, lengths, D):
+    """A position so far past its table that the window holds none of its keys: 0 and -inf, in every form."""
+    a = Attend(2, dtype, 6, 2, D, 16, lengths, window=2000 if max(lengths) > 2000 else 30)
+    a.pos[0] = 100000
+    a.pos[-1] = a.width * 16 + 5
+    want = a.upload().run().check()
+    assert (want[0][0] == 0).all() and (want[0][1] == -np.inf).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_scores_without_a_share(dtype):
     """Keys whose score is -inf, some of a row's or all of them; scores near the type's limits."""
     a = Attend(4, dtype, 4, 2, 64, 16, [70, 70, 130])

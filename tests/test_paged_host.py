@@ -137,11 +137,15 @@ def test_short_workspaces_are_refused():
     if need:
         refused("sj_paged_attention", changed(ATTEND, workspace=X, workspace_bytes=need - 1), 2, b"required %d bytes" % need)
         refused("sj_paged_attention", changed(ATTEND, workspace=None, workspace_bytes=need), 2, b"available 0 bytes")
+        odd = ctypes.c_void_p(0x1008)
+        refused("sj_paged_attention", changed(ATTEND, workspace=odd, workspace_bytes=need), 1, b"16-byte aligned")
     need = lib.sj_token_logprobs_workspace_bytes(4, 150000, 5)
     if need:
         big = dict(vocab=150000, ldx=150000)
         refused("sj_token_logprobs", changed(SCORE, workspace=X, workspace_bytes=need - 1, **big), 2,
                 b"required %d bytes" % need)
+        refused("sj_token_logprobs", changed(SCORE, workspace=ctypes.c_void_p(0x1004), workspace_bytes=need, **big), 1,
+                b"16-byte aligned")
 
 
 def test_the_gradient_formula_against_differences():
