@@ -370,7 +370,7 @@ def test_attention_bad_pages_and_empty_rows(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("lengths,D", [([40, 70, 20], 64), ([40, 7000, 20, 3000], 64), ([40, 70], 20)])
+@pytest.mark.parametrize("lengths,D", [([40, 70, 20], 64), ([40, 7000, 20, 3000], 64), ([40, 70, 20], 20)])
 def test_attention_windows_past_the_table(dtype, lengths, D):
     """A position so far past its table that the window holds none of its keys: 0 and -inf, in every form."""
     a = Attend(2, dtype, 6, 2, D, 16, lengths, window=2000 if max(lengths) > 2000 else 30)
