@@ -952,7 +952,7 @@ int attend(hipStream_t s, PagedArgs& a, long most, void* workspace) {
     // uneven, not long.  us, direct / split, bf16: heads of 64, 1 request x 2
     // of 512 keys 7.8 / 10.1, of 1024 11.6 / 10.6, of 8192 62 / 11.6; 64 x 2 of
     // 1024 12.8 / 14.9, of 4096 40 / 39; 64 x 8 of 1024 34 / 42, of 4096 117 /
-    // 127, of 8192 228 / 243 (but 45 x 4 of 1 to 6000 32 / 17); heads of 128,
+    // 127, of 8192 228 / 243 (but 45 x 4 of 1 to 6000 47 / 17); heads of 128,
     // 256 x 8 of 1024 200 / 188
     direct = direct || tiles <= 8 || (units >= 128 && tiles <= 16) || (units >= 512 && units < 2048 && tiles <= 64);
     if (direct) st = launch_direct(s, a, tiles <= 4 || units >= 1024 ? 4 : 8, w);

@@ -25,10 +25,10 @@ namespace {
 // (64 disjoint sets of entries) has at least k entries at or above it and
 // rarely many more; those are collected in LDS and each finds its place by
 // counting the larger ones.  Rows longer than a slice are joined from the
-// slices' sums and lists: by the last of their workgroups where they are few,
-// by a second launch where they are many and the meeting's waits would cost
-// more than a launch (32 rows of 131072, 20 alternatives: 19.7 us with a
-// second launch, 14.4 without).
+// slices' sums and lists: by the last of their workgroups up to 1024 slices, by
+// a second launch where they are more.  us, meeting / second launch: 32 rows of
+// 50001 fp32 7.2 / 8.0, with 20 alternatives of 131072 14.0 / 14.1; 1024 slices
+// (512 rows of 16384) 11.8 / 12.2; 1792 (256 of 50008) 17.2 / 15.3.
 // The bound is the read, and where an entry has 2 bytes the vector units: per
 // entry about 7 operations, one of them an exponential, and as much again per
 // thread for the threshold and the list.  2048 rows of 50001 bf16, 8
@@ -102,13 +102,14 @@ struct ScoreArgs {
   float* alt;
   u64* flag;      // [rows][slices], of the meetings
   u64 number;
-  uint8_t* part;  // per row: (m, rest, xs, -) of each slice, then each slice's `top` keys
+  float* sums;    // [rows][slices] of (m, rest, xs, -)
+  u64* keys;      // [rows][slices][top]
 };
 __device__ __forceinline__ float* part_sums(const ScoreArgs& a, long row) {
-  return (float*)(a.part + row * a.slices * (16 + 8L * a.top));
+  return a.sums + row * a.slices * 4;
 }
 __device__ __forceinline__ u64* part_keys(const ScoreArgs& a, long row) {
-  return (u64*)(a.part + row * a.slices * (16 + 8L * a.top) + 16L * a.slices);
+  return a.keys + row * a.slices * a.top;
 }
 
 // what every thread of a row's group knows of its token, asked for early
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   constexpr int NU = EV / E, NW = NT / 64, GROUPS = 256 / NT, CAP = NT == 64 ? 64 * EV : CAP_SLICE;
   __shared__ __attribute__((aligned(16))) float s_best[256];
   __shared__ u64 s_cand[GROUPS][CAP], s_last[4];
-  __shared__ float s_max[4], s_sum[2][2][4], s_T[GROUPS];
+  __shared__ float s_max[4], s_sum[2][2][4], s_T[4];
   __shared__ int s_n[GROUPS];
   const int gt = threadIdx.x / NT, t = threadIdx.x % NT, lane = threadIdx.x & 63, w = t >> 6;
   auto sync = [] {
@@ -328,21 +329,26 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
     sync();
     m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
   }
-  // the threshold, by the first wave of the group
-  if (w == 0 && top) {
+  // The threshold.  Up to 32 alternatives by the first wave of the group from
+  // 64 columns, for more of them by every wave from the threads' 256: the 64th
+  // largest of 64 would be the least, with some 300 entries above it and at
+  // times 1000 (2048 rows of 32000 bf16, 64 alternatives: 133 -> 74 us).
+  if (top && (w == 0 || top > 32)) {
+    const bool all = NT > 64 && top > 32;
     float col = best;
-    if (NT > 64) col = fmaxf(fmaxf(best, s_best[lane + 64]), fmaxf(s_best[lane + 128], s_best[lane + 192]));
+    if (NT > 64 && !all) col = fmaxf(fmaxf(best, s_best[lane + 64]), fmaxf(s_best[lane + 128], s_best[lane + 192]));
     float* cols = s_best + (NT > 64 ? 0 : gt * 64);
-    cols[lane] = col;
+    if (!all) cols[lane] = col;
     sync_wave();
     int larger = 0;
+    for (int j = 0; j < (all ? 256 : 64); j += 64)
 #pragma unroll
-    for (int i = 0; i < 64; i += 4) {
-      const f32x4 c = *(const f32x4*)(cols + i);
-      larger += (c[0] > col) + (c[1] > col) + (c[2] > col) + (c[3] > col);
-    }
+      for (int i = 0; i < 64; i += 4) {
+        const f32x4 c = *(const f32x4*)(cols + j + i);
+        larger += (c[0] > col) + (c[1] > col) + (c[2] > col) + (c[3] > col);
+      }
     const float least = all_min(larger < top ? col : INFINITY);
-    if (lane == 0) s_T[gt] = least;
+    if (NT == 64 ? lane == 0 : all ? lane == 0 : lane < 4) s_T[NT == 64 ? gt : all ? w : lane] = least;
   }
   const float ref = m == -INFINITY ? 0.f : m;
   float rest = 0.f, xs = 0.f;
@@ -443,7 +449,7 @@ __global__ __launch_bounds__(256) void k_score(ScoreArgs a) {
   };
   if (!top) return done();
   sync();
-  const float T0 = s_T[gt];
+  const float T0 = NT == 64 ? s_T[gt] : fminf(fminf(s_T[0], s_T[1]), fminf(s_T[2], s_T[3]));
   // counted first, so that a wave takes its places in the list at once
   uint32_t mine = 0;
 #pragma unroll
@@ -604,9 +610,10 @@ void launch_score(hipStream_t s, ScoreArgs& a) {
   } else if (a.V <= 4096) {
     k_score<T, 256, 16><<<rows, 256, 0, s>>>(a);
   } else {
-    const bool few = a.V <= SLICE || a.rows * slices_of(a.V) < 2048;
+    const bool few = a.V <= SLICE || a.rows * slices_of(a.V) <= 1024;
     // entries a thread holds of a long slice: 64 of fp32 leave 3 waves a SIMD
-    // (2048 rows of 50008, 8 alternatives: 97 us, with 32 84; bf16 63, with 32 67)
+    // (2048 rows of 50008, 8 alternatives: 97 us, with 32 84); of bf16 1024
+    // rows of 131072 take 65 us, with 32 72
     constexpr int LONG = sizeof(T) == 2 ? 64 : 32;
     const int most = few ? SLICE : 256 * LONG;
     a.slices = (a.V + most - 1) / most;
@@ -661,8 +668,10 @@ extern "C" int sj_token_logprobs(void* stream, const void* x, int dtype, long ld
   ScoreArgs a = {};
   a.x = x; a.ldx = ldx; a.rows = rows; a.V = (int)vocab; a.top = (int)top;
   a.tokens = tokens; a.logprob = logprob; a.entropy = entropy; a.stats = stats; a.ids = top_ids; a.alt = top_logprob;
-  a.flag = (u64*)workspace;
-  a.part = (uint8_t*)workspace + 8 * (size_t)rows * slices_of(vocab);
+  const size_t all = (size_t)rows * slices_of(vocab);
+  a.sums = (float*)workspace;
+  a.flag = (u64*)workspace + 2 * all;
+  a.keys = a.flag + all;
   if (dtype == SJ_BF16)
     launch_score<bf16_t>((hipStream_t)stream, a);
   else

@@ -338,3 +338,52 @@ def test_captured_scores_replay(n, V):
         check_forward(s.host(), x, tokens, 6)
         check_backward(dx.host().reshape(n, V), x, tokens, np.ones(n), np.full(n, 0.5), "f32")
     g.close()
+
+
+@pytest.mark.parametrize("n,V,top,ld,offset", [
+    (530, 16384, 64, 16385, 3), (1030, 8200, 40, 8203, 0), (350, 24601, 5, 24601, 1), (520, 16377, 0, 16379, 7),
+    (260, 32768, 64, 32768, 8)])
+def test_many_long_rows_of_bf16(n, V, top, ld, offset):
+    """Many long rows that begin at any of the 8 places of 16 bytes; masked ends and beginnings, equal entries, a row
+    of nothing, NaN."""
+    rng = np.random.default_rng(V)
+    x = logits(rng, n, V, "bf16")
+    for r in range(9, n, 10):
+        x[r, :rng.integers(1, 40)] = -np.inf
+        x[r, V - rng.integers(1, 40):] = -np.inf
+    for r in range(16):  # each place twice: entries that count only at the ends, and equal ones
+        x[16 + r] = -np.inf
+        x[16 + r, 0] = x[16 + r, V - 1] = 1.0
+        x[32 + r] = -2.5
+        x[48 + r, :9] = x[48 + r, V - 9:] = 30.0
+    x[5] = -np.inf
+    x[6] = G.O.round_to(np.array([-3.38e38]), "bf16")[0]
+    tokens = rng.integers(0, V, n)
+    tokens[::2], tokens[1::4] = 0, V - 1
+    s = Score(x, "bf16", tokens, top, ld, offset)
+    s.forward()
+    check_forward(s.host(), x, tokens, top)
+    y = x[:8].copy()
+    y[3, 0], y[4, V - 1] = np.nan, np.nan
+    y = np.concatenate([y, x[8:]])
+    s = Score(y, "bf16", tokens, top, ld, offset)
+    s.forward()
+    got = s.host()
+    assert np.isnan(got["lp"][3:5]).all() and np.isnan(got["ent"][3:5]).all()
+    keep = np.r_[0:3, 5:n]
+    check_forward({k: v[keep] for k, v in got.items()}, x[keep], tokens[keep], top)
+
+
+@pytest.mark.parametrize("n,V,dtype", [(3, 1025, "bf16"), (2, 1025, "f32"), (300, 4096, "bf16"), (2, 8192, "f32"),
+                                       (3, 50001, "f32"), (530, 16390, "f32")])
+def test_long_lists(n, V, dtype):
+    """33, 48 and 64 alternatives, with entries of -inf that leave fewer than those, and -inf almost everywhere."""
+    rng = np.random.default_rng(n + V)
+    x = logits(rng, n, V, dtype)
+    x[0, 20:] = -np.inf
+    x[1, rng.permutation(V)[:V - 64]] = -np.inf
+    tokens = rng.integers(0, V, n)
+    for top in (33, 48, 64):
+        s = Score(x, dtype, tokens, top)
+        s.forward()
+        check_forward(s.host(), x, tokens, top)
