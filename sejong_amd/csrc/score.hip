@@ -21,8 +21,8 @@ namespace {
 // slice of it in registers: the maximum, then the sums relative to it.  Where
 // the sum of all terms is 2 or more, taking the 1 off loses nothing; where it
 // is less, the thread that holds the maximum sums again without it.
-// The alternatives come from a threshold: the k-th largest of 64 column maxima
-// (64 disjoint sets of entries) has at least k entries at or above it and
+// The alternatives come from a threshold: the k-th largest of 64 or 256 column
+// maxima (disjoint sets of entries) has at least k entries at or above it and
 // rarely many more; those are collected in LDS and each finds its place by
 // counting the larger ones.  Rows longer than a slice are joined from the
 // slices' sums and lists: by the last of their workgroups up to 1024 slices, by
