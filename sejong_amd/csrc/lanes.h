@@ -1,23 +1,10 @@
-// Division by multiplication; sums, maxima and scans over a wave with
-// data-parallel moves (no LDS); the meeting of workgroups that each hold a
-// part of a result.
+// Sums, maxima and scans over a wave with data-parallel moves (no LDS); the
+// meeting of workgroups that each hold a part of a result.
 #pragma once
 #include "common.h"
+#include "keys.h"
 
 namespace sj {
-
-// n / d for n < 2^31: mul = floor(2^32 (2^shift - d) / d) + 1 with 2^shift >=
-// d; the added n is the 33rd bit of 2^32 + mul
-struct Div {
-  uint32_t mul, shift;
-};
-inline Div make_div(uint32_t d) {
-  Div r = {0, 0};
-  while ((1ul << r.shift) < d) r.shift++;
-  r.mul = (uint32_t)((((1ul << r.shift) - d) << 32) / d + 1);
-  return r;
-}
-__device__ __forceinline__ int div(int n, Div d) { return (int)((__umulhi(d.mul, (uint32_t)n) + (uint32_t)n) >> d.shift); }
 
 // ------------------------------------------------ reductions and scans
 // Four steps within rows of 16 lanes, then the four rows' values as scalars,

@@ -319,16 +319,15 @@ struct Walk {
   __device__ __forceinline__ void look(const PagedArgs& a, const int32_t* pages, int base, int hi, int lane) {
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      const int j = base + 16 * s + (lane & 15);
-      pid[s] = j < hi ? pages[div(j, a.d_page)] : -1;
+      const uint32_t j = key_at(base, 16 * s + (lane & 15));
+      pid[s] = is_key(j, hi) ? pages[div(j, a.d_page)] : -1;
     }
   }
   __device__ __forceinline__ void place(const PagedArgs& a, int base, int lane) {
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      const int j = base + 16 * s + (lane & 15);
       const bool in = (uint32_t)pid[s] < (uint32_t)a.pages;
-      sl[s] = in ? pid[s] * a.P + (j - div(j, a.d_page) * a.P) : -1;
+      sl[s] = in ? pid[s] * a.P + in_page(key_at(base, 16 * s + (lane & 15)), a.d_page, a.P) : -1;
     }
   }
   // a key without a slot reads slot 0 and is masked in scores() and store_v()
@@ -634,7 +633,7 @@ __global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArg
   if (!row_range(a, row, owner, lo, hi)) return;
   W wk;
   wk.start(a, row, kh, qt, lane);
-  const int tiles = (hi - lo + W::KT - 1) / W::KT, n = min(16, a.G - qt * 16);
+  const int tiles = tiles_of(hi - lo, W::KT), n = min(16, a.G - qt * 16);
   wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, w, tiles, nw, (bf16_t*)(lds + w * W::LDS), lane);
   leave(wk, sh, lds, n, w, lane);
   __syncthreads();
@@ -676,7 +675,7 @@ __global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs
     const int r = t * per + i;
     int owner, lo, hi;
     if (i < per && r < a.rows && row_range(a, r, owner, lo, hi))
-      n[i] = max(1, (hi - lo + 4 * W::KT - 1) / (4 * W::KT));  // a row without keys is written too
+      n[i] = max(1, tiles_of(hi - lo, 4 * W::KT));  // a row without keys is written too
     mine += n[i];
   }
   int at = (int)scan_add((uint32_t)mine);
@@ -722,7 +721,7 @@ __global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs
     row_range(a, row, owner, lo, hi);
     owner = __builtin_amdgcn_readfirstlane(owner);
     wk.start(a, row, kh, qt, lane);
-    wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, 4 * c0 + w, min(4 * c1, (hi - lo + W::KT - 1) / W::KT), 4,
+    wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, 4 * c0 + w, min(4 * c1, tiles_of(hi - lo, W::KT)), 4,
            (bf16_t*)(lds + w * W::LDS), lane);
     leave(wk, sh, lds, nq, w, lane);
     __syncthreads();

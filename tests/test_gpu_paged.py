@@ -570,3 +570,44 @@ def test_decoding_many_requests_together():
         assert np.abs(alt.host().reshape(cap, 3) - sc["alt"]).max() < 2.0 ** -18
     for g in graphs:
         g.close()
+
+
+# 129 x 16647160 = 2^31 - 8: the last tile of a walk to the table's end reaches past 2^31
+FAR_PAGE, FAR_WIDTH = 129, 16647160
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D,window", [(16, 100), (32, 3000), (64, 100), (64, 3000), (128, 100), (128, 3000), (20, 100)])
+def test_attention_at_the_last_positions(dtype, D, window):
+    """Tables of nearly 2^31 positions (whose pages are few and shared), windows that end with them, in every form.  A
+    key past the first request's table would be in the second's first page, which holds large values."""
+    a = Attend(D, dtype, 6, 2, D, FAR_PAGE, [FAR_PAGE] * 4, window=window)
+    a.k, a.v = (G.rnd(t.shape, dtype, a.rng) for t in (a.k, a.v))
+    far = FAR_PAGE * FAR_WIDTH - 1
+    a.tab = np.tile(np.arange(FAR_WIDTH, dtype=np.int32) % 4 + 1, (2, 1))
+    a.tab[1, 0] = 0
+    a.v[:FAR_PAGE] = 2.0 ** 60
+    a.width = FAR_WIDTH
+    a.pos, a.own = np.array([far, far - 40, 5]), np.array([0, 0, 1])
+    a.q = a.q[:3]
+    a.upload().run().check()
+
+
+def test_attention_over_2_to_the_31_keys():
+    """A whole walk of 2^31 - 8 keys, each of four pages as often as the others: o and lse are those of one copy of
+    the pages, lse + ln(copies).  A lane adds 4096 tiles' sums one after another and a matrix tile four times as many
+    products of two planes: relative 2^-24 each, in the shares' sum and in the values'."""
+    a = Attend(31, "bf16", 2, 1, 16, FAR_PAGE, [FAR_PAGE] * 4)
+    a.k, a.v = (G.rnd(t.shape, "bf16", a.rng) for t in (a.k, a.v))
+    a.tab = (np.arange(FAR_WIDTH, dtype=np.int32) % 4)[None]
+    a.width = FAR_WIDTH
+    a.pos, a.own, a.q = np.array([FAR_PAGE * FAR_WIDTH - 1]), np.array([0]), a.q[:1]
+    a.upload().run()
+    k, v, q = a.k[:4 * FAR_PAGE, 0], a.v[:4 * FAR_PAGE, 0], a.q[0]
+    s = q @ k.T / 4.0
+    e = np.exp(s - s.max(1, keepdims=True))
+    o, lse = e @ v / e.sum(1, keepdims=True), s.max(1) + np.log(e.sum(1)) + math.log(FAR_WIDTH // 4)
+    mag = e @ np.abs(v) / e.sum(1, keepdims=True)
+    steps = 2.0 ** -24 * (4096 + 2 * 4 * 4096 + 1024)
+    assert (np.abs(a.O.host()[:32].reshape(2, 16) - o) <= mag * (2 * steps + 2.0 ** -14) + np.abs(o) * 2.0 ** -8).all()
+    assert (np.abs(a.L.host()[:2] - lse) <= steps + 2.0 ** -16).all()
