@@ -395,7 +395,7 @@ size_t sj_attention_bwd_p_workspace_bytes(long batch, long t, long hq, long hk, 
  * status bit the step is void: every row is -1, starts are 0, and the table,
  * the free list's position and the lengths stay.  lengths_after may not be
  * lengths or counts, nor free_head summary + 1 (a captured loop alternates two
- * of each).  Calls on one table must not overlap. */
+ * of each).  At most 2^24 requests.  Calls on one table must not overlap. */
 #define SJ_PLAN_NO_PAGES 1    /* the free list is too short */
 #define SJ_PLAN_TABLE_WIDTH 2 /* a request outgrows its table row */
 #define SJ_PLAN_ROWS 4        /* more tokens than capacity */
@@ -424,9 +424,10 @@ int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long l
  * key gives o = 0 and lse = -inf; rows with position or owner below 0 (or an
  * owner past the requests) are left as they were.  Slots past a request's
  * length are never read into a result, whatever they hold.  head_dim at most
- * 256; rows times hk at most 2^23; any strides and element alignment.  Workspace:
- * sj_paged_attention_workspace_bytes, 16-byte aligned, not cleared and not
- * kept; calls that share one must not overlap. */
+ * 256, hq at most 65535; rows times the tiles of 16 query heads, hk * (hq / hk
+ * / 16 rounded up), at most 2^23; any strides and element alignment.
+ * Workspace: sj_paged_attention_workspace_bytes, 16-byte aligned, not cleared
+ * and not kept; calls that share one must not overlap. */
 size_t sj_paged_attention_workspace_bytes(long rows, long hq, long hk, long head_dim);
 int sj_paged_attention(void *stream, const void *q, long ldq, const void *k_cache, const void *v_cache, long ldkv,
                        int dtype, long pages, long page_size, const int32_t *table, long ldt, long requests,

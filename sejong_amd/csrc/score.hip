@@ -656,7 +656,7 @@ extern "C" int sj_token_logprobs(void* stream, const void* x, int dtype, long ld
              "token log probabilities: %ld rows of %ld (stride %ld)", rows, vocab, ldx);
   SJ_REQUIRE(top >= 0 && top <= SJ_LOGPROBS_MAX_TOP && top <= vocab, "token log probabilities: %ld alternatives of %ld",
              top, vocab);
-  SJ_REQUIRE(rows < (1L << 23) / slices_of(vocab), "token log probabilities: %ld rows of %ld", rows, vocab);
+  SJ_REQUIRE(rows * slices_of(vocab) < 1L << 23, "token log probabilities: %ld rows of %ld", rows, vocab);
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && (logprob == nullptr || tokens) && (top == 0 || (top_ids && top_logprob)),
              "token log probabilities: null");
@@ -687,7 +687,7 @@ extern "C" int sj_token_logprobs_bwd(void* stream, const void* x, int dtype, lon
              "token log probabilities backward dtypes %d, %d", dtype, dx_dtype);
   SJ_REQUIRE(rows >= 0 && rows <= 0x7fffffffL && vocab > 0 && vocab <= 1L << 24 && ldx >= vocab && lddx >= vocab,
              "token log probabilities backward: %ld rows of %ld (strides %ld, %ld)", rows, vocab, ldx, lddx);
-  SJ_REQUIRE(rows < (1L << 23) / slices_of(vocab), "token log probabilities backward: %ld rows of %ld", rows, vocab);
+  SJ_REQUIRE(rows * slices_of(vocab) < 1L << 23, "token log probabilities backward: %ld rows of %ld", rows, vocab);
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && stats && dx && (dlogprob == nullptr || tokens) && (dentropy == nullptr || entropy),
              "token log probabilities backward: null");

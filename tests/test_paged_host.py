@@ -162,3 +162,18 @@ def test_the_gradient_formula_against_differences():
             e[r, v] = h
             f = [dlp @ s["logprob"] + dent @ s["entropy"] for s in (U.scores(x + e, tokens), U.scores(x - e, tokens))]
             assert abs((f[0] - f[1]) / (2 * h) - got[r, v]) < 1e-8
+
+
+def test_limits_are_the_documented_ones():
+    """Rows times tiles of 16 query heads up to 2^23; rows times slices of 8192 entries below 2^23 (the refusal that
+    follows is the missing workspace's)."""
+    wide = dict(hq=40, hk=2, ldq=40 * 64, ldo=40 * 64, requests=2 ** 23, workspace=X, workspace_bytes=2 ** 40)
+    refused("sj_paged_attention", changed(ATTEND, rows=2 ** 21 + 1, **wide), 1, b"rows of 2 heads")
+    refused("sj_paged_attention", changed(ATTEND, hq=65536, hk=65536, ldq=2 ** 22, ldo=2 ** 22, ldkv=2 ** 22), 1,
+            b"paged attention")
+    for slices in (3, 5, 7):
+        most = (2 ** 23 - 1) // slices
+        at = dict(vocab=slices * 8192, ldx=slices * 8192)
+        refused("sj_token_logprobs", changed(SCORE, rows=most, **at), 2, b"required")
+        refused("sj_token_logprobs", changed(SCORE, rows=most + 1, **at), 1, b"rows of")
+        refused("sj_token_logprobs_bwd", changed(BACK, rows=most + 1, lddx=slices * 8192, **at), 1, b"rows of")
