@@ -135,10 +135,11 @@ int sj_rope_frequencies(void *stream, uint64_t *turns, long rotary_dim, const sj
  * written.  Pairs: INTERLEAVED (2i, 2i + 1), as sj_rope; HALF (i, i +
  * rotary_dim / 2).  (a, b) -> amplitude (a cos - b sin, a sin + b cos);
  * inverse != 0 negates the sine: the gradient of the forward call.  The angle
- * is good to 2^-22 up to position 2^27.  x and y fp32 or bf16 (stored value in, fp32
- * products, one rounding); y may be x.  head_dim even, at most 1024; any
- * strides and element alignment (16-byte rows are fastest).  turns may be
- * null when rotary_dim is 0; below 2^24 rows, at most 2^14 heads. */
+ * is good to 2^-22 up to position 2^27.  x and y fp32 or bf16 (stored value
+ * in, fp32 products, one rounding); y may be x with the same stride.  head_dim
+ * even, at most 1024; any strides and element alignment (16-byte rows are
+ * fastest).  turns may be null when rotary_dim is 0; below 2^24 rows, at most
+ * 2^14 heads. */
 #define SJ_ROPE_INTERLEAVED 0
 #define SJ_ROPE_HALF 1
 int sj_rope_rows(void *stream, const void *x, long ldx, void *y, long ldy, int dtype, long rows, long heads,
@@ -408,8 +409,8 @@ int sj_paged_plan(void *stream, const int32_t *lengths, const int32_t *counts, l
  * keys rotated and values copied into the cache rows of their slots; the
  * rotation as sj_rope_rows.  A row whose slot is not in 0 .. cache_slots - 1
  * is left out whole (q_out too).  The slots of one call are distinct.  q_out
- * may be q; hq may be 0.  Any strides and element alignment; below 2^24 rows, hq and hk
- * at most 2^14. */
+ * may be q with the same stride; hq may be 0.  Any strides and element alignment;
+ * below 2^24 rows, hq and hk at most 2^14. */
 int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, int dtype,
                     long rows, long hq, long hk, long head_dim, long rotary_dim, int layout, const int32_t *positions,
                     const int32_t *slots, const uint64_t *turns, float amplitude, void *q_out, long ldqo,
@@ -418,12 +419,13 @@ int sj_paged_append(void *stream, const void *q, long ldq, const void *k, long l
  * request owners[i]; owners null: request i) at position positions[i] sees its
  * request's keys 0 .. positions[i], with window > 0 the `window` last of them;
  * scale head_dim^-1/2.  Several rows may belong to one request (drafted
- * tokens, chunks of a prompt).  o [rows][ldo] in the q dtype, lse (nullable)
- * fp32 [rows][hq] natural log of the sum of exp(score).  Keys whose page id is
- * not in 0 .. pages - 1, and scores of -inf (of finite values), have no share; a row without any
- * key gives o = 0 and lse = -inf; rows with position or owner below 0 (or an
- * owner past the requests) are left as they were.  Slots past a request's
- * length are never read into a result, whatever they hold.  head_dim at most
+ * tokens, chunks of a prompt).  o [rows][ldo] in the q dtype, and may be q with
+ * the same stride; lse (nullable) fp32 [rows][hq] natural log of the sum of
+ * exp(score).  Keys whose page id is not in 0 .. pages - 1, and scores of -inf
+ * (of finite values), have no share; a row without any key gives o = 0 and lse
+ * = -inf; rows with position or owner below 0 (or an owner past the requests)
+ * are left as they were.  Slots past a request's length are never read into a
+ * result, whatever they hold.  head_dim at most
  * 256, hq at most 65535; rows times the tiles of 16 query heads, hk * (hq / hk
  * / 16 rounded up), at most 2^23; any strides and element alignment.
  * Workspace: sj_paged_attention_workspace_bytes, 16-byte aligned, not cleared

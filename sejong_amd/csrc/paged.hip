@@ -988,6 +988,7 @@ extern "C" int sj_paged_attention(void* stream, const void* q, long ldq, const v
   SJ_REQUIRE(owners || rows <= requests, "paged attention: %ld rows of %ld requests without owners", rows, requests);
   if (rows == 0 || requests == 0) return SJ_OK;
   SJ_REQUIRE(q && k_cache && v_cache && table && positions && o, "paged attention: null");
+  SJ_REQUIRE(q != o || ldq == ldo || rows == 1, "paged attention: in place with strides %ld and %ld", ldq, ldo);
   const size_t need = sj_paged_attention_workspace_bytes(rows, hq, hk, head_dim);
   SJ_REQUIRE(((uintptr_t)workspace & 15) == 0, "paged attention: the workspace is not 16-byte aligned");
   if (need > workspace_bytes || (need && !workspace))

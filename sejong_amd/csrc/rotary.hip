@@ -243,6 +243,7 @@ extern "C" int sj_rope_rows(void* stream, const void* x, long ldx, void* y, long
              "rope rows dimensions");
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && y && positions && (turns || rotary_dim == 0), "rope rows: null");
+  SJ_REQUIRE(x != y || ldx == ldy || rows == 1, "rope rows: in place with strides %ld and %ld", ldx, ldy);
   SJ_REQUIRE(rows < 1L << 24, "rope rows: %ld rows", rows);
   RopeArgs a = {};
   a.seg[0] = RopeSeg{x, ldx, y, ldy, (int)heads, 1, 0};
@@ -273,6 +274,8 @@ extern "C" int sj_paged_append(void* stream, const void* q, long ldq, const void
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(k && v && positions && slots && (turns || rotary_dim == 0) && k_cache && v_cache && (hq == 0 || (q && q_out)),
              "paged append: null");
+  SJ_REQUIRE(hq == 0 || q != q_out || ldq == ldqo || rows == 1, "paged append: queries in place with strides %ld and %ld",
+             ldq, ldqo);
   SJ_REQUIRE(rows < 1L << 24, "paged append: %ld rows", rows);
   RopeArgs a = {};
   a.seg[0] = RopeSeg{q, ldq, q_out, ldqo, (int)hq, 1, 0};

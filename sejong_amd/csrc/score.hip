@@ -691,6 +691,9 @@ extern "C" int sj_token_logprobs_bwd(void* stream, const void* x, int dtype, lon
   if (rows == 0) return SJ_OK;
   SJ_REQUIRE(x && stats && dx && (dlogprob == nullptr || tokens) && (dentropy == nullptr || entropy),
              "token log probabilities backward: null");
+  SJ_REQUIRE(x != dx || (dtype == dx_dtype && (ldx == lddx || rows == 1)),
+             "token log probabilities backward: in place with dtypes %d and %d, strides %ld and %ld", dtype, dx_dtype, ldx,
+             lddx);
   ScoreBwdArgs a = {};
   a.x = x; a.ldx = ldx; a.rows = rows; a.V = (int)vocab; a.tokens = tokens; a.stats = stats; a.entropy = entropy;
   a.dlp = dlogprob; a.dent = dentropy; a.dx = dx; a.lddx = lddx;

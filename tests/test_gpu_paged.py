@@ -611,3 +611,17 @@ def test_attention_over_2_to_the_31_keys():
     steps = 2.0 ** -24 * (4096 + 2 * 4 * 4096 + 1024)
     assert (np.abs(a.O.host()[:32].reshape(2, 16) - o) <= mag * (2 * steps + 2.0 ** -14) + np.abs(o) * 2.0 ** -8).all()
     assert (np.abs(a.L.host()[:2] - lse) <= steps + 2.0 ** -16).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lengths,D", [([20, 1, 7], 64), ([20000, 300], 64), ([20, 1, 7], 20)])
+def test_attention_in_place(dtype, lengths, D):
+    """o over q, in every form (one workgroup a walk, walks cut into pieces, narrow heads): the same bits as apart."""
+    a = Attend(13, dtype, 6, 2, D, 16, lengths).upload().run()
+    a.check()
+    apart = a.O.host()[:len(lengths) * a.ldq]
+    guard = G.dev(np.full(len(lengths) * a.ldq + 8, 55.0), dtype)
+    q = np.concatenate([a.q.ravel(), np.full(8, 55.0)])
+    a.Q = a.O = guard.upload(q)
+    a.run().check()
+    np.testing.assert_array_equal(a.O.host()[:len(apart)], apart)

@@ -177,3 +177,14 @@ def test_limits_are_the_documented_ones():
         refused("sj_token_logprobs", changed(SCORE, rows=most, **at), 2, b"required")
         refused("sj_token_logprobs", changed(SCORE, rows=most + 1, **at), 1, b"rows of")
         refused("sj_token_logprobs_bwd", changed(BACK, rows=most + 1, lddx=slices * 8192, **at), 1, b"rows of")
+
+
+def test_in_place_calls_keep_their_rows_places():
+    """The output may be the input only where each element stays in its own place: other strides or types would have
+    rows overwritten before they are read."""
+    refused("sj_rope_rows", changed(ROPE, ldx=128, ldy=136), 1, b"in place")
+    refused("sj_rope_rows", changed(ROPE, ldx=256, ldy=128), 1, b"in place")
+    refused("sj_paged_append", changed(APPEND, ldq=512, ldqo=256), 1, b"in place")
+    refused("sj_paged_attention", changed(ATTEND, ldq=512, ldo=256), 1, b"in place")
+    for kw in (dict(ldx=264, lddx=265), dict(dx_dtype=N.SJ_BF16), dict(dtype=N.SJ_BF16)):
+        refused("sj_token_logprobs_bwd", changed(BACK, **kw), 1, b"in place")
