@@ -387,3 +387,67 @@ def test_long_lists(n, V, dtype):
         s = Score(x, dtype, tokens, top)
         s.forward()
         check_forward(s.host(), x, tokens, top)
+
+
+def check_long_rows(got, x, tokens, top):
+    """As check_forward, with the sums counted as they are formed: a term is off by 2 |x - m| + 5 units (its argument's
+    two roundings, the power, the factor back to the maximum), and again 2 |m_s - m| + 4 from its slice's maximum to
+    the row's; a thread adds 64 terms, then 8 levels, 8 slices at most and 8 levels: 100 + 4 |x - m| in all."""
+    want = U.scores(x, tokens, top)
+    np.testing.assert_array_equal(got["ids"], want["ids"])
+    with np.errstate(invalid="ignore"):
+        spread = np.abs(x - want["ref"][:, None])
+        mean = np.where(want["p"] > 0, want["p"] * spread, 0.0).sum(1)
+        part = np.where(want["p"] > 0, want["p"] * spread * spread, 0.0).sum(1)
+    total = ULP * (100 + 4 * mean)
+    log = total + 2 * ULP * (want["ll"] + 2)
+    assert (got["stats"][:, 0] == want["ref"]).all()
+    assert (np.abs(got["stats"][:, 1] - want["ll"]) <= log).all()
+
+    def close(g, w, d, tol):
+        with np.errstate(invalid="ignore"):
+            near = np.isfinite(w) & (np.abs(g - w) <= tol + 2 * ULP * (d + np.abs(w)))
+            assert (near | (g == w)).all(), np.nanmax(np.abs(g - w))
+    rows = np.arange(len(x))
+    close(got["lp"], want["logprob"], spread[rows, want["at"]], log)
+    close(got["alt"], want["alt"], np.take_along_axis(spread, want["ids"], 1), log[:, None])
+    tol = log + ULP * (104 * mean + 4 * part) + total * mean + 8 * ULP * (want["ll"] + mean)
+    assert (np.abs(got["ent"] - want["entropy"]) <= tol).all(), np.max(np.abs(got["ent"] - want["entropy"]) / tol)
+
+
+def many_slices(n, V, dtype, seed):
+    """Rows of very many slices: the largest value twice, 256 slices of 8192 or 16384 apart; nothing but -inf in most
+    slices or in all; equal entries; the largest at either end."""
+    x = logits(np.random.default_rng(seed), n, V, dtype)
+    i = np.arange(V)
+    for at in (3 * 8192 + 5, 259 * 8192 + 7, 3 * 16384 + 9, 259 * 16384 + 11):
+        if at < V:
+            x[0, at] = 24.0
+    if n > 1:
+        x[1, (i // 8192) % 50 != 7] = -np.inf
+    if n > 2:
+        x[2] = -np.inf
+        x[2, [V - 1, V // 2, 12345]] = [1.0, 2.0, 1.0]
+    if n > 3:
+        x[3] = -np.inf
+    if n > 4:
+        x[4] = -1.5
+    if n > 5:
+        x[5, 0] = x[5, V - 1] = 30.0
+    return x
+
+
+@pytest.mark.parametrize("n,V,dtype,top", [
+    (6, 70 * 8192 - 77, "f32", 20), (6, 70 * 8192 - 77, "f32", 64), (15, 70 * 8192, "f32", 1), (15, 70 * 8192, "f32", 64),
+    (3, 300 * 8192 - 8191, "f32", 64), (3, 300 * 8192 - 1, "f32", 1), (4, 300 * 8192 - 77, "f32", 20),
+    (4, 270 * 8192 - 77, "f32", 64), (2, 300 * 8192 - 3, "bf16", 20), (1, 600 * 8192 - 77, "bf16", 64),
+    (2, 300 * 16384 - 77, "bf16", 1), (2, 300 * 16384 - 77, "bf16", 64), (16, 70 * 16384 - 5, "bf16", 20),
+    (1, 1 << 24, "f32", 64), (1, 1 << 24, "bf16", 5)])
+def test_rows_of_many_slices(n, V, dtype, top):
+    """More than 64 slices and more than 256, met within the launch (up to 1024 in all) and joined by a second one."""
+    x = many_slices(n, V, dtype, V + n)
+    tokens = np.random.default_rng(n).integers(0, V, n)
+    tokens[0] = 3 * 8192 + 5
+    s = Score(x, dtype, tokens, top)
+    s.forward()
+    check_long_rows(s.host(), x, tokens, top)
