@@ -625,3 +625,36 @@ def test_attention_in_place(dtype, lengths, D):
     a.Q = a.O = guard.upload(q)
     a.run().check()
     np.testing.assert_array_equal(a.O.host()[:len(apart)], apart)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lengths,hq,hk,D", [(LENGTHS, 6, 2, 64), ([20000, 3000, 1], 6, 2, 64), ([9000, 3], 8, 8, 128),
+                                             ([4000, 50], 3, 1, 16), ([400, 30], 6, 2, 20), ([5000, 700], 2, 1, 256)])
+def test_attention_writes_every_output_again(dtype, lengths, hq, hk, D):
+    """The workspace as the last call left it, the outputs refilled: each call writes all of o and lse, the same bits."""
+    a = Attend(14, dtype, hq, hk, D, 16, lengths, pad=1).upload().run()
+    a.check()
+    first = a.O.host(), a.L.host()
+    for _ in range(3):
+        a.O.upload(np.full(a.O.n, 55.0))
+        a.L.upload(np.full(a.L.n, 55.0))
+        a.run().check()
+        for x, y in zip(first, (a.O, a.L)):
+            np.testing.assert_array_equal(y.host()[:len(x)], x)
+
+
+def test_replays_of_one_workspace_write_every_output():
+    """Two graphs that share a workspace, replayed in turn with o and lse refilled, their captured calls' numbers kept."""
+    a = Attend(15, "bf16", 6, 2, 64, 16, [5000, 700, 1]).upload()
+    b = Attend(16, "f32", 4, 2, 32, 16, [3000, 10]).upload()
+    need = max(a.need, b.need)
+    a.ws = b.ws = G.Dev(need, "u8").upload(np.full(need, 0xFF))
+    graphs = [PU.Graph(x.run) for x in (a, b)]
+    for _ in range(3):
+        for g, x in zip(graphs, (a, b)):
+            x.O.upload(np.full(x.O.n, 55.0))
+            x.L.upload(np.full(x.L.n, 55.0))
+            g.replay()
+            x.check()
+    for g in graphs:
+        g.close()

@@ -451,3 +451,27 @@ def test_rows_of_many_slices(n, V, dtype, top):
     s = Score(x, dtype, tokens, top)
     s.forward()
     check_long_rows(s.host(), x, tokens, top)
+
+
+def refill(s):
+    """Guard values in every output of a call."""
+    for b, v in ((s.lp, 55.0), (s.ent, 55.0), (s.stats, 55.0), (s.ids, 99), (s.alt, 55.0)):
+        b.upload(np.full(b.n, v))
+
+
+@pytest.mark.parametrize("n,V,dtype,top", [(5, 257, "f32", 5), (3, 4099, "bf16", 8), (4, 50001, "f32", 20),
+                                           (2, 131072, "bf16", 64), (600, 16400, "f32", 3), (300, 40000, "bf16", 0)])
+def test_scores_write_every_output_again(n, V, dtype, top):
+    """The workspace as the last call left it, the outputs refilled: each call writes all of them, the same bits."""
+    rng = np.random.default_rng(V)
+    x, tokens = logits(rng, n, V, dtype), rng.integers(0, V, n)
+    s = Score(x, dtype, tokens, top)
+    s.forward()
+    first = s.host()
+    check_forward(first, x, tokens, top)
+    for _ in range(3):
+        refill(s)
+        s.forward()
+        again = s.host()
+        for k in first:
+            np.testing.assert_array_equal(again[k], first[k])

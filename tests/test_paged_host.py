@@ -188,3 +188,16 @@ def test_in_place_calls_keep_their_rows_places():
     refused("sj_paged_attention", changed(ATTEND, ldq=512, ldo=256), 1, b"in place")
     for kw in (dict(ldx=264, lddx=265), dict(dx_dtype=N.SJ_BF16), dict(dtype=N.SJ_BF16)):
         refused("sj_token_logprobs_bwd", changed(BACK, **kw), 1, b"in place")
+
+
+def test_cut_walks_and_long_rows_need_a_workspace():
+    lib = N.load()
+    need = lib.sj_paged_attention_workspace_bytes(4, 4, 2, 64)
+    assert need > 0
+    refused("sj_paged_attention", changed(ATTEND, workspace=X, workspace_bytes=need - 1), 2, b"required %d bytes" % need)
+    refused("sj_paged_attention", changed(ATTEND, workspace=None, workspace_bytes=need), 2, b"available 0 bytes")
+    need = lib.sj_token_logprobs_workspace_bytes(4, 150000, 5)
+    assert need > 0
+    big = dict(vocab=150000, ldx=150000)
+    refused("sj_token_logprobs", changed(SCORE, workspace=X, workspace_bytes=need - 1, **big), 2, b"required %d bytes" % need)
+    refused("sj_token_logprobs", changed(SCORE, workspace=None, workspace_bytes=need, **big), 2, b"available 0 bytes")
