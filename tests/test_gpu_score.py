@@ -475,3 +475,23 @@ def test_scores_write_every_output_again(n, V, dtype, top):
         again = s.host()
         for k in first:
             np.testing.assert_array_equal(again[k], first[k])
+
+
+def test_scores_on_two_streams_at_once():
+    """Rows of several slices on two streams with a workspace each, several times, outputs refilled."""
+    rng = np.random.default_rng(8)
+    both = [Score(logits(rng, n, V, d), d, rng.integers(0, V, n), 9) for n, V, d in ((12, 60000, "f32"), (5, 131072, "bf16"))]
+    graphs = [PU.Graph(s.forward) for s in both]
+    for _ in range(3):
+        data = []
+        for s in both:
+            refill(s)
+            data.append(logits(rng, s.n, s.V, s.dtype))
+            s.x.upload(data[-1])
+        for g in graphs:
+            g.do(g.hip.hipGraphLaunch(g.exe, g.stream))
+        G.sync()
+        for s, x in zip(both, data):
+            check_forward(s.host(), x, s.tokens.host(), 9)
+    for g in graphs:
+        g.close()
