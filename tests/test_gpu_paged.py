@@ -658,3 +658,15 @@ def test_replays_of_one_workspace_write_every_output():
             x.check()
     for g in graphs:
         g.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lengths,hq,hk,D", [([700] * 70, 6, 2, 64), ([5, 30, 64, 1, 0] * 40, 16, 4, 64),
+                                             ([900] + [10] * 300, 8, 4, 128), ([100] * 2100, 2, 1, 32), ([60] * 9, 6, 2, 20)])
+def test_attention_of_short_requests_in_wide_tables(dtype, lengths, hq, hk, D):
+    """Tables for 131072 tokens, as a server that allows so many keeps them: the form for long walks, whatever the
+    lengths."""
+    a = Attend(17, dtype, hq, hk, D, 16, lengths)
+    a.tab = np.pad(a.tab, ((0, 0), (0, 131072 // 16 - a.width)), constant_values=-1)
+    a.width = a.tab.shape[1]
+    a.upload().run().check()
