@@ -57,7 +57,6 @@ struct RopeSeg {
   long ldy;
   int heads;   // heads of this segment
   int rotate;  // 0: copied
-  int slots;   // the destination row is the row's slot, not the row
 };
 
 struct RopeArgs {
@@ -246,7 +245,7 @@ extern "C" int sj_rope_rows(void* stream, const void* x, long ldx, void* y, long
   SJ_REQUIRE(x != y || ldx == ldy || rows == 1, "rope rows: in place with strides %ld and %ld", ldx, ldy);
   SJ_REQUIRE(rows < 1L << 24, "rope rows: %ld rows", rows);
   RopeArgs a = {};
-  a.seg[0] = RopeSeg{x, ldx, y, ldy, (int)heads, 1, 0};
+  a.seg[0] = RopeSeg{x, ldx, y, ldy, (int)heads, 1};
   a.nseg = 1;
   a.rows = rows;
   a.heads = (int)heads;
@@ -278,9 +277,9 @@ extern "C" int sj_paged_append(void* stream, const void* q, long ldq, const void
              ldq, ldqo);
   SJ_REQUIRE(rows < 1L << 24, "paged append: %ld rows", rows);
   RopeArgs a = {};
-  a.seg[0] = RopeSeg{q, ldq, q_out, ldqo, (int)hq, 1, 0};
-  a.seg[1] = RopeSeg{k, ldk, k_cache, ldkv, (int)hk, 1, 1};
-  a.seg[2] = RopeSeg{v, ldv, v_cache, ldkv, (int)hk, 0, 1};
+  a.seg[0] = RopeSeg{q, ldq, q_out, ldqo, (int)hq, 1};
+  a.seg[1] = RopeSeg{k, ldk, k_cache, ldkv, (int)hk, 1};
+  a.seg[2] = RopeSeg{v, ldv, v_cache, ldkv, (int)hk, 0};
   a.nseg = 3;
   a.rows = rows;
   a.heads = (int)(hq + 2 * hk);
