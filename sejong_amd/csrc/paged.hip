@@ -200,7 +200,7 @@ __global__ __launch_bounds__(PT) void k_paged_plan(PlanArgs a) {
 //
 //   o = sum_j e^(s_j - m) v_j / l,  m = max s_j,  l = sum_j e^(s_j - m)
 //
-// One wave walks tiles of 16 to 64 keys of one KV head for up to 16 of its
+// One wave walks tiles of 16 to 128 keys of one KV head for up to 16 of its
 // query heads at once, with the running maximum and sum of each query: the
 // group's query heads are the columns of one MFMA tile, so a key is read once
 // for all of them, and padding the group to 16 columns costs matrix time that
@@ -276,7 +276,10 @@ __device__ __forceinline__ uint32_t cvt2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){a, b}, bf16x2v));
 }
 
-// A wave's walk.  DC: the head in units of 32 columns.  E: elements of 16
+// A wave's walk.  DC: the head in units of 32 columns; heads between the sizes
+// are walked as the next one, their missing columns read again and multiplied
+// by 0 (64 requests of 2048 keys, 16/4 heads, bf16: heads of 104 57 us, of 128
+// 54, of 160 106, of 192 111, of 256 121).  E: elements of 16
 // bytes, KT: keys of a tile, NC: 16-byte chunks that a lane holds of a row.
 template <typename T, int DC>
 struct Walk {
@@ -655,7 +658,11 @@ __global__ __launch_bounds__(64 * direct_waves(DC)) void k_paged_direct(PagedArg
 // and the meeting behind them 5; with the join as a launch of its own 16.7 and
 // for one request of 1000 keys 11.6 against 10.4.
 constexpr int STREAM_ROWS = 2048;
-// workgroups that 256 CUs hold at once (by registers), and the most there are
+// Workgroups that 256 CUs hold at once (by registers), and the most there are.
+// Three of heads of 33 to 64 a CU, though a lane then spills 2 (bf16) or 4
+// (fp32) registers: us with 3 / 2, bf16 | fp32: 45 requests of 1 to 6000 keys
+// 16.4 / 19.4 | 22.9 / 25.5, 64 x 4 of 4096 56.3 / 55.5 | 122 / 112, 64 x 8 of
+// 8192 245 / 233 | 389 / 380.
 constexpr int split_per_cu(int dc) { return dc == 8 ? 1 : dc == 2 || dc == 3 ? 3 : 2; }
 constexpr int STREAM_GROUPS = 1024;
 
@@ -785,7 +792,10 @@ __global__ __launch_bounds__(256, split_per_cu(DC)) void k_paged_split(PagedArgs
 
 // Heads that are no whole 16-byte chunks: one workgroup per row and query
 // head.  A lane owns a key in the products with q and columns lane + 64 c in
-// the sums over v.
+// the sums over v.  Bound by that: a group's keys are read once per query head,
+// element by element, the values' keys one after another, and a long walk is
+// not cut.  64 requests of 2048 keys, 16/4 heads, bf16: heads of 20 210 us (of
+// 32, above, 26), of 36 226 (of 64 33); one request of 8192 469 and 818 (12).
 template <typename T>
 __global__ __launch_bounds__(256) void k_paged_rows(PagedArgs a) {
   __shared__ float q[256], p[4][64], acc[4][256], wm[4], wl[4];
@@ -947,12 +957,27 @@ int attend(hipStream_t s, PagedArgs& a, long most, void* workspace) {
   by_width<T>(a.D, [&](auto w) {
     const long tiles = (most + decltype(w)::KT - 1) / decltype(w)::KT;
     // The direct form, which sums no rows and joins in LDS alone, where a wave
-    // has one tile, and where the workgroups are many and the walks, however
-    // uneven, not long.  us, direct / split, bf16: heads of 64, 1 request x 2
-    // of 512 keys 7.8 / 10.1, of 1024 11.6 / 10.6, of 8192 62 / 11.6; 64 x 2 of
-    // 1024 12.8 / 14.9, of 4096 40 / 39; 64 x 8 of 1024 34 / 42, of 4096 117 /
-    // 127, of 8192 228 / 243 (but 45 x 4 of 1 to 6000 47 / 17); heads of 128,
-    // 256 x 8 of 1024 200 / 188
+    // has one tile, and where the workgroups are many and the tables not wide.
+    // us, direct / split, bf16, requests x KV heads of L keys each | of 1 to L
+    // keys, in tables of L:
+    //   heads of 64        1 x 2  512    7.7 / 10.2 |
+    //                      1 x 2  1024  11.6 / 10.6 |
+    //     (16 tiles)      64 x 2  1024  12.6 / 14.0 | 11.2 / 10.6
+    //                     64 x 2  2048  21.5 / 20.5 | 18.6 / 10.8
+    //                     64 x 4  1024  15.7 / 19.8 | 11.3 / 12.4
+    //                     64 x 4  2048  26.6 / 32.8 | 19.1 / 13.3
+    //                     64 x 8  2048  50.3 / 59.2 | 28.6 / 19.2
+    //     (64 tiles)      64 x 8  4096   119 / 128  | 44.0 / 25.5
+    //                     64 x 8  8192   235 / 245  | 74.0 / 33.0
+    //                    128 x 8  4096   233 / 236  | 69.5 / 40.8
+    //     (16 tiles)     256 x 8  1024   120 / 115  | 29.8 / 37.3
+    //                    256 x 8  2048   234 / 215  | 46.1 / 45.8
+    //   heads of 128      64 x 8  1024  47.9 / 55.0 | 27.7 / 24.3
+    //     (64 tiles)      64 x 8  2048   107 / 111  | 43.6 / 27.8
+    //                     64 x 8  4096   205 / 204  | 72.4 / 38.8
+    // From 17 to 64 tiles the rule takes up to a sixth off requests of one
+    // length and costs very uneven ones up to 1.7 times the split form's time:
+    // the lengths, which would tell them apart, are on the device.
     direct = direct || tiles <= 8 || (units >= 128 && tiles <= 16) || (units >= 512 && units < 2048 && tiles <= 64);
     if (direct) st = launch_direct(s, a, tiles <= 4 || units >= 1024 ? 4 : 8, w);
   });

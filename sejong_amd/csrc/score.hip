@@ -29,11 +29,16 @@ namespace {
 // a second launch where they are more.  us, meeting / second launch: 32 rows of
 // 50001 fp32 7.2 / 8.0, with 20 alternatives of 131072 14.0 / 14.1; 1024 slices
 // (512 rows of 16384) 11.8 / 12.2; 1792 (256 of 50008) 17.2 / 15.3.
-// The bound is the read, and where an entry has 2 bytes the vector units: per
-// entry about 7 operations, one of them an exponential, and as much again per
-// thread for the threshold and the list.  2048 rows of 50001 bf16, 8
-// alternatives: forward 70 us (2.9 TB/s) and join 8, gradient 78 (5.2 TB/s, a
-// copy's rate); 1024 rows of 131072 fp32 97 us (5.5 TB/s).
+// The bound is the read, and where an entry has 2 bytes the vector units: 7
+// operations per entry, one of them an exponential, and per slice, whatever it
+// holds, 245 a wave, with 240 more for 8 alternatives (threshold, and the two
+// walks that count and place), 530 for 32 and 1225 for 64.  2048 rows of 50001
+// bf16, 8 alternatives, four slices of 49 entries a thread (810 operations a
+// wave), by the kernel trace: forward 70 us (2.9 TB/s) and join 8, gradient 79
+// (5.2 TB/s, a copy's rate); a pass of the three 148.  1024 rows of 131072 fp32
+// 97 us (5.5 TB/s).  2048 rows with 8 / 32 / 64 alternatives, us: bf16 of 32000
+// 42 / 49 / 70, of 131072 125 / 152 / 216 (at a copy's rate 26 and 105); fp32 of
+// 131072 191 / 224 / 325 (211).
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int CAP_SLICE = 1024;  // entries at or above the threshold that LDS holds of a slice
