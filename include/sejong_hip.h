@@ -401,6 +401,7 @@ size_t sj_attention_bwd_p_workspace_bytes(long batch, long t, long hq, long hk, 
 #define SJ_PLAN_TABLE_WIDTH 2 /* a request outgrows its table row */
 #define SJ_PLAN_ROWS 4        /* more tokens than capacity */
 #define SJ_PLAN_LENGTHS 8     /* a negative length or count, or a length past 2^31 - 1 */
+#define SJ_FORK_LIST_FULL 16  /* no room before the free list's position (sj_paged_fork) */
 int sj_paged_plan(void *stream, const int32_t *lengths, const int32_t *counts, long requests, long page_size,
                   long pages, int32_t *table, long ldt, const int32_t *free_pages, long free_count,
                   const int32_t *free_head, int32_t *lengths_after, int32_t *starts, int32_t *positions,
@@ -435,6 +436,91 @@ int sj_paged_attention(void *stream, const void *q, long ldq, const void *k_cach
                        int dtype, long pages, long page_size, const int32_t *table, long ldt, long requests,
                        const int32_t *owners, const int32_t *positions, long rows, long hq, long hk, long head_dim,
                        long window, void *o, long ldo, float *lse, void *workspace, size_t workspace_bytes);
+
+/* The requests change places: request i after the step is request parents[i]
+ * before it (several may have one parent; below 0: empty), as beam search, a
+ * prompt answered several times, and the end of requests (all others keep their
+ * place) need it.  shared [pages] counts the table rows, or other holders, that
+ * a page has beyond its first: 0 for a page of one row and for a free one, so
+ * that sj_paged_plan hands pages out without it; who keeps a page besides the
+ * tables adds 1.  table_after [requests][ldt] and lengths_after are the parents'
+ * (entries behind the last page -1); full pages are shared; a last page that is
+ * not full stays with the lowest child if nobody else holds it, the other
+ * children get a page from the free list (from position free_head[0] on, in
+ * their order) and an entry in copies [requests][3] = (page, its copy, tokens in
+ * it), else (-1, -1, 0): sj_paged_copy's.  Pages without a holder left go back
+ * to the list, to the places before its position, the highest number first.
+ * shared_after [pages] and free_after [free_count] are the holders and the list
+ * after the step; all state after it needs arrays of its own (a captured loop
+ * alternates two of each).  summary [4] = pages taken, the list's position
+ * after the step, status bits, pages given back.  With SJ_PLAN_NO_PAGES or
+ * SJ_PLAN_LENGTHS (a parent past the requests, a length below 0 or longer than a
+ * table row) the step is void: shared, list and position are as before, all
+ * requests after it empty.  SJ_FORK_LIST_FULL: more pages to give back than
+ * places before the position; the others keep -1 in shared_after and are given
+ * back by a later step.  Table entries that are no page are handed on as they
+ * are.  At most 16384 requests, before and after.  Workspace:
+ * sj_paged_fork_workspace_bytes, 16-byte aligned, not cleared and not kept;
+ * calls that share one must not overlap. */
+size_t sj_paged_fork_workspace_bytes(long requests, long requests_before, long pages);
+int sj_paged_fork(void *stream, const int32_t *parents, long requests, const int32_t *table, long ldt,
+                  const int32_t *lengths, long requests_before, long page_size, long pages, const int32_t *shared,
+                  const int32_t *free_pages, long free_count, const int32_t *free_head, int32_t *table_after,
+                  int32_t *lengths_after, int32_t *shared_after, int32_t *free_after, int32_t *copies,
+                  int32_t *summary, void *workspace, size_t workspace_bytes);
+/* Makes room to shrink the pool to pages_after pages: every page of that number
+ * or more that is not on the free list (from its position on) moves to a free
+ * page below, the j-th by number to the list's j-th.  table_after, shared_after
+ * [pages] (0 from pages_after on), free_after [free_count] (the low pages left,
+ * in their order at the list's end; -1 before them) are the state after it in
+ * arrays of its own, copies [capacity][3] = (page, where it went, page_size)
+ * for sj_paged_copy and for holders besides the tables, the rest (-1, -1, 0).
+ * Table entries behind a request's last page and entries that are no page
+ * become -1.  summary [4] = moved pages, the list's position after it, status
+ * bits, free pages left.  With SJ_PLAN_NO_PAGES (fewer free pages below than
+ * pages that move) or SJ_PLAN_ROWS (more of them than capacity) the step is
+ * void and the state after it that before.  At most 2^24 requests.  Workspace:
+ * sj_paged_compact_workspace_bytes, as above. */
+size_t sj_paged_compact_workspace_bytes(long pages, long free_count);
+int sj_paged_compact(void *stream, const int32_t *table, long ldt, const int32_t *lengths, long requests,
+                     long page_size, long pages, long pages_after, const int32_t *shared, const int32_t *free_pages,
+                     long free_count, const int32_t *free_head, int32_t *table_after, int32_t *shared_after,
+                     int32_t *free_after, int32_t *copies, long capacity, int32_t *summary, void *workspace,
+                     size_t workspace_bytes);
+/* The keys and values of the listed pages: for each of copies [count][3] =
+ * (source, target, tokens) the first rows of `width` elements of the source page
+ * to the target page, in both caches of every layer (layer l at l * layer_stride
+ * elements).  Entries whose source or target is no page, or that have no
+ * tokens, are left out; tokens past the page size are not copied.  The targets
+ * of one call are distinct and none of them is a source.  Any strides and
+ * element alignment; at most 2^24 copies, below 2^30 times layers. */
+int sj_paged_copy(void *stream, void *k_cache, void *v_cache, long ldkv, int dtype, long layers, long layer_stride,
+                  long pages, long page_size, long width, const int32_t *copies, long count);
+/* sj_paged_attention where requests share the beginning of their sequences
+ * (beams of one prompt, a document that many ask about): group g is the
+ * requests group_starts[g] .. group_starts[g + 1] - 1 (group_starts [groups +
+ * 1], ascending), whose first prefix[g] positions hold the same keys and
+ * values: their table rows name the same pages there, or pages of the same
+ * content.  Those are read once for all rows of the group, from the first
+ * request's table row; every row's other keys as in sj_paged_attention, whose
+ * results these are but for the order of the sums.  starts [requests + 1]: the
+ * requests' first rows (sj_paged_plan's; null: row i is request i's).  A row
+ * attends alone, all its keys through its own table row, where its owner is
+ * in no group or its row not among the group's, where it does not see the
+ * whole prefix (its position, or a window), and where prefix[g] is 0 or less or
+ * longer than the table; all rows do where group_starts or their starts
+ * descend, and beyond 2048 rows, 1024 groups, 2^31 - 1 key tiles, or in heads
+ * of another width than multiples of 8.  Padded rows, bad pages, strides,
+ * types and limits as there; o may be q.  Workspace:
+ * sj_paged_attention_shared_workspace_bytes, 16-byte aligned, not cleared and
+ * not kept; calls that share one must not overlap. */
+size_t sj_paged_attention_shared_workspace_bytes(long rows, long hq, long hk, long head_dim, long groups);
+int sj_paged_attention_shared(void *stream, const void *q, long ldq, const void *k_cache, const void *v_cache, long ldkv,
+                              int dtype, long pages, long page_size, const int32_t *table, long ldt, long requests,
+                              const int32_t *owners, const int32_t *positions, long rows, const int32_t *starts,
+                              const int32_t *group_starts, const int32_t *prefix, long groups, long hq, long hk,
+                              long head_dim, long window, void *o, long ldo, float *lse, void *workspace,
+                              size_t workspace_bytes);
 
 /* ------------------------------------------- Hierarchical model patches
  * The byte <-> patch maps of the hierarchical (cfg3) model (hidden_from_
@@ -751,6 +837,34 @@ int sj_token_logprobs(void *stream, const void *x, int dtype, long ldx, long row
 int sj_token_logprobs_bwd(void *stream, const void *x, int dtype, long ldx, long rows, long vocab,
                           const int32_t *tokens, const float *stats, const float *entropy, const float *dlogprob,
                           const float *dentropy, void *dx, int dx_dtype, long lddx);
+/* One step of beam search for `groups` prompts of `beams` beams (no counterpart
+ * in the reference).  Row r = group * beams + beam of logits x [rows][ldx]
+ * (fp32 or bf16), scores [rows] the beams' sums of log probabilities.  A beam's
+ * candidates: every token v, total = score + ln softmax(x)[v]; of an ended beam
+ * (ended[r] != 0, nullable: none; its logits are not read) the end_token alone,
+ * total = score.  Per group the `keep` candidates of the highest rank, total /
+ * length^length_power with length = lengths[r] + 1 (an ended beam's lengths[r];
+ * 1 at least), the lowest beam * vocab + token first among equals, are written
+ * in their order to [groups][keep]: parents (the row; what sj_paged_fork
+ * takes), tokens, scores_after = total, lengths_after (nullable) = lengths + 1
+ * (an ended beam's lengths), ended_after (nullable) 1 where the beam had ended
+ * or the token is end_token (-1: no token is), else 0.  Sums, totals and ranks
+ * are formed in 64 bits; among a beam's own tokens the logits decide.  A logit
+ * of -inf is no candidate, nor any of a beam whose score or whose row's sum is
+ * not finite (a first step has one live beam, the others' scores -inf).
+ * Places without a candidate get parent and token -1, score -inf, length 0 and
+ * 1 in ended_after.  lengths is nullable where length_power is 0 and
+ * lengths_after null.  length_power 0 .. 16; beams and keep at most SJ_BEAM_MAX; vocab
+ * at most 2^24; rows times vocab / 8192 (rounded up) below 2^23; any stride and
+ * element alignment; the arrays after the step are not those before.  Workspace:
+ * sj_beam_select_workspace_bytes, 16-byte aligned, not cleared and not kept;
+ * calls that share one must not overlap. */
+#define SJ_BEAM_MAX 64
+size_t sj_beam_select_workspace_bytes(long groups, long beams, long vocab, long keep);
+int sj_beam_select(void *stream, const void *x, int dtype, long ldx, long groups, long beams, long vocab,
+                   const float *scores, const int32_t *lengths, const int32_t *ended, int32_t end_token,
+                   double length_power, long keep, int32_t *parents, int32_t *tokens, float *scores_after,
+                   int32_t *lengths_after, int32_t *ended_after, void *workspace, size_t workspace_bytes);
 /* Engine::gather, lib.rs:1010-1028 (kernel gather, kernels.py:241-245):
  * y [rows][d] = x[idx[r]] (row stride ldx) in y's dtype (a gather followed
  * by Graph::cast to F32 when yd = SJ_F32). */

@@ -113,6 +113,17 @@ SIGNATURES = {
     "sj_paged_attention_workspace_bytes": (_S, [_L, _L, _L, _L]),
     "sj_paged_attention": (_I, [_P, _P, _L, _P, _P, _L, _I, _L, _L, _P, _L, _L, _P, _P, _L, _L, _L, _L, _L, _P, _L,
                                 _P, _P, _S]),
+    "sj_paged_fork_workspace_bytes": (_S, [_L, _L, _L]),
+    "sj_paged_fork": (_I, [_P, _P, _L, _P, _L, _P, _L, _L, _L, _P, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _S]),
+    "sj_paged_compact_workspace_bytes": (_S, [_L, _L]),
+    "sj_paged_compact": (_I, [_P, _P, _L, _P, _L, _L, _L, _L, _P, _P, _L, _P, _P, _P, _P, _P, _L, _P, _P, _S]),
+    "sj_paged_copy": (_I, [_P, _P, _P, _L, _I, _L, _L, _L, _L, _L, _P, _L]),
+    "sj_paged_attention_shared_workspace_bytes": (_S, [_L, _L, _L, _L, _L]),
+    "sj_paged_attention_shared": (_I, [_P, _P, _L, _P, _P, _L, _I, _L, _L, _P, _L, _L, _P, _P, _L, _P, _P, _P, _L, _L,
+                                       _L, _L, _L, _P, _L, _P, _P, _S]),
+    "sj_beam_select_workspace_bytes": (_S, [_L, _L, _L, _L]),
+    "sj_beam_select": (_I, [_P, _P, _I, _L, _L, _L, _L, _P, _P, _P, ctypes.c_int32, _DB, _L, _P, _P, _P, _P, _P,
+                            _P, _S]),
     "sj_token_logprobs_workspace_bytes": (_S, [_L, _L, _L]),
     "sj_token_logprobs": (_I, [_P, _P, _I, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _P, _S]),
     "sj_token_logprobs_bwd": (_I, [_P, _P, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P, _I, _L]),

@@ -1,0 +1,477 @@
+// One step of beam search: of all beams of a prompt and all tokens, those whose
+// sequences are the most likely (no counterpart in the reference, which samples
+// one sequence).
+//
+//   L_b = ln sum_v e^(x_bv),  total_bv = s_b + (x_bv - L_b)
+//   rank_bv = total_bv / length_b^power
+//
+// Totals of different beams may lie next to each other, and which is the larger
+// decides what the search goes on with: sums, totals and ranks are 64 bits.
+// Within a beam the order is that of its logits, which are exact.
+#include "order.h"
+
+using namespace sj;
+
+namespace {
+
+constexpr int SLICE = 8192;   // entries of a slice
+constexpr int CAP = 1024;     // entries at or above a threshold that LDS holds
+
+struct BeamArgs {
+  const void* x;
+  long ldx;
+  int groups, B, V, keep, k;  // k: entries of a slice's list, min(keep, V)
+  int slices, width;          // of a row; width: entries of a slice, a multiple of 8
+  const float* scores;
+  const int32_t *lengths, *ended;
+  int end_token;
+  double power;
+  int32_t *parents, *tokens;
+  float* scores_after;
+  int32_t *lengths_after, *ended_after;
+  u64* flag;  // [rows][slices], of the meetings
+  u64 number;
+  u64* sums;  // [rows][slices] of (maximum, sum)
+  u64* keys;  // [rows][slices][k]
+};
+
+// e^d for d <= 0, to 2^-45: 2^n times a polynomial of degree 9 (least largest
+// relative error over half a step to each side, 1.6e-14).  Below -700 it is that
+// of -700, 1e-304, which no sum of 1 or more sees; NaN is NaN.
+__device__ __forceinline__ double exp_down(double d) {
+  const double magic = 6755399441055744.0;  // 1.5 2^52: the nearest whole number lies in the low bits
+  const double tm = fma(d, 1.4426950408889634, magic), f = fma(d, 1.4426950408889634, -(tm - magic));
+  double p = 1.0150995588009233e-07;
+  p = fma(p, f, 1.3259453829428669e-06);
+  p = fma(p, f, 1.5252982626321696e-05);
+  p = fma(p, f, 0.00015403434767100833);
+  p = fma(p, f, 0.0013333557617282988);
+  p = fma(p, f, 0.009618129192228842);
+  p = fma(p, f, 0.05550410866872767);
+  p = fma(p, f, 0.24022650695650039);
+  p = fma(p, f, 0.6931471805598701);
+  p = fma(p, f, 1.0000000000000127);
+  const long long b = __double_as_longlong(p);
+  return __hiloint2double((int)(b >> 32) + (__double2loint(tm) << 20), (int)b);
+}
+// e^(x - ref) in 64 bits
+__device__ __forceinline__ double power_of(float x, float ref, float low) {
+  return exp_down((double)(x < low ? low : x) - (double)ref);
+}
+
+// the order of finite ranks as whole numbers above 0
+__device__ __forceinline__ u64 rank_key(double r) {
+  const u64 b = (u64)__double_as_longlong(r + 0.0);
+  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+
+// ---------------------------------------------------------------- one row
+//
+// NT threads (a wave or a workgroup) hold entries [base, end) of a row, EV a
+// thread: the maximum, the sum of powers relative to it, and the k largest
+// entries in their order (put(place, key), key 0 where there are fewer).  As in
+// the token scores the largest come from a threshold, the k-th largest of 64 or
+// 256 column maxima.
+template <int NT, int EV>
+struct RowShared {
+  static constexpr int CAPR = NT == 64 ? 64 * EV : CAP;
+  u64 cand[CAPR], last[4];
+  double sum[4];
+  __attribute__((aligned(16))) float best[NT];
+  float max[4], T[4];
+  int n;
+};
+
+template <typename T, int NT, int EV, int E, class P>
+__device__ __forceinline__ void row_best(const T* x, int base, int end, int k, RowShared<NT, EV>& sh, float& m_out,
+                                         double& sum_out, P put) {
+  typedef Unit<T, E> U;
+  constexpr int NU = EV / E, NW = NT / 64, CAPR = RowShared<NT, EV>::CAPR;
+  const int t = threadIdx.x % NT, lane = threadIdx.x & 63, w = t >> 6;
+  auto sync = [] {
+    if constexpr (NT == 64)
+      sync_wave();
+    else
+      __syncthreads();
+  };
+  auto index = [&](int i) { return base + E * (t + NT * (i / E)) + i % E; };
+  U u[NU];
+#pragma unroll
+  for (int i = 0; i < NU; i++) {
+    const int v = base + E * (t + NT * i);
+    if (v + E <= end) u[i].r = *(const typename U::Raw*)(x + v);
+  }
+  constexpr int PART = 4, PARTS = EV / PART;
+  float pm[PARTS], best = -INFINITY;
+  auto f = [&](int i) { return u[i / E].get(i % E); };
+#pragma unroll
+  for (int i = 0; i < NU; i++) {
+    const int v = base + E * (t + NT * i);
+    if (v < end) {
+      if (v + E > end) {  // a unit that crosses the end is filled with -inf
+#pragma unroll
+        for (int e = 0; e < E; e++) u[i].set(e, v + e < end ? at_f32(x, v + e) : -INFINITY);
+      }
+#pragma unroll
+      for (int j = i * E / PART; j < (i + 1) * E / PART; j++) {
+        pm[j] = fmaxf(fmaxf(f(PART * j), f(PART * j + 1)), fmaxf(f(PART * j + 2), f(PART * j + 3)));
+        best = fmaxf(best, pm[j]);
+      }
+    }
+  }
+  float m = all_max(best);
+  if (t == 0) sh.n = 0;
+  if (NT > 64) {
+    sh.best[t] = best;
+    if (lane == 0) sh.max[w] = m;
+    sync();
+    m = fmaxf(fmaxf(sh.max[0], sh.max[1]), fmaxf(sh.max[2], sh.max[3]));
+  }
+  if (w == 0 || k > 32) {
+    const bool all = NT > 64 && k > 32;
+    float col = best;
+    if (NT > 64 && !all) col = fmaxf(fmaxf(best, sh.best[lane + 64]), fmaxf(sh.best[lane + 128], sh.best[lane + 192]));
+    if (!all) sh.best[lane] = col;
+    sync_wave();
+    int larger = 0;
+    for (int j = 0; j < (all ? 256 : 64); j += 64)
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        const f32x4 c = *(const f32x4*)(sh.best + j + i);
+        larger += (c[0] > col) + (c[1] > col) + (c[2] > col) + (c[3] > col);
+      }
+    const float least = all_min(larger < k ? col : INFINITY);
+    if (NT == 64 ? lane == 0 : all ? lane == 0 : lane < 4) sh.T[NT == 64 ? 0 : all ? w : lane] = least;
+  }
+  // -inf has no share in the sum (its power is that of -700); where there is
+  // nothing else, the sum is only asked for NaN
+  const float ref = m == -INFINITY ? 0.f : m, low = ref - 700.f;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < NU; i++)
+    if (base + E * (t + NT * i) < end)
+#pragma unroll
+      for (int e = 0; e < E; e++) sum += power_of(f(i * E + e), ref, low);
+  sum = wave_sum(sum);
+  if (NT > 64) {
+    if (lane == 0) sh.sum[w] = sum;
+    sync();
+    sum = (sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]);
+  } else {
+    sync();
+  }
+  m_out = m;
+  sum_out = m == -INFINITY && sum == sum ? 0.0 : sum;
+  const float T0 = NT == 64 ? sh.T[0] : fminf(fminf(sh.T[0], sh.T[1]), fminf(sh.T[2], sh.T[3]));
+  uint32_t mine = 0;
+#pragma unroll
+  for (int j = 0; j < PARTS; j++)
+    if (index(PART * j) < end && pm[j] >= T0)
+#pragma unroll
+      for (int i = PART * j; i < PART * (j + 1); i++) mine += f(i) >= T0 && index(i) < end;
+  const uint32_t upto = scan_add(mine);
+  int from = 0;
+  if (lane == 63 && upto) from = atomicAdd(&sh.n, (int)upto);
+  from = __builtin_amdgcn_readlane(from, 63) + (int)(upto - mine);
+#pragma unroll
+  for (int j = 0; j < PARTS; j++)
+    if (index(PART * j) < end && pm[j] >= T0) {
+#pragma unroll
+      for (int i = PART * j; i < PART * (j + 1); i++)
+        if (f(i) >= T0 && index(i) < end) {
+          if (from < CAPR) sh.cand[from] = order_key(f(i), index(i));
+          from++;
+        }
+    }
+  sync();
+  const int n = sh.n, held = min(k, end - base);
+  if (n <= CAPR && n >= held) {
+    rank<NT>(sh.cand, n, k, t, put);
+    for (int i = held + t; i < k; i += NT) put(i, 0ull);
+    return;
+  }
+  // more than LDS holds at the threshold (a masked row's -inf), or fewer
+  // entries than asked for beside NaN: the largest below the last, k times
+  u64 last = ~0ull;
+  for (int j = 0; j < k; j++) {
+    u64 k0 = 0;
+    for (int v = base + t; v < end; v += NT) {
+      const u64 key = order_key(at_f32(x, v), v);
+      if (key < last && key > k0) k0 = key;
+    }
+    k0 = all_max(k0);
+    if (NT > 64) {
+      sync();
+      if (lane == 0) sh.last[w] = k0;
+      sync();
+#pragma unroll
+      for (int i = 0; i < NW; i++) k0 = larger_of(k0, sh.last[i]);
+    }
+    last = k0;
+    if (t == 0) put(j, k0);
+  }
+}
+
+// ------------------------------------------------------------- the prompt
+//
+// One workgroup takes the lists of a prompt's beams together: their sums, the
+// ranks of all entries, and the `keep` first of them, again through a threshold.
+struct GroupShared {
+  double base[64], factor[64];  // the beam's L (of an ended one its score), length^power
+  int live[64];                 // 0: no candidate, 1: its tokens, 2: ended
+  u64 cand[CAP];
+  int32_t where[CAP];
+  double total[CAP];
+  u64 best[256], last[4];
+  int at[4];
+  int n;
+};
+struct Candidate {
+  u64 key;  // 0: none
+  int flat;
+  double total;
+};
+
+template <bool MEET>
+__device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared& sh) {
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, B = a.B, S = a.slices, k = a.k, keep = a.keep;
+  const long row0 = (long)g * B;
+  const u64* keys = a.keys + row0 * S * k;
+  for (int b = w; b < B; b += 4) {
+    const long row = row0 + b;
+    const float score = a.scores[row];
+    const bool ended = a.ended && a.ended[row];
+    double base = score;
+    int live = score == score && fabsf(score) < INFINITY ? 2 : 0;
+    if (!ended) {
+      const u64* sums = a.sums + 2 * row * S;
+      auto get = [&](const u64* p) { return MEET ? part_get(p) : *p; };
+      float M = -INFINITY;
+      for (int s = lane; s < S; s += 64) M = fmaxf(M, __uint_as_float((uint32_t)get(sums + 2 * s)));
+      M = all_max(M);
+      double sum = 0.0;
+      for (int s = lane; s < S; s += 64) {
+        const float m = __uint_as_float((uint32_t)get(sums + 2 * s));
+        const double v = __longlong_as_double((long long)get(sums + 2 * s + 1));
+        sum += v * power_of(m, M == -INFINITY ? 0.f : M, M == -INFINITY ? -700.f : M - 700.f);
+      }
+      sum = wave_sum(sum);
+      base = (double)M + log(sum);
+      if (live) live = base == base && fabs(base) < INFINITY ? 1 : 0;
+    }
+    if (lane == 0) {
+      const int len = a.lengths ? a.lengths[row] : 0;
+      const long after = max(ended ? (long)len : len + 1L, 1L);
+      sh.base[b] = base;
+      sh.live[b] = live;
+      sh.factor[b] = a.power == 0.0 ? 1.0 : pow((double)after, a.power);
+    }
+  }
+  if (t == 0) sh.n = 0;
+  __syncthreads();
+  const int all = B * S * k;
+  auto candidate = [&](int i) {
+    Candidate c = {0, 0, 0.0};
+    if (i >= all) return c;
+    const int b = i / (S * k), in = i - b * S * k, live = sh.live[b];
+    if (live == 1) {
+      const u64 key = MEET ? part_get(keys + i) : keys[i];
+      const float x = key_value(key);
+      if (key == 0 || x == -INFINITY) return c;
+      c.total = (double)a.scores[row0 + b] + ((double)x - sh.base[b]);
+      c.flat = b * a.V + key_index(key);
+    } else if (live == 2 && in == 0) {
+      c.total = sh.base[b];
+      c.flat = b * a.V + max(a.end_token, 0);
+    } else {
+      return c;
+    }
+    c.key = rank_key(a.power == 0.0 ? c.total : c.total / sh.factor[b]);
+    return c;
+  };
+  constexpr int HELD = 4;
+  Candidate c[HELD];
+  u64 best = 0;
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    c[i] = candidate(t + 256 * i);
+    best = larger_of(best, c[i].key);
+  }
+  for (int i = t + 256 * HELD; i < all; i += 256) best = larger_of(best, candidate(i).key);
+  sh.best[t] = best;
+  __syncthreads();
+  // the threshold: the keep-th largest of the threads' largest, 1 where fewer
+  // have any
+  int larger = 0;
+  for (int i = 0; i < 256; i++) larger += sh.best[i] > best;
+  u64 least = larger < keep && best ? best : ~0ull;
+  int have = __syncthreads_count(best != 0);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const u64 o = __shfl_xor(least, d, 64);
+    least = o < least ? o : least;
+  }
+  if (lane == 0) sh.last[w] = least;
+  __syncthreads();
+  u64 T0 = 1;
+  if (have >= keep) {
+    T0 = sh.last[0];
+    for (int i = 1; i < 4; i++) T0 = sh.last[i] < T0 ? sh.last[i] : T0;
+  }
+  auto collect = [&](const Candidate& q) {
+    if (q.key >= T0) {
+      const int n = atomicAdd(&sh.n, 1);
+      if (n < CAP) sh.cand[n] = q.key, sh.where[n] = q.flat, sh.total[n] = q.total;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; i++) collect(c[i]);
+  for (int i = t + 256 * HELD; i < all; i += 256) collect(candidate(i));
+  __syncthreads();
+  auto write = [&](int place, bool some, int flat, double total) {
+    const long at = (long)g * keep + place;
+    const int b = some ? flat / a.V : 0, token = flat - b * a.V;
+    const long row = row0 + b;
+    const bool was = some && sh.live[b] == 2;
+    a.parents[at] = some ? (int)row : -1;
+    a.tokens[at] = !some ? -1 : was ? a.end_token : token;
+    a.scores_after[at] = some ? (float)total : -INFINITY;
+    if (a.lengths_after) a.lengths_after[at] = some ? (a.lengths ? a.lengths[row] : 0) + (was ? 0 : 1) : 0;
+    if (a.ended_after) a.ended_after[at] = !some || was || token == a.end_token;
+  };
+  const int n = sh.n;
+  if (n <= CAP) {
+    for (int i = t >> 2; i < n; i += 64) {
+      const u64 key = sh.cand[i];
+      const int flat = sh.where[i];
+      uint32_t place = 0;
+      for (int j = t & 3; j < n; j += 4) place += sh.cand[j] > key || (sh.cand[j] == key && sh.where[j] < flat);
+      place += dpp<0xB1>(place);
+      place += dpp<0x4E>(place);
+      if ((t & 3) == 0 && (int)place < keep) write((int)place, true, flat, sh.total[i]);
+    }
+    for (int i = n + t; i < keep; i += 256) write(i, false, 0, 0.0);
+    return;
+  }
+  // more of the same rank than LDS holds: the first behind the last, keep times
+  u64 last = ~0ull;
+  int last_flat = -1;
+  for (int j = 0; j < keep; j++) {
+    Candidate top = {0, 0x7fffffff, 0.0};
+    for (int i = t; i < all; i += 256) {
+      const Candidate q = candidate(i);
+      const bool behind = q.key && (q.key < last || (q.key == last && q.flat > last_flat));
+      if (behind && (q.key > top.key || (q.key == top.key && q.flat < top.flat))) top = q;
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      const u64 key = __shfl_xor(top.key, d, 64);
+      const int flat = __shfl_xor(top.flat, d, 64);
+      const double total = __shfl_xor(top.total, d, 64);
+      if (key > top.key || (key == top.key && flat < top.flat)) top = Candidate{key, flat, total};
+    }
+    __syncthreads();
+    if (lane == 0) sh.cand[w] = top.key, sh.where[w] = top.flat, sh.total[w] = top.total;
+    __syncthreads();
+    for (int i = 0; i < 4; i++)
+      if (sh.cand[i] > top.key || (sh.cand[i] == top.key && sh.where[i] < top.flat))
+        top = Candidate{sh.cand[i], sh.where[i], sh.total[i]};
+    if (t == 0) write(j, top.key != 0, top.key ? top.flat : 0, top.total);
+    last = top.key;
+    last_flat = top.flat;
+  }
+}
+
+template <typename T, int NT, int EV, int E = WIDE<T>>
+__global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
+  __shared__ RowShared<NT, EV> sh[256 / NT];
+  const int gt = threadIdx.x / NT, item = blockIdx.x * (256 / NT) + gt;
+  const long row = NT == 64 ? item : item / a.slices;
+  if (row >= (long)a.groups * a.B) return;
+  const int slice = NT == 64 ? 0 : item - (int)row * a.slices;
+  if (a.ended && a.ended[row]) return;
+  const int base = slice * a.width, end = min(a.V, base + a.width);
+  float m;
+  double sum;
+  u64* list = a.keys + (row * a.slices + slice) * a.k;
+  row_best<T, NT, EV, E>((const T*)a.x + row * a.ldx, base, end, a.k, sh[gt], m, sum,
+                         [&](int place, u64 key) { list[place] = key; });
+  if (threadIdx.x % NT == 0) {
+    u64* p = a.sums + 2 * (row * a.slices + slice);
+    p[0] = __float_as_uint(m);
+    p[1] = (u64)__double_as_longlong(sum);
+  }
+}
+__global__ __launch_bounds__(256) void k_beam_join(BeamArgs a) {
+  __shared__ GroupShared sh;
+  group_best<false>(a, blockIdx.x, sh);
+}
+
+long slices_of(long vocab) { return (vocab + SLICE - 1) / SLICE; }
+
+template <typename T>
+void launch_select(hipStream_t s, BeamArgs& a) {
+  const long rows = (long)a.groups * a.B;
+  a.slices = 1;
+  a.width = (a.V + 7) / 8 * 8;
+  if (a.V <= 512) {
+    k_beam_rows<T, 64, 8, 4><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
+  } else if (a.V <= 1024) {
+    k_beam_rows<T, 64, 16><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
+  } else if (a.V <= 4096) {
+    k_beam_rows<T, 256, 16><<<(unsigned)rows, 256, 0, s>>>(a);
+  } else {
+    a.slices = (int)slices_of(a.V);
+    a.width = ((a.V + a.slices - 1) / a.slices + 7) / 8 * 8;
+    k_beam_rows<T, 256, 32><<<(unsigned)(rows * a.slices), 256, 0, s>>>(a);
+  }
+  k_beam_join<<<(unsigned)a.groups, 256, 0, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" size_t sj_beam_select_workspace_bytes(long groups, long beams, long vocab, long keep) {
+  if (groups <= 0 || beams <= 0 || vocab <= 0 || keep <= 0) return 0;
+  return (size_t)groups * beams * slices_of(vocab) * (24 + 8 * (size_t)(keep < vocab ? keep : vocab));
+}
+
+extern "C" int sj_beam_select(void* stream, const void* x, int dtype, long ldx, long groups, long beams, long vocab,
+                              const float* scores, const int32_t* lengths, const int32_t* ended, int32_t end_token,
+                              double length_power, long keep, int32_t* parents, int32_t* tokens, float* scores_after,
+                              int32_t* lengths_after, int32_t* ended_after, void* workspace, size_t workspace_bytes) {
+  SJ_REQUIRE(dtype == SJ_F32 || dtype == SJ_BF16, "beam selection dtype %d", dtype);
+  SJ_REQUIRE(groups >= 0 && groups <= 1L << 24 && beams > 0 && beams <= SJ_BEAM_MAX && keep > 0 && keep <= SJ_BEAM_MAX &&
+                 vocab > 0 && vocab <= 1L << 24 && ldx >= vocab,
+             "beam selection: %ld prompts of %ld beams, %ld of %ld (stride %ld)", groups, beams, keep, vocab, ldx);
+  SJ_REQUIRE(groups * beams * slices_of(vocab) < 1L << 23, "beam selection: %ld rows of %ld", groups * beams, vocab);
+  SJ_REQUIRE(end_token >= -1 && end_token < vocab, "beam selection: end token %d of %ld", end_token, vocab);
+  SJ_REQUIRE(length_power >= 0.0 && length_power <= 16.0, "beam selection: length power %g", length_power);
+  if (groups == 0) return SJ_OK;
+  SJ_REQUIRE(x && scores && parents && tokens && scores_after && (length_power == 0.0 || lengths) &&
+                 (lengths_after == nullptr || lengths),
+             "beam selection: null");
+  SJ_REQUIRE((const float*)scores_after != scores && (!lengths_after || (const int32_t*)lengths_after != lengths) &&
+                 (!ended_after || (const int32_t*)ended_after != ended),
+             "beam selection: the beams after the step need arrays of their own");
+  const size_t need = sj_beam_select_workspace_bytes(groups, beams, vocab, keep);
+  SJ_REQUIRE(((uintptr_t)workspace & 15) == 0, "beam selection: the workspace is not 16-byte aligned");
+  if (need > workspace_bytes || !workspace)
+    return sjh::fail(SJ_ERR_CAPACITY, "beam selection workspace: required %zu bytes, available %zu bytes", need,
+                     workspace ? workspace_bytes : 0);
+  BeamArgs a = {};
+  a.x = x; a.ldx = ldx; a.groups = (int)groups; a.B = (int)beams; a.V = (int)vocab; a.keep = (int)keep;
+  a.k = (int)(keep < vocab ? keep : vocab);
+  a.scores = scores; a.lengths = lengths; a.ended = ended; a.end_token = end_token; a.power = length_power;
+  a.parents = parents; a.tokens = tokens; a.scores_after = scores_after;
+  a.lengths_after = lengths_after; a.ended_after = ended_after;
+  const size_t all = (size_t)groups * beams * slices_of(vocab);
+  a.sums = (u64*)workspace;
+  a.flag = a.sums + 2 * all;
+  a.keys = a.flag + all;
+  if (dtype == SJ_BF16)
+    launch_select<bf16_t>((hipStream_t)stream, a);
+  else
+    launch_select<float>((hipStream_t)stream, a);
+  SJ_LAUNCH_CHECK("beam selection");
+  return SJ_OK;
+}
