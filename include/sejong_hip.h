@@ -509,7 +509,7 @@ int sj_paged_copy(void *stream, void *k_cache, void *v_cache, long ldkv, int dty
  * in no group or its row not among the group's, where it does not see the
  * whole prefix (its position, or a window), and where prefix[g] is 0 or less or
  * longer than the table; all rows do where group_starts or their starts
- * descend, and beyond 2048 rows, 1024 groups, 2^31 - 1 key tiles, or in heads
+ * descend, and beyond 2048 rows, 256 groups, 2^31 - 1 key tiles, or in heads
  * of another width than multiples of 8.  Padded rows, bad pages, strides,
  * types and limits as there; o may be q.  Workspace:
  * sj_paged_attention_shared_workspace_bytes, 16-byte aligned, not cleared and

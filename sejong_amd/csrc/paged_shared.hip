@@ -27,7 +27,7 @@ namespace {
 
 constexpr int CT = 2, COLS = 16 * CT, BLOCK = 4 * COLS;
 constexpr int WIDE_PLACE = 64;  // keys of a place of a walk whose waves go by columns
-constexpr int MAX_ROWS = 2048, MAX_GROUPS = 1024;
+constexpr int MAX_ROWS = 2048, MAX_GROUPS = 256;  // what LDS lists beside two stages of tiles
 constexpr int GROUPS_OF_WAVES = 512;  // workgroups, at most
 
 struct SharedArgs {
@@ -44,18 +44,18 @@ struct SharedArgs {
   int lead_slot, own_slot;
 };
 
-// index of the last of n ascending values that is at or below y (v[0] is):
-// counted by 16s or 32s, then within
+// index of the last of n <= 64 STEP ascending values that is at or below y (below
+// 0 if none is): counted by STEPs, then within
 template <int STEP>
 __device__ __forceinline__ int last_at(const int* v, int n, int y, int lane) {
   const int far = STEP * lane;
   const int c = STEP * (__popcll(__ballot(far < n && v[min(far, n - 1)] <= y)) - 1);
-  return c + __popcll(__ballot(lane < STEP && c + lane < n && v[min(c + lane, n - 1)] <= y)) - 1;
+  return c + __popcll(__ballot(lane < STEP && c + lane < n && v[max(min(c + lane, n - 1), 0)] <= y)) - 1;
 }
 
 // -------------------------------------------------------- staged key tiles
 //
-// 32 or 64 keys and their values go through LDS (two stages), and each wave
+// 64 keys and their values go through LDS (two stages), and each wave
 // multiplies all of them with its own 32 columns: a key is read once for 128
 // columns, and with neighbouring lanes along its row.  (Operands loaded straight
 // from memory have neighbouring lanes on different keys, each an access of its
@@ -82,9 +82,9 @@ __device__ __forceinline__ float column_sum(float v) {
 template <int DC>
 struct Staged {
   static constexpr int POS = DC == 1 ? 4 : DC == 2 ? 8 : 16, RB = 16 * POS;  // chunks and bytes of a row in LDS
-  static constexpr int KT = DC > 2 ? 32 : 64, KS = KT / 16, TILE = KT * RB, STAGE = 2 * TILE, LDS = 2 * STAGE;
+  static constexpr int KT = 64, KS = KT / 16, TILE = KT * RB, STAGE = 2 * TILE, LDS = 2 * STAGE;
   static constexpr int MINE = KT / 4, ROWS = 1024 / RB, LOADS = MINE / ROWS;  // keys a wave brings, rows of a load
-  static constexpr int NO = 2 * DC, FULL = DC == 1 ? 0 : DC - 1;  // chunks of 32 columns that every width has
+  static constexpr int NO = 2 * DC;
 
   u32x4 q[CT][DC];
   f32x4 o[CT][NO];
@@ -133,47 +133,52 @@ struct Staged {
       v[i] = load16(V + at);
     }
   }
-  // to a stage, values of keys without a slot as zeros (whatever lies there counts
-  // 0 times 0); and which keys there are
-  __device__ __forceinline__ void store(uint8_t* stage, uint32_t* valid, int w, int lane) {
+  // to a stage, columns past the head and values of keys without a slot as zeros
+  // (whatever lies there counts 0 times 0); and which keys there are
+  __device__ __forceinline__ void store(const PagedArgs& a, uint8_t* stage, uint32_t* valid, int w, int lane) {
     const uint32_t there = (uint32_t)__ballot(sl >= 0) & ((1u << MINE) - 1);
     if (lane == 0) valid[w] = there;
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
       const int row = ROWS * i + lane / POS;
       uint8_t* to = stage + (MINE * w + row) * RB + 16 * ((lane % POS) ^ turn(MINE * w + row));
-      *(u32x4*)to = k[i];
+      *(u32x4*)to = 8 * (lane % POS) < a.D ? k[i] : u32x4{0u, 0u, 0u, 0u};
       *(u32x4*)(to + TILE) = (there >> row) & 1 ? v[i] : u32x4{0u, 0u, 0u, 0u};
     }
   }
   __device__ __forceinline__ void multiply(const PagedArgs& a, const uint8_t* stage, const uint32_t* valid, int nt, int lane) {
     const int g = lane >> 4, k15 = lane & 15, tk = turn(k15);
+    const u32x4 there = *(const u32x4*)valid;
+    const uint8_t* krow = stage + k15 * RB;
     f32x4 p[CT][KS];
+    // the next 16 keys are on their way while these are multiplied
+    u32x4 kk[2][DC];
+    auto keys = [&](int s) {
+#pragma unroll
+      for (int c = 0; c < DC; c++) kk[s & 1][c] = *(const u32x4*)(krow + 16 * s * RB + 16 * ((4 * c + g) ^ tk));
+    };
+    keys(0);
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      f32x4 acc[CT];
+      if (s + 1 < KS) keys(s + 1);
+      __builtin_amdgcn_sched_barrier(0);  // the compiler would put each read before its use
 #pragma unroll
-      for (int ct = 0; ct < CT; ct++) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int ct = 0; ct < CT; ct++) p[ct][s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < DC; c++) {
-        u32x4 kk = *(const u32x4*)(stage + (16 * s + k15) * RB + 16 * ((4 * c + g) ^ tk));
-        if (c >= FULL && (4 * c + g) * 8 >= a.D) kk = u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++)
-          acc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk),
-                                                            __builtin_bit_cast(bf16x8, q[ct][c]), acc[ct], 0, 0, 0);
-      }
-      const uint32_t there = MINE == 16 ? valid[s] : valid[2 * s] | valid[2 * s + 1] << 8;
-      if (there != 0xffffu) {
+      for (int c = 0; c < DC; c++)
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (!((there >> (4 * g + i)) & 1)) acc[ct][i] = -INFINITY;
-      }
-#pragma unroll
-      for (int ct = 0; ct < CT; ct++) p[ct][s] = acc[ct];
+          p[ct][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk[s & 1][c]),
+                                                             __builtin_bit_cast(bf16x8, q[ct][c]), p[ct][s], 0, 0, 0);
     }
+    if ((there[0] & there[1] & there[2] & there[3]) != 0xffffu)
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (!((there[s] >> (4 * g + i)) & 1))
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) p[ct][s][i] = -INFINITY;
     const float c = a.scale;
     float top[CT];
     bool passed = false;
@@ -212,34 +217,41 @@ struct Staged {
       l[ct] += sum;  // this lane's keys alone: joined in run()
     }
     const int e = (lane >> 2) & 3, tv = turn(4 * g + e), half = 8 * (lane & 1), odd = (lane >> 1) & 1;
-    const uint8_t* v = stage + TILE + (4 * g + e) * RB + half;
+    const uint8_t* vrow = stage + TILE + (4 * g + e) * RB + half;
+    bf16x8 vt[2];
+    auto values = [&](int n) {  // n-th of the products: 32 keys, 16 columns
+      const int s = 2 * (n / NO), d = n % NO;
+      s16x4 r[2];
 #pragma unroll
-    for (int s = 0; s < KS; s += 2) {
-      u32x4 ph[CT], pl[CT];
+      for (int h = 0; h < 2; h++)
+        r[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vrow + 16 * (s + h) * RB + 16 * ((2 * d + odd) ^ tv)));
+      vt[n & 1] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    values(0);
+    u32x4 ph[CT], pl[CT];
+#pragma unroll
+    for (int n = 0; n < KS / 2 * NO; n++) {
+      const int s = 2 * (n / NO), d = n % NO;
+      if (d == 0) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const float x = p[ct][s + h][2 * i], y = p[ct][s + h][2 * i + 1];
+              const uint32_t w = cvt2(x, y);
+              ph[ct][2 * h + i] = w;
+              pl[ct][2 * h + i] = cvt2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xffff0000u));
+            }
+      }
+      if (n + 1 < KS / 2 * NO) values(n + 1);
 #pragma unroll
       for (int ct = 0; ct < CT; ct++)
+        o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[n & 1], __builtin_bit_cast(bf16x8, ph[ct]), o[ct][d], 0, 0, 0);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const float x = p[ct][s + h][2 * i], y = p[ct][s + h][2 * i + 1];
-            const uint32_t w = cvt2(x, y);
-            ph[ct][2 * h + i] = w;
-            pl[ct][2 * h + i] = cvt2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xffff0000u));
-          }
-#pragma unroll
-      for (int d = 0; d < NO; d++) {
-        s16x4 r[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-          r[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v + 16 * (s + h) * RB + 16 * ((2 * d + odd) ^ tv)));
-        const bf16x8 vt = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-          o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, __builtin_bit_cast(bf16x8, ph[ct]), o[ct][d], 0, 0, 0);
-          o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, __builtin_bit_cast(bf16x8, pl[ct]), o[ct][d], 0, 0, 0);
-        }
-      }
+      for (int ct = 0; ct < CT; ct++)
+        o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[n & 1], __builtin_bit_cast(bf16x8, pl[ct]), o[ct][d], 0, 0, 0);
     }
   }
   // tiles t0 .. t1 - 1 of the keys [0, hi); every wave of the workgroup, those
@@ -256,7 +268,7 @@ struct Staged {
     look(a, pages, t0, hi, w, lane);
     fetch(t0);
     __syncthreads();  // the walk before has read its tiles
-    store(lds, valid[0], w, lane);
+    store(a, lds, valid[0], w, lane);
     if (t0 + 1 < t1) fetch(t0 + 1);
     __syncthreads();
     for (int t = t0; t < t1; t++) {
@@ -264,7 +276,7 @@ struct Staged {
       if (nt) multiply(a, lds + now * STAGE, valid[now], nt, lane);
       if (t + 1 == t1) break;
       // the other stage was read before the last barrier
-      store(lds + (now ^ 1) * STAGE, valid[now ^ 1], w, lane);
+      store(a, lds + (now ^ 1) * STAGE, valid[now ^ 1], w, lane);
       if (t + 2 < t1) fetch(t + 2);
       __syncthreads();
     }
@@ -306,13 +318,24 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
   // requests, rows, places, slots and keys of the groups
   __shared__ int g_request[MAX_GROUPS + 1], g_row[MAX_GROUPS + 1], g_pre[MAX_GROUPS + 1], g_sub[MAX_GROUPS],
       g_keys[MAX_GROUPS];
-  __shared__ int pre[MAX_ROWS + 1], from[MAX_ROWS];  // a row's places before it, its first own key
-  __shared__ uint32_t valid[2][4];
+  __shared__ int pre[MAX_ROWS + 1];  // the places before a row
+  __shared__ __attribute__((aligned(16))) uint32_t valid[2][4];
   __shared__ int ws[2][4];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, nb = a.HK * a.QT, ng = s.groups;
   const int most = (int)(a.ldt * a.P);
   constexpr int PLACE = 4 * W::KT;  // keys of a place of a row's own walk: four tiles
 
+  // the rows' positions and requests, asked for early (what row_range reads)
+  constexpr int HELD = MAX_ROWS / 256;
+  const int per_row = (a.rows + 255) / 256;
+  int held_pos[HELD], held_owner[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    const int r = t * per_row + i;
+    const bool in = i < per_row && r < a.rows;
+    held_pos[i] = in ? a.positions[r] : -1;
+    held_owner[i] = in && a.owners ? a.owners[r] : r;
+  }
   // the groups: requests, rows and shared keys
   for (int g = t; g <= ng; g += 256) {
     const int r = min(max(s.group_starts[g], 0), a.requests);
@@ -378,30 +401,32 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
   }
   const int lead = g_pre[ng];
 
+  // Whether row r, of a request in group g, walks its group's keys: it sees all
+  // of them.  Among groups without requests the last at or before the owner is
+  // the one that has it.
+  auto shares = [&](int g, int r, int owner, int lo, int hi) {
+    return lo == 0 && owner >= g_request[g] && owner < g_request[g + 1] && r >= g_row[g] && r < g_row[g + 1] &&
+           g_keys[g] > 0 && g_keys[g] <= hi;
+  };
   // the rows: where their own keys begin
   {
-    constexpr int MOST = MAX_ROWS / 256;
-    const int per = (a.rows + 255) / 256;
-    int n[MOST], group[MOST], mine = 0;
+    int n[HELD], group[HELD], from[HELD], mine = 0;
 #pragma unroll
-    for (int i = 0; i < MOST; i++) {
-      n[i] = 0;
+    for (int i = 0; i < HELD; i++) {
+      n[i] = from[i] = 0;
       group[i] = -1;
-      const int r = t * per + i;
-      int owner, lo, hi;
-      if (i < per && r < a.rows && row_range(a, r, owner, lo, hi)) {
-        if (lead > 0 && lo == 0) {
+      const int r = t * per_row + i;
+      int lo, hi;
+      if (i < per_row && r < a.rows && range_of(a, held_pos[i], held_owner[i], lo, hi)) {
+        if (lead > 0) {
           int g = 0, e = ng;  // the last group that begins at or before the owner
           while (e - g > 1) {
             const int m = (g + e) >> 1;
-            if (g_request[m] <= owner) g = m; else e = m;
+            if (g_request[m] <= held_owner[i]) g = m; else e = m;
           }
-          // among groups without requests it is the last, the one that has them
-          if (owner >= g_request[g] && owner < g_request[g + 1] && r >= g_row[g] && r < g_row[g + 1] && g_keys[g] > 0 &&
-              g_keys[g] <= hi)
-            group[i] = g, lo = g_keys[g];
+          if (shares(g, r, held_owner[i], lo, hi)) group[i] = g, lo = g_keys[g];
         }
-        from[r] = lo;
+        from[i] = lo;
         n[i] = tiles_of(hi - lo, PLACE);
       }
       mine += n[i];
@@ -415,18 +440,22 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
     if (t == 255) pre[a.rows] = at;
     at -= mine;
 #pragma unroll
-    for (int i = 0; i < MOST; i++) {
-      const int r = t * per + i;
-      if (i < per && r < a.rows) {
+    for (int i = 0; i < HELD; i++) {
+      const int r = t * per_row + i;
+      if (i < per_row && r < a.rows) {
         pre[r] = at;
-        if (blockIdx.x == 0) s.row_info[r] = make_int4(from[r], group[i], at, n[i]);
+        if (blockIdx.x == 0) s.row_info[r] = make_int4(from[i], group[i], at, n[i]);
         at += n[i];
       }
     }
     __syncthreads();
   }
-  const int own = pre[a.rows] * nb, waves = 4 * gridDim.x;
-  const int piece = max(1, (int)(((long)lead + gridDim.x - 1) / gridDim.x)), own_piece = max(1, (int)(((long)own + waves - 1) / waves));
+  // where there are workgroups enough, some take shared walks and the others own
+  // ones, else all of them both
+  const int own = pre[a.rows] * nb, all = gridDim.x;
+  const bool apart = (long)lead + (own + 3) / 4 <= all;
+  const int own_groups = apart ? all - lead : all, waves = 4 * max(own_groups, 1);
+  const int piece = max(1, (int)(((long)lead + all - 1) / all)), own_piece = max(1, (int)(((long)own + waves - 1) / waves));
   if (blockIdx.x == 0) {
     for (int g = t; g < ng; g += 256) {
       const Group r = group_of(g);
@@ -435,15 +464,16 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
     }
     if (t == 0) *s.line = make_int2(piece, own_piece);
   }
-  // neighbours on the line on one XCD, where there is a piece for everybody:
-  // the blocks of columns of one KV head walk the same keys
-  const int b = piece > 1 ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
+  // Neighbours on the line on different XCDs: a KV head's rows lie in a few of an
+  // L2's channels (64 rows over 16384 keys, 8 heads of 128, a head to an XCD: 49
+  // us, its loads at 3.6 TB/s whatever else it does)
+  const int b = blockIdx.x;
   int x = (int)min((long)lead, (long)b * piece);
   const int e = (int)min((long)lead, (long)x + piece);
   const int quads = a.D / 4, lane0 = lane;
   while (x < e) {
     const int lane = here(lane0);
-    const int g = __builtin_amdgcn_readfirstlane(last_at<16>(g_pre, ng, x, lane));
+    const int g = __builtin_amdgcn_readfirstlane(last_at<4>(g_pre, ng, x, lane));
     const Group r = group_of(g);
     const int keys = __builtin_amdgcn_readfirstlane(g_keys[g]), places = r.places, in = x - g_pre[g];
     const int walk = __builtin_amdgcn_readfirstlane(in / places), c0 = in - walk * places, c1 = min(places, c0 + e - x);
@@ -521,7 +551,9 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
   }
   __syncthreads();  // the waves' tiles lie elsewhere in the rows' own walks
   // a wave's piece; those of one workgroup lie apart, so that few walks go over all workgroups
-  const int wave = w * gridDim.x + blockIdx.x;
+  const int mine = apart ? (int)blockIdx.x - lead : (int)blockIdx.x;
+  if (mine < 0) return;
+  const int wave = w * own_groups + mine;
   int y = (int)min((long)own, (long)wave * own_piece);
   const int ye = (int)min((long)own, (long)y + own_piece);
   while (y < ye) {
@@ -534,7 +566,11 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
     int owner, lo, hi;
     row_range(a, row, owner, lo, hi);
     owner = __builtin_amdgcn_readfirstlane(owner);
-    lo = __builtin_amdgcn_readfirstlane(from[row]);
+    if (lead > 0) {
+      const int g = max(__builtin_amdgcn_readfirstlane(last_at<4>(g_request, ng, owner, lane)), 0);
+      if (shares(g, row, owner, lo, hi)) lo = g_keys[g];
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
     W wk;
     wk.start(a, row, kh, qt, lane);
     wk.run(a, a.table + (long)owner * a.ldt, kh, lo, hi, 4 * c0, min(4 * c1, tiles_of(hi - lo, W::KT)), 1,

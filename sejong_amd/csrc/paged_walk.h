@@ -56,16 +56,20 @@ struct PagedArgs {
   int slot;     // floats of a walk's totals: 16 maxima and sums of shares, min(G, 16) rows of D
 };
 
-// the keys a row sees, [lo, hi), and its request; false for a padded row
-__device__ __forceinline__ bool row_range(const PagedArgs& a, int row, int& owner, int& lo, int& hi) {
-  const int pos = a.positions[row];
-  owner = a.owners ? a.owners[row] : row;
+// the keys that a row at position pos sees, [lo, hi); false for a padded row
+__device__ __forceinline__ bool range_of(const PagedArgs& a, int pos, int owner, int& lo, int& hi) {
   if (pos < 0 || owner < 0 || owner >= a.requests) return false;
   const long most = a.ldt * a.P;  // at most 2^31 - 1 (checked on the host)
   hi = (int)(pos + 1L < most ? pos + 1L : most);
   lo = a.window > 0 && pos + 1L > a.window ? (int)(pos + 1L - a.window) : 0;
   if (lo > hi) lo = hi;
   return true;
+}
+// those of a row, and its request
+__device__ __forceinline__ bool row_range(const PagedArgs& a, int row, int& owner, int& lo, int& hi) {
+  const int pos = a.positions[row];
+  owner = a.owners ? a.owners[row] : row;
+  return range_of(a, pos, owner, lo, hi);
 }
 
 // 16 bytes at any alignment

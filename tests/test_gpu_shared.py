@@ -72,7 +72,7 @@ def test_shared(dtype, hq, hk, D, P):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("groups,hq,hk,D,P", [([(9000, [1] * 40)], 8, 2, 64, 16), ([(5000, [300] * 5), (20, [900] * 3)], 8, 8, 128, 64),
-                                              ([(600, [2, 3])] * 60, 4, 2, 64, 24), ([(70000, [5, 9])], 2, 1, 16, 256),
+                                              ([(600, [2, 3])] * 60, 4, 2, 64, 24), ([(30, [2, 3])] * 256, 2, 2, 64, 8), ([(9, [1] * 8)] * 255, 2, 2, 32, 4), ([(70000, [5, 9])], 2, 1, 16, 256),
                                               ([(100, [4] * 300)], 16, 2, 64, 16), ([(2000, [1])], 6, 2, 64, 16),
                                               ([(17, [1, 1])] * 1000, 2, 1, 32, 16), ([(500, [3] * 3), (3, [6000])], 6, 2, 64, 16),
                                               ([(300, [20] * 70)], 8, 1, 256, 16), ([(256, [1] * 64)], 4, 4, 96, 32)])
@@ -181,7 +181,7 @@ def test_shared_in_place_and_without_lse(dtype):
 
 
 def test_shared_no_groups_and_more_than_are_walked_together():
-    """No group at all; more than 2048 rows and more than 1024 groups attend alone."""
+    """No group at all; more than 2048 rows and more than 256 groups attend alone."""
     Shared(1, "bf16", 6, 2, 64, 16, [], alone=[5, 300]).upload().run().check()
     Shared(2, "bf16", 2, 1, 32, 16, [(32, [1] * 2100)]).upload().run().check()
     Shared(3, "bf16", 2, 1, 32, 16, [(16, [1])] * 1100).upload().run().check()
