@@ -8,14 +8,26 @@
 // Totals of different beams may lie next to each other, and which is the larger
 // decides what the search goes on with: sums, totals and ranks are 64 bits.
 // Within a beam the order is that of its logits, which are exact.
+//
+// What bounds it.  A prompt's step is two dependent halves, its rows and then
+// all of its beams, and each ends with reductions of one workgroup: 64 prompts of
+// 4 beams over 257 f32 take 9.6 us, 2 of them the launch's.  Over 8 rows of
+// 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 16.9 us with the
+// meeting of their parts; a launch of its own for the second half had 8.5 + 15.2.
+// Over 384 rows of 50001 bf16 (38 MB, 7.5 us) the powers of e in 64 bits decide:
+// 14 operations of half rate an entry, 25.6 us, and 7.0 for the second half.
+#include <type_traits>
+
 #include "order.h"
 
 using namespace sj;
 
 namespace {
 
-constexpr int SLICE = 8192;   // entries of a slice
+constexpr int SLICE = 4096;   // entries of a slice where slices are few
+constexpr int NEAR = 256;     // lists whose sums and first entries LDS holds
 constexpr int CAP = 1024;     // entries at or above a threshold that LDS holds
+constexpr int MEETING = 1024; // slices of a call whose workgroups meet within the launch, at most
 
 struct BeamArgs {
   const void* x;
@@ -32,31 +44,33 @@ struct BeamArgs {
   u64* flag;  // [rows][slices], of the meetings
   u64 number;
   u64* sums;  // [rows][slices] of (maximum, sum)
-  u64* keys;  // [rows][slices][k]
+  u64* keys;  // [groups][k][beams][slices]
 };
 
-// e^d for d <= 0, to 2^-45: 2^n times a polynomial of degree 9 (least largest
-// relative error over half a step to each side, 1.6e-14).  Below -700 it is that
-// of -700, 1e-304, which no sum of 1 or more sees; NaN is NaN.
-__device__ __forceinline__ double exp_down(double d) {
+// 2^t for -1000 <= t <= 1/2, to 2^-40: 2^n times a polynomial of degree 8 (least
+// largest relative error over half a step to each side, 7.8e-13).  NaN is NaN:
+// the last 12 bits of one that was 32 bits or comes of infinities are 0.
+__device__ __forceinline__ double power2(double t) {
   const double magic = 6755399441055744.0;  // 1.5 2^52: the nearest whole number lies in the low bits
-  const double tm = fma(d, 1.4426950408889634, magic), f = fma(d, 1.4426950408889634, -(tm - magic));
-  double p = 1.0150995588009233e-07;
-  p = fma(p, f, 1.3259453829428669e-06);
-  p = fma(p, f, 1.5252982626321696e-05);
-  p = fma(p, f, 0.00015403434767100833);
-  p = fma(p, f, 0.0013333557617282988);
-  p = fma(p, f, 0.009618129192228842);
-  p = fma(p, f, 0.05550410866872767);
-  p = fma(p, f, 0.24022650695650039);
-  p = fma(p, f, 0.6931471805598701);
-  p = fma(p, f, 1.0000000000000127);
+  const double tm = t + magic, f = t - (tm - magic);
+  double p = 1.3175896059925506e-06;
+  p = fma(p, f, 1.530973869952211e-05);
+  p = fma(p, f, 0.00015403851471546215);
+  p = fma(p, f, 0.0013333452055198773);
+  p = fma(p, f, 0.009618128543494182);
+  p = fma(p, f, 0.05550410939355053);
+  p = fma(p, f, 0.2402265069887592);
+  p = fma(p, f, 0.6931471805465064);
+  p = fma(p, f, 0.9999999999997622);
   const long long b = __double_as_longlong(p);
   return __hiloint2double((int)(b >> 32) + (__double2loint(tm) << 20), (int)b);
 }
-// e^(x - ref) in 64 bits
-__device__ __forceinline__ double power_of(float x, float ref, float low) {
-  return exp_down((double)(x < low ? low : x) - (double)ref);
+constexpr double LOG2E_64 = 1.4426950408889634;
+constexpr double FAR = 690.0;  // a power of e that no sum of 1 or more sees, and that 64 bits hold
+// e^(x - ref), x - ref <= 0; below -FAR it is that of -FAR, 1e-300
+__device__ __forceinline__ double power_of(float x, float ref) {
+  const double d = (double)x - (double)ref;
+  return power2((d < -FAR ? -FAR : d) * LOG2E_64);
 }
 
 // the order of finite ranks as whole numbers above 0
@@ -102,7 +116,7 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
     if (v + E <= end) u[i].r = *(const typename U::Raw*)(x + v);
   }
   constexpr int PART = 4, PARTS = EV / PART;
-  float pm[PARTS], best = -INFINITY;
+  float pm[PARTS], best = -INFINITY, least_of = INFINITY;
   auto f = [&](int i) { return u[i / E].get(i % E); };
 #pragma unroll
   for (int i = 0; i < NU; i++) {
@@ -116,6 +130,7 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
       for (int j = i * E / PART; j < (i + 1) * E / PART; j++) {
         pm[j] = fmaxf(fmaxf(f(PART * j), f(PART * j + 1)), fmaxf(f(PART * j + 2), f(PART * j + 3)));
         best = fmaxf(best, pm[j]);
+        least_of = fminf(least_of, fminf(fminf(f(PART * j), f(PART * j + 1)), fminf(f(PART * j + 2), f(PART * j + 3))));
       }
     }
   }
@@ -143,15 +158,24 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
     const float least = all_min(larger < k ? col : INFINITY);
     if (NT == 64 ? lane == 0 : all ? lane == 0 : lane < 4) sh.T[NT == 64 ? 0 : all ? w : lane] = least;
   }
-  // -inf has no share in the sum (its power is that of -700); where there is
-  // nothing else, the sum is only asked for NaN
-  const float ref = m == -INFINITY ? 0.f : m, low = ref - 700.f;
+  // Entries too far below the maximum for power2 (a mask's) are moved up to
+  // where they still count for nothing; where there is nothing but -inf, the
+  // sum is only asked for NaN
+  const float ref = m == -INFINITY ? 0.f : m;
+  const double scaled = -(double)ref * LOG2E_64;
+  const bool far = (double)least_of - (double)ref < -FAR;
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < NU; i++)
-    if (base + E * (t + NT * i) < end)
+    if (base + E * (t + NT * i) < end) {
+      if (__any(far)) {
 #pragma unroll
-      for (int e = 0; e < E; e++) sum += power_of(f(i * E + e), ref, low);
+        for (int e = 0; e < E; e++) sum += power_of(f(i * E + e), ref);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) sum += power2(fma((double)f(i * E + e), LOG2E_64, scaled));
+      }
+    }
   sum = wave_sum(sum);
   if (NT > 64) {
     if (lane == 0) sh.sum[w] = sum;
@@ -217,14 +241,18 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
 // One workgroup takes the lists of a prompt's beams together: their sums, the
 // ranks of all entries, and the `keep` first of them, again through a threshold.
 struct GroupShared {
-  double base[64], factor[64];  // the beam's L (of an ended one its score), length^power
-  int live[64];                 // 0: no candidate, 1: its tokens, 2: ended
+  double base[64], factor[64], score[64];  // the beam's L, length^power
+  int live[64];                            // 0: no candidate, 1: its tokens, 2: ended
   u64 cand[CAP];
   int32_t where[CAP];
   double total[CAP];
-  u64 best[256], last[4];
-  int at[4];
+  __attribute__((aligned(16))) u64 best[256];
+  u64 last[4];
   int n;
+};
+// sums and entries of the lists, as many as LDS holds
+struct Near {
+  u64 sums[2 * NEAR], keys[8 * NEAR];
 };
 struct Candidate {
   u64 key;  // 0: none
@@ -233,55 +261,69 @@ struct Candidate {
 };
 
 template <bool MEET>
-__device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared& sh) {
+__device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared& sh, Near& near, bool there) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, B = a.B, S = a.slices, k = a.k, keep = a.keep;
   const long row0 = (long)g * B;
   const u64* keys = a.keys + row0 * S * k;
-  for (int b = w; b < B; b += 4) {
+  const int lists = B * S, all = lists * k;  // all lists' first entries, then their second ones
+  const u64* sums = a.sums + 2 * row0 * S;
+  auto get = [&](const u64* p) { return MEET ? part_get(p) : *p; };
+  const int near_sums = min(2 * lists, 2 * NEAR), near_keys = min(all, 8 * NEAR);
+  if (!there) {
+    for (int i = t; i < near_sums; i += 256) near.sums[i] = get(sums + i);
+#pragma unroll 4
+    for (int i = t; i < near_keys; i += 256) near.keys[i] = get(keys + i);
+  }
+  auto sum_at = [&](int i) { return i < near_sums ? near.sums[i] : get(sums + i); };
+  auto key_at = [&](int i) { return i < near_keys ? near.keys[i] : get(keys + i); };
+  if (t == 0) sh.n = 0;
+  __syncthreads();
+  // 16 lanes a beam
+  for (int b = t >> 4; b < B; b += 16) {
+    const int l = t & 15;
     const long row = row0 + b;
     const float score = a.scores[row];
     const bool ended = a.ended && a.ended[row];
-    double base = score;
-    int live = score == score && fabsf(score) < INFINITY ? 2 : 0;
+    const int len = a.lengths ? a.lengths[row] : 0;
+    float M = -INFINITY;
+    double sum = 0.0;
     if (!ended) {
-      const u64* sums = a.sums + 2 * row * S;
-      auto get = [&](const u64* p) { return MEET ? part_get(p) : *p; };
-      float M = -INFINITY;
-      for (int s = lane; s < S; s += 64) M = fmaxf(M, __uint_as_float((uint32_t)get(sums + 2 * s)));
-      M = all_max(M);
-      double sum = 0.0;
-      for (int s = lane; s < S; s += 64) {
-        const float m = __uint_as_float((uint32_t)get(sums + 2 * s));
-        const double v = __longlong_as_double((long long)get(sums + 2 * s + 1));
-        sum += v * power_of(m, M == -INFINITY ? 0.f : M, M == -INFINITY ? -700.f : M - 700.f);
+      for (int s = l; s < S; s += 16) M = fmaxf(M, __uint_as_float((uint32_t)sum_at(2 * (b * S + s))));
+#pragma unroll
+      for (int d = 8; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+#pragma unroll 1
+      for (int s = l; s < S; s += 16) {
+        const float m = __uint_as_float((uint32_t)sum_at(2 * (b * S + s)));
+        const double v = __longlong_as_double((long long)sum_at(2 * (b * S + s) + 1));
+        sum += v * power_of(m, M == -INFINITY ? 0.f : M);
       }
-      sum = wave_sum(sum);
-      base = (double)M + log(sum);
-      if (live) live = base == base && fabs(base) < INFINITY ? 1 : 0;
+#pragma unroll
+      for (int d = 8; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
     }
-    if (lane == 0) {
-      const int len = a.lengths ? a.lengths[row] : 0;
-      const long after = max(ended ? (long)len : len + 1L, 1L);
+    // one logarithm for both
+    const double after = (double)max(ended ? (long)len : len + 1L, 1L), ln = log(l == 0 ? sum : after);
+    if (l == 0) {
+      int live = score == score && fabsf(score) < INFINITY ? 2 : 0;
+      const double base = (double)M + ln;
+      if (live && !ended) live = base == base && fabs(base) < INFINITY ? 1 : 0;
       sh.base[b] = base;
+      sh.score[b] = score;
       sh.live[b] = live;
-      sh.factor[b] = a.power == 0.0 ? 1.0 : pow((double)after, a.power);
+    } else if (l == 1) {
+      sh.factor[b] = power2(a.power * ln * LOG2E_64);  // up to 2^496
     }
   }
-  if (t == 0) sh.n = 0;
   __syncthreads();
-  const int all = B * S * k;
-  auto candidate = [&](int i) {
+  auto candidate = [&](int list, int i, u64 key) {  // place i / lists of the list
     Candidate c = {0, 0, 0.0};
-    if (i >= all) return c;
-    const int b = i / (S * k), in = i - b * S * k, live = sh.live[b];
-    if (live == 1) {
-      const u64 key = MEET ? part_get(keys + i) : keys[i];
-      const float x = key_value(key);
-      if (key == 0 || x == -INFINITY) return c;
-      c.total = (double)a.scores[row0 + b] + ((double)x - sh.base[b]);
+    const int b = list / S, live = sh.live[b];
+    const double score = sh.score[b];
+    const float x = key_value(key);
+    if (live == 1 && key != 0 && x != -INFINITY) {
+      c.total = score + ((double)x - sh.base[b]);
       c.flat = b * a.V + key_index(key);
-    } else if (live == 2 && in == 0) {
-      c.total = sh.base[b];
+    } else if (live == 2 && i == b * S) {
+      c.total = score;
       c.flat = b * a.V + max(a.end_token, 0);
     } else {
       return c;
@@ -289,44 +331,50 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
     c.key = rank_key(a.power == 0.0 ? c.total : c.total / sh.factor[b]);
     return c;
   };
-  constexpr int HELD = 4;
-  Candidate c[HELD];
+  // Each list is in order: `each` threads go down every each-th entry of it, and
+  // stop at the first below the threshold.
+  const int each = max(256 / lists, 1), step = each * lists, from = t / lists * lists;
+  const int list0 = t < step || each == 1 ? t - from : lists;
   u64 best = 0;
-#pragma unroll
-  for (int i = 0; i < HELD; i++) {
-    c[i] = candidate(t + 256 * i);
-    best = larger_of(best, c[i].key);
-  }
-  for (int i = t + 256 * HELD; i < all; i += 256) best = larger_of(best, candidate(i).key);
+#pragma unroll 1
+  for (int list = list0; list < lists; list += 256)
+    if (from + list < all) best = larger_of(best, candidate(list, from + list, key_at(from + list)).key);
+  // the threshold: the keep-th largest of 64 columns' largest, 1 where fewer
+  // columns have any
   sh.best[t] = best;
   __syncthreads();
-  // the threshold: the keep-th largest of the threads' largest, 1 where fewer
-  // have any
-  int larger = 0;
-  for (int i = 0; i < 256; i++) larger += sh.best[i] > best;
-  u64 least = larger < keep && best ? best : ~0ull;
-  int have = __syncthreads_count(best != 0);
+  if (w == 0) {
+    const u64 col = larger_of(larger_of(best, sh.best[lane + 64]), larger_of(sh.best[lane + 128], sh.best[lane + 192]));
+    sync_wave();
+    sh.best[lane] = col;
+    sync_wave();
+    int larger = 0;
+#pragma unroll 4
+    for (int i = 0; i < 64; i += 2) {
+      const ulonglong2 q = *(const ulonglong2*)(sh.best + i);
+      larger += (q.x > col) + (q.y > col);
+    }
+    // equal columns have one place: the least of those with fewer than keep larger ones
+    u64 least = col && larger < keep ? col : ~0ull;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const u64 o = __shfl_xor(least, d, 64);
-    least = o < least ? o : least;
+    for (int d = 32; d; d >>= 1) {
+      const u64 o = __shfl_xor(least, d, 64);
+      least = o < least ? o : least;
+    }
+    const bool enough = __popcll(__ballot(col != 0)) >= keep;
+    if (lane == 0) sh.last[0] = enough ? least : 1;
   }
-  if (lane == 0) sh.last[w] = least;
   __syncthreads();
-  u64 T0 = 1;
-  if (have >= keep) {
-    T0 = sh.last[0];
-    for (int i = 1; i < 4; i++) T0 = sh.last[i] < T0 ? sh.last[i] : T0;
-  }
-  auto collect = [&](const Candidate& q) {
-    if (q.key >= T0) {
+  const u64 T0 = sh.last[0];
+#pragma unroll 1
+  for (int list = list0; list < lists; list += 256)
+#pragma unroll 1
+    for (int i = from + list; i < all; i += step) {
+      const Candidate q = candidate(list, i, key_at(i));
+      if (q.key < T0) break;
       const int n = atomicAdd(&sh.n, 1);
       if (n < CAP) sh.cand[n] = q.key, sh.where[n] = q.flat, sh.total[n] = q.total;
     }
-  };
-#pragma unroll
-  for (int i = 0; i < HELD; i++) collect(c[i]);
-  for (int i = t + 256 * HELD; i < all; i += 256) collect(candidate(i));
   __syncthreads();
   auto write = [&](int place, bool some, int flat, double total) {
     const long at = (long)g * keep + place;
@@ -359,7 +407,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   for (int j = 0; j < keep; j++) {
     Candidate top = {0, 0x7fffffff, 0.0};
     for (int i = t; i < all; i += 256) {
-      const Candidate q = candidate(i);
+      const Candidate q = candidate(i % lists, i, key_at(i));
       const bool behind = q.key && (q.key < last || (q.key == last && q.flat > last_flat));
       if (behind && (q.key > top.key || (q.key == top.key && q.flat < top.flat))) top = q;
     }
@@ -382,29 +430,67 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   }
 }
 
-template <typename T, int NT, int EV, int E = WIDE<T>>
+// One wave per row (NT = 64: a workgroup has four rows of a prompt) or one
+// workgroup per slice.  MEET: the last of a prompt's workgroups takes its beams
+// together.
+template <typename T, int NT, int EV, int E = WIDE<T>, bool MEET = false>
 __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
-  __shared__ RowShared<NT, EV> sh[256 / NT];
-  const int gt = threadIdx.x / NT, item = blockIdx.x * (256 / NT) + gt;
-  const long row = NT == 64 ? item : item / a.slices;
-  if (row >= (long)a.groups * a.B) return;
-  const int slice = NT == 64 ? 0 : item - (int)row * a.slices;
-  if (a.ended && a.ended[row]) return;
-  const int base = slice * a.width, end = min(a.V, base + a.width);
-  float m;
-  double sum;
-  u64* list = a.keys + (row * a.slices + slice) * a.k;
-  row_best<T, NT, EV, E>((const T*)a.x + row * a.ldx, base, end, a.k, sh[gt], m, sum,
-                         [&](int place, u64 key) { list[place] = key; });
-  if (threadIdx.x % NT == 0) {
-    u64* p = a.sums + 2 * (row * a.slices + slice);
-    p[0] = __float_as_uint(m);
-    p[1] = (u64)__double_as_longlong(sum);
+  __shared__ union {
+    RowShared<NT, EV> row[256 / NT];
+    std::conditional_t<MEET, GroupShared, int> group;
+  } sh;
+  __shared__ std::conditional_t<MEET, Near, int> near;
+  const int gt = threadIdx.x / NT;
+  // the prompt's parts, and the row and slice of this one
+  const int parts = NT == 64 ? (a.B + 3) / 4 : a.B * a.slices, g = blockIdx.x / parts, part = blockIdx.x - g * parts;
+  const int beam = NT == 64 ? 4 * part + gt : part / a.slices, slice = NT == 64 ? 0 : part - beam * a.slices;
+  const long row = (long)g * a.B + beam;
+  const bool there = MEET && NT == 64 && parts == 1;  // the lists go from LDS to LDS
+  if (beam < a.B && !(a.ended && a.ended[row])) {
+    const int base = slice * a.width, end = min(a.V, base + a.width);
+    float m;
+    double sum;
+    const int lists = a.B * a.slices;
+    u64* list = a.keys + (long)g * lists * a.k + beam * a.slices + slice;
+    row_best<T, NT, EV, E>((const T*)a.x + row * a.ldx, base, end, a.k, sh.row[gt], m, sum, [&](int place, u64 key) {
+      if constexpr (MEET) {
+        if (there)  // slice 0 is all
+          near.keys[place * lists + beam] = key;
+        else
+          part_put(list + (long)place * lists, key);
+      } else {
+        list[(long)place * lists] = key;
+      }
+    });
+    if (threadIdx.x % NT == 0) {
+      u64* p = a.sums + 2 * (row * a.slices + slice);
+      if constexpr (MEET) {
+        const u64 own[2] = {(u64)__float_as_uint(m), (u64)__double_as_longlong(sum)};
+        for (int i = 0; i < 2; i++)
+          if (there)
+            near.sums[2 * beam + i] = own[i];
+          else
+            part_put(p + i, own[i]);
+      } else {
+        p[0] = __float_as_uint(m);
+        p[1] = (u64)__double_as_longlong(sum);
+      }
+    }
+  }
+  if constexpr (MEET) {
+    __shared__ int complete;
+    u64* flags = a.flag + (long)g * a.B * a.slices;
+    if (there)
+      __syncthreads();
+    else if (!meet([&](int i) { return flags + i; }, part, parts, a.number, &complete))
+      return;
+    group_best<true>(a, g, sh.group, near, there);
   }
 }
 __global__ __launch_bounds__(256) void k_beam_join(BeamArgs a) {
   __shared__ GroupShared sh;
-  group_best<false>(a, blockIdx.x, sh);
+  __shared__ Near near;
+  group_best<false>(a, blockIdx.x, sh, near, false);
 }
 
 long slices_of(long vocab) { return (vocab + SLICE - 1) / SLICE; }
@@ -414,18 +500,27 @@ void launch_select(hipStream_t s, BeamArgs& a) {
   const long rows = (long)a.groups * a.B;
   a.slices = 1;
   a.width = (a.V + 7) / 8 * 8;
-  if (a.V <= 512) {
-    k_beam_rows<T, 64, 8, 4><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
-  } else if (a.V <= 1024) {
-    k_beam_rows<T, 64, 16><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
-  } else if (a.V <= 4096) {
-    k_beam_rows<T, 256, 16><<<(unsigned)rows, 256, 0, s>>>(a);
+  a.number = sjh::call_number();
+  if (a.V <= 1024) {
+    const unsigned blocks = (unsigned)(a.groups * ((a.B + 3) / 4));
+    if (a.V <= 512)
+      k_beam_rows<T, 64, 8, 4, true><<<blocks, 256, 0, s>>>(a);
+    else
+      k_beam_rows<T, 64, 16, WIDE<T>, true><<<blocks, 256, 0, s>>>(a);
   } else {
-    a.slices = (int)slices_of(a.V);
+    const bool meets = a.V <= SLICE || rows * slices_of(a.V) <= MEETING;
+    constexpr int LONG = sizeof(T) == 2 ? 64 : 32;  // entries a thread holds where slices are many
+    const int most = meets ? SLICE : 256 * LONG;
+    a.slices = (a.V + most - 1) / most;
     a.width = ((a.V + a.slices - 1) / a.slices + 7) / 8 * 8;
-    k_beam_rows<T, 256, 32><<<(unsigned)(rows * a.slices), 256, 0, s>>>(a);
+    const unsigned blocks = (unsigned)(rows * a.slices);
+    if (meets) {
+      k_beam_rows<T, 256, 16, WIDE<T>, true><<<blocks, 256, 0, s>>>(a);
+    } else {
+      k_beam_rows<T, 256, LONG><<<blocks, 256, 0, s>>>(a);
+      k_beam_join<<<(unsigned)a.groups, 256, 0, s>>>(a);
+    }
   }
-  k_beam_join<<<(unsigned)a.groups, 256, 0, s>>>(a);
 }
 
 }  // namespace
