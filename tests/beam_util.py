@@ -80,10 +80,9 @@ def fork(parents, table, lengths, P, pages, shared, free, head):
         return dict(void, status=NO_PAGES)
     out["shared"] = shared + change
     head += taken
-    back = [p for p in range(pages) if out["shared"][p] < 0]
-    for p in back[:head]:
-        head_at = head - 1 - back.index(p)
-        out["free"][head_at], out["shared"][p] = p, 0
+    back = np.flatnonzero(out["shared"] < 0).tolist()
+    for i, p in enumerate(back[:head]):
+        out["free"][head - 1 - i], out["shared"][p] = p, 0
     given = min(len(back), head)
     return dict(out, status=LIST_FULL if given < len(back) else 0, taken=taken, head=head - given, back=given)
 
@@ -91,7 +90,8 @@ def fork(parents, table, lengths, P, pages, shared, free, head):
 def compact(table, lengths, P, pages, after, shared, free, head, capacity):
     rest = [int(p) for p in free[max(head, 0):]]
     below = [p for p in rest if 0 <= p < after]
-    moves = [p for p in range(after, pages) if p not in set(rest)]
+    known = set(rest)
+    moves = [p for p in range(after, pages) if p not in known]
     status = NO_PAGES * (head < 0 or head > len(free) or len(moves) > len(below)) | ROWS * (len(moves) > capacity)
     copies = np.tile([-1, -1, 0], (capacity, 1))
     if status:

@@ -243,6 +243,47 @@ def test_void_compactions(status, change):
     assert c.check()["status"] == status
 
 
+@pytest.mark.parametrize("status,change", [(1, "small"), (1, "far"), (4, "capacity"), (5, "both")])
+def test_void_compactions_of_many_workgroups(status, change):
+    rng = np.random.default_rng(15)
+    lengths, table, shared, free, head, pages = state(rng, 60, 2, 8, 2000, 30000)
+    used = pages - (len(free) - head)
+    after = used - 1 if change in ("small", "both") else used + 20
+    head = len(free) + 1 if change == "far" else head
+    c = Compact(lengths, table, shared, free, head, pages, 8, after, 2 if change in ("capacity", "both") else None).run()
+    assert c.check()["status"] == status
+
+
+@pytest.mark.parametrize("pages,rounds", [(16384, 0), (16385, 1), (5_000_003, 2)])
+def test_pools_of_one_workgroup_and_of_rounds(pages, rounds):
+    """Pages of which one workgroup holds all, one more, and so many that a workgroup takes several rounds."""
+    rng = np.random.default_rng(pages)
+    R, P, cols = 40, 4, 60
+    names = rng.permutation(pages)
+    table, lengths = names[:R * cols].reshape(R, cols), np.full(R, P * cols)
+    free = np.concatenate([np.full(R * cols, -1), names[R * cols:]])
+    shared = np.zeros(pages, int)
+    want = Fork(np.arange(0, R, 2), lengths, table, shared, free, R * cols, pages, P).run().check()
+    assert want["status"] == 0 and want["back"] == R * cols // 2
+    want = Compact(lengths, table, shared, free, R * cols, pages, P, pages // 3).run().check()
+    assert want["status"] == 0 and want["moves"] > R * cols // 2
+    want = Compact(lengths, table, shared, free, R * cols, pages, P, 100).run().check()
+    assert want["status"] == 1
+
+
+def test_compact_replays_of_many_workgroups():
+    rng = np.random.default_rng(19)
+    st = state(rng, 30, 4, 16, 900, 40000)
+    c = Compact(st[0], st[1], st[2], st[3], st[4], st[5], 16, st[5] - 30000)
+    g = PU.Graph(c.run)
+    for _ in range(3):
+        for b in c.outs.values():
+            b.upload(np.full(b.n, 55))
+        g.replay()
+        c.check()
+    g.close()
+
+
 def test_compact_empty_and_bad_entries():
     rng = np.random.default_rng(8)
     lengths, table, shared, free, head, pages = state(rng, 4, 2, 8, 100, 60, lo=20)
