@@ -24,6 +24,15 @@ namespace {
 // nobody to join with).  So few long prefixes and many short tails fill the chip
 // alike.  What was summed of a walk goes to the workspace; a second launch joins
 // the parts of each row's two walks.
+//
+// 4 rows over 960 shared keys (6/2 heads of 64, bf16) take 14.6 us: 1.6 to launch,
+// 3.3 for the lists, a walk's chain of page, keys and products, 4.5 for the join.
+// 24 groups of 5 rows over up to 6000 keys (16/4 heads of 64, fp32) take 36.5 us,
+// 12 of them their 61 MB at a copy's rate: each wave waits for two or three tiles.
+// 64 rows over 16384 keys (32/8 heads of 128, bf16) take 56 us, where their 91 MB
+// are 18 and their products, P as two planes, 18: the lists 3, the shared walks
+// 37 (the multiplying waves' own instructions 21), own walks 6, the join of 34 MB
+// of parts 10.  One plane (54 us) would round P to 8 bits.
 
 constexpr int CT = 2, COLS = 16 * CT, BLOCK = 4 * COLS;
 constexpr int WIDE_PLACE = 64;  // keys of a place of a walk whose waves go by columns
@@ -450,12 +459,21 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
     }
     __syncthreads();
   }
-  // where there are workgroups enough, some take shared walks and the others own
-  // ones, else all of them both
+  // Every workgroup takes both, its shared places and then its waves' own ones,
+  // or some take the ones and the others the others, whichever leaves the longest
+  // with fewer places (24 groups of 5 fp32 rows: 39 us, apart 36; 48 groups 58 and
+  // 50).  Where that is the same, few places and many own walks are better apart
+  // (24 groups with up to 1000 own keys a row 44 and 37), else not (100 groups 93
+  // and 109; 8 rows over 16384 keys 40 and 43).
   const int own = pre[a.rows] * nb, all = gridDim.x;
-  const bool apart = (long)lead + (own + 3) / 4 <= all;
-  const int own_groups = apart ? all - lead : all, waves = 4 * max(own_groups, 1);
-  const int piece = max(1, (int)(((long)lead + all - 1) / all)), own_piece = max(1, (int)(((long)own + waves - 1) / waves));
+  auto each = [](long n, long of) { return (int)((n + of - 1) / of); };
+  const int lead_each = each(lead, all), mixed = max(1, each((long)lead + each(own, 4), all));
+  const int sum = lead_each + each(own, 4L * all);
+  const bool fewer = mixed < sum || (mixed == sum && mixed <= 3 && 2 * (long)own >= all);
+  const bool apart = fewer && (own == 0 || each(lead, mixed) < all);
+  const int piece = max(1, apart ? mixed : lead_each);
+  const int taken = apart ? each(lead, piece) : 0, own_groups = max(all - taken, 1), waves = 4 * own_groups;
+  const int own_piece = max(1, each(own, waves));
   if (blockIdx.x == 0) {
     for (int g = t; g < ng; g += 256) {
       const Group r = group_of(g);
@@ -464,9 +482,6 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
     }
     if (t == 0) *s.line = make_int2(piece, own_piece);
   }
-  // Neighbours on the line on different XCDs: a KV head's rows lie in a few of an
-  // L2's channels (64 rows over 16384 keys, 8 heads of 128, a head to an XCD: 49
-  // us, its loads at 3.6 TB/s whatever else it does)
   const int b = blockIdx.x;
   int x = (int)min((long)lead, (long)b * piece);
   const int e = (int)min((long)lead, (long)x + piece);
@@ -551,7 +566,7 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
   }
   __syncthreads();  // the waves' tiles lie elsewhere in the rows' own walks
   // a wave's piece; those of one workgroup lie apart, so that few walks go over all workgroups
-  const int mine = apart ? (int)blockIdx.x - lead : (int)blockIdx.x;
+  const int mine = (int)blockIdx.x - taken;
   if (mine < 0) return;
   const int wave = w * own_groups + mine;
   int y = (int)min((long)own, (long)wave * own_piece);

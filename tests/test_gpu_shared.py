@@ -80,6 +80,14 @@ def test_shared_long_and_many(dtype, groups, hq, hk, D, P):
     Shared(len(groups) + D, dtype, hq, hk, D, P, groups).upload().run().check()
 
 
+@pytest.mark.parametrize("rows", [1, 3, 9])
+@pytest.mark.parametrize("places", [509, 511, 512, 1021, 1023, 1024])
+def test_shared_and_own_walks_of_just_so_many_workgroups(places, rows):
+    """As many places of 128 keys as leave few workgroups, one or none for the rows' own keys: the parts of those that
+    nobody took would be what lies in the workspace, NaN."""
+    Shared(places + rows, "f32", 1, 1, 64, 256, [(128 * places, [1] * rows)]).upload().run().check()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_shared_several_tokens_a_request(dtype):
     """Drafted tokens: those that do not see the whole prefix attend alone."""
