@@ -334,7 +334,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   // Each list is in order: `each` threads go down every each-th entry of it, and
   // stop at the first below the threshold.
   const int each = max(256 / lists, 1), step = each * lists, from = t / lists * lists;
-  const int list0 = t < step || each == 1 ? t - from : lists;
+  const int list0 = t < step ? t - from : lists;
   u64 best = 0;
 #pragma unroll 1
   for (int list = list0; list < lists; list += 256)

@@ -66,8 +66,10 @@ class Select:
         s, w = s[:-1], want["scores"]
         none = w == -np.inf
         assert (s[none] == -np.inf).all()
-        # totals of 64 bits, the sum's powers to 2^-45: one rounding to fp32
-        assert (np.abs(s[~none] - w[~none]) <= np.abs(w[~none]) * 2.0 ** -24 * 1.001 + 1e-12).all()
+        # totals of 64 bits, the sum's powers to 7.8e-13: one rounding to fp32; and one of the logarithm on each side,
+        # which has the size of its row's largest logit
+        large = np.abs(np.nan_to_num(self.x.max(1), nan=0.0, neginf=0.0))[want["parents"][~none]]
+        assert (np.abs(s[~none] - w[~none]) <= np.abs(w[~none]) * 2.0 ** -24 * 1.001 + 1e-12 + large * 2.0 ** -52).all()
         return want
 
 
@@ -93,6 +95,14 @@ def test_select(dtype, V, groups, beams, keep):
     s.clear()
     s.run()
     assert all((a == b.host()).all() for a, b in zip(first, s.ints + [s.out]))  # every output again, the same bits
+
+
+@pytest.mark.parametrize("beams,slices", [(1, 1), (5, 1), (31, 2), (63, 2), (64, 2), (43, 3), (17, 11), (51, 5), (64, 4), (37, 7)])
+def test_select_lists_of_any_number(beams, slices):
+    """As many lists as threads of the workgroup that takes them together, half as many, a few more, a few less."""
+    rng = np.random.default_rng(beams)
+    x = logits(rng, beams, 4096 * slices - 5, "f32")
+    Select(x, rng.normal(-20, 2, beams), beams, 11, "f32", lengths=np.full(beams, 3)).run().check()
 
 
 @pytest.mark.parametrize("V", [5, 257, 3000, 9000])
@@ -122,6 +132,17 @@ def test_select_first_step(dtype, V):
     s = Select(logits(rng, 20, V, dtype), scores.ravel(), 5, 5, dtype).run()
     want = s.check()
     assert (want["parents"][:15].reshape(3, 5) == np.arange(3)[:, None] * 5).all() and (want["parents"][15:] == -1).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [300, 900, 5000, 200000])
+@pytest.mark.parametrize("size", [3e2, 1e6, 2.0 ** 33, 1e30])
+def test_select_large_logits(dtype, V, size):
+    """Differences past every power's range, at sizes where fp32 cannot hold the maximum less a few hundred."""
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 1, (8, V)) * size
+    x[:, 7] = x[:, 11] = np.abs(x).max(1)  # two tokens have all of the row
+    Select(G.O.round_to(x, dtype), rng.normal(-8, 3, 8), 4, 7, dtype, lengths=np.full(8, 5)).run().check()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
