@@ -23,6 +23,7 @@ Chunks chunks_of(long n) {
   return {rounds * ROUND, (n + rounds * ROUND - 1) / (rounds * ROUND)};
 }
 constexpr int ALONE = 16384;  // entries, at most, that one workgroup takes by itself: 16 a thread
+constexpr int COMPACT_ALONE = 8192;  // of a compaction (8192 pages 13.8 us, 16.6 in five launches; 16384 18.9 and 16.8)
 
 struct __attribute__((packed, aligned(4))) Int4 {
   u32x4 v;
@@ -77,6 +78,44 @@ __device__ __forceinline__ int block_scan(int v, int* ws, int& before) {
   }
   return all;
 }
+// One workgroup's entries: rounds of four consecutive ones a thread, so that
+// neighbouring lanes lie next to each other (16 consecutive ones a thread, each a
+// store of its own, took 6 us more for 16384 entries).
+template <int N>
+__device__ __forceinline__ void entries_alone(const int32_t* x, long n, int fill, int32_t (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N / 4; j++) {
+    int32_t u[4];
+    entries(x, 4096 * j + 4 * threadIdx.x, n, fill, u);
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[4 * j + k] = u[k];
+  }
+}
+// of 4 R flags a thread in that order: those before each of its rounds; all
+template <int R>
+__device__ __forceinline__ int ranks_alone(uint32_t flags, int* ws, int (&before)[R]) {
+  int base = 0;
+#pragma unroll
+  for (int h = 0; h < R / 2; h++) {  // two rounds' counts in one word: neither passes 4096
+    const uint32_t f = flags >> (8 * h);
+    int at;
+    const int all = block_scan<1024>(__popc(f & 15u) | (__popc(f & 240u) << 16), ws, at);
+    before[2 * h] = base + (at & 0xffff);
+    before[2 * h + 1] = base + (all & 0xffff) + (at >> 16);
+    base += (all & 0xffff) + (all >> 16);
+  }
+  return base;
+}
+// four entries from i0 on, as far as there are n
+__device__ __forceinline__ void put_entries(int32_t* y, long i0, long n, const int32_t (&v)[4]) {
+  if (i0 + 4 <= n) {
+    ((Int4*)(y + i0))->v = u32x4{(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (i0 + k < n) y[i0 + k] = v[k];
+  }
+}
 // the first n of the workgroups' counts
 template <int N>
 __device__ __forceinline__ int sum_counts(const int32_t* counts, long n, int* ws) {
@@ -95,11 +134,10 @@ __device__ __forceinline__ int sum_counts(const int32_t* counts, long n, int* ws
 // between them (integers: the order does not matter): children and copies;
 // tables and holders; the pages to free, by their number.
 //
-// Launches and the loads that wait for each other bound it, not bytes: 64
-// requests take 10.8 us (2.7 + 4.3 + 3.8), a pool of 170000 pages with 2000
-// requests 20.3 us (5.5 + 9.0 + 2.5 + 3.4; its 8 MB are 2 us at a copy's rate).
-// Sixteen entries a thread by loads of 4 bytes, on the few workgroups that this
-// leaves, took 9.0 + 12.1 for the last two.
+// Launches and the loads that wait for each other bound it, not bytes: a pool of
+// 162233 pages with 2000 requests takes 19.7 us (5.4 + 8.8 + 2.0 + 3.4; its 6 MB
+// are 1.2 us at a copy's rate).  Sixteen entries a thread by loads of 4 bytes, on
+// the few workgroups that this leaves, took 9.0 + 12.1 for the last two.
 
 constexpr int FORK_ROWS = 16384;  // requests, at most: the children are counted in LDS
 
@@ -267,18 +305,129 @@ __global__ __launch_bounds__(NT_) void k_fork_free(ForkArgs a) {
   }
 }
 
+// The same in one launch, where one workgroup can hold the holders (ALONE pages
+// and list entries) and go over the rows (SMALL_CELLS entries of tables): a
+// workgroup for each row after, which finds its place in the list by itself, and
+// one for the pool.  16 to 128 requests take 7.9 to 9.0 us, in three launches 11.2
+// to 12.2; 256 take 12.7 and 11.9.
+constexpr long SMALL_CELLS = 32768;
+constexpr int SMALL_REQUESTS = 192;
+__global__ __launch_bounds__(1024) void k_fork_small(ForkArgs a) {
+  constexpr int N = ALONE / 1024, MANY = 4;
+  extern __shared__ __attribute__((aligned(16))) int holders[];  // [ALONE]
+  __shared__ int count[1024], first[1024], len[1024], ws[16], wrong, mine[2];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, i = blockIdx.x;
+  const bool pool = i == a.requests;
+  const int head = a.head ? a.head[0] : 0;
+  // this workgroup's row and its pages before, asked for early
+  const int r = pool ? -1 : a.parents[i], m = r >= 0 && r < a.before ? a.lengths[r] : 0;
+  const int rows_full = bad_length(m, a.ldt, a.P) ? 0 : div(m, a.d_page), cols = rows_full + (rows_full * a.P < m);
+  const int32_t* row = a.table + (long)r * a.ldt;
+  int32_t v[N];
+  if (pool) {
+    entries_alone(a.shared, a.pages, 0, v);
+    copy_ints(a.free_after, a.free_pages, a.nfree, t, 1024);
+  }
+  const int p = t < a.requests ? a.parents[t] : -1, n = t < a.before ? a.lengths[t] : 0;
+  count[t] = 0;
+  first[t] = a.requests;
+  len[t] = n;
+  if (t == 0) wrong = 0;
+  __syncthreads();
+  if (p >= 0 && p < a.before) {
+    atomicAdd(&count[p], 1);
+    atomicMin(&first[p], t);
+  }
+  if (p >= a.before || bad_length(n, a.ldt, a.P)) wrong = 1;
+  const int cell = t < cols ? row[t] : -1;
+  __syncthreads();
+  const bool bad = wrong;
+  bool alone = true, takes = false;
+  if (!bad && p >= 0 && open_page(a, p, len[p], alone) >= 0) takes = first[p] != t || !alone;
+  int place;
+  const int taken = block_scan<1024>(takes, ws, place);
+  int status = bad ? SJ_PLAN_LENGTHS : 0;
+  if (head < 0 || (long)head + taken > a.nfree) status |= SJ_PLAN_NO_PAGES;
+  if (!pool) {
+    if (t == i) mine[0] = takes, mine[1] = place;
+    __syncthreads();
+    const bool good = !status && r >= 0, own = good && mine[0];
+    const int fresh = own ? a.free_pages[head + mine[1]] : -1;
+    for (long c = t; c < a.ldt; c += 1024) {
+      int page = -1;
+      if (good && c < cols) page = own && c == rows_full ? fresh : c == t ? cell : row[c];
+      a.table_after[i * a.ldt + c] = page;
+    }
+    if (t == 0) {
+      a.lengths_after[i] = good ? m : 0;
+      a.copies[3 * i] = own ? row[rows_full] : -1;
+      a.copies[3 * i + 1] = fresh;
+      a.copies[3 * i + 2] = own ? m - rows_full * a.P : 0;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < N; k += 4) *(u32x4*)(holders + 1024 * k + 4 * t) = *(const u32x4*)(v + k);
+  const int last = !status && t < a.before ? open_page(a, t, n, alone) : -1;
+  __syncthreads();
+  if (last >= 0 && (count[t] == 0 || !alone)) atomicAdd(&holders[last], -1);
+  // a row's full pages by a wave, MANY rows at once
+  for (int r0 = w; !status && r0 < a.before; r0 += 16 * MANY) {
+    int full[MANY], most = 0;
+#pragma unroll
+    for (int k = 0; k < MANY; k++) {
+      const int q = r0 + 16 * k;
+      full[k] = q < a.before && count[q] != 1 ? div(len[q], a.d_page) : 0;
+      most = max(most, full[k]);
+    }
+    for (int c = lane; c < most; c += 64) {
+      int page[MANY];
+#pragma unroll
+      for (int k = 0; k < MANY; k++) page[k] = c < full[k] ? a.table[(r0 + 16 * k) * a.ldt + c] : -1;
+#pragma unroll
+      for (int k = 0; k < MANY; k++)
+        if (page[k] >= 0 && page[k] < a.pages) atomicAdd(&holders[page[k]], count[r0 + 16 * k] - 1);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; k += 4) *(u32x4*)(v + k) = *(const u32x4*)(holders + 1024 * k + 4 * t);
+  const uint32_t back = status ? 0 : flags_of(v, [](int h, int) { return h < 0; });
+  int before[4];
+  const int all = ranks_alone(back, ws, before), from = status ? 0 : head + taken, given = min(all, from);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    int32_t u[4];
+    int at = from - 1 - before[j];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const bool goes = (back >> (4 * j + k)) & 1, room = goes && at >= 0;
+      if (room) a.free_after[at] = 4096 * j + 4 * t + k;
+      at -= goes;
+      u[k] = room ? 0 : v[4 * j + k];
+    }
+    put_entries(a.shared_after, 4096 * j + 4 * t, a.pages, u);
+  }
+  if (t == 0) {
+    a.summary[0] = status ? 0 : taken;
+    a.summary[1] = status ? head : from - given;
+    a.summary[2] = status ? status : given < all ? SJ_FORK_LIST_FULL : 0;
+    a.summary[3] = given;
+  }
+}
+
 // ---------------------------------------------------------------- compact
 //
 // The pages of number `after` and more that are not on the free list move, in
 // ascending order, into the free pages below, in the list's order.  Which pages
-// are free is only on the list.  Where one workgroup can hold all of it (ALONE)
-// it does; else each launch waits for the one before: marks on all high pages;
+// are free is only on the list.  Where one workgroup can hold all of it
+// (COMPACT_ALONE) it does; else each launch waits for the one before: marks on all high pages;
 // the list takes its own off, and counts its low pages; they are put in a row,
 // the moving pages counted; moves.  The tables are a launch of their own.
 //
-// 2048 pages to half take 9.8 us (7.3 + 2.5; the five launches took 23.4), 400001
-// pages to three quarters 20.8 us (2.9 + 3.5 + 3.3 + 6.6 + 4.6; 78 us with 16
-// entries a thread): again launches, and the moves' scattered writes.
+// 2048 pages to half take 8.9 us (5.2 + 2.7; five launches 16.6), 400001 pages to
+// three quarters 19.7 us (2.9 + 3.4 + 3.5 + 6.8 + 4.7; 78 us with 16 entries a
+// thread): again launches, and the moves' scattered writes.
 
 struct CompactArgs {
   const int32_t *table, *lengths, *shared, *free_pages, *head;
@@ -314,29 +463,29 @@ __device__ __forceinline__ int list_after(const CompactArgs& a, long i, const I*
 __device__ __forceinline__ void no_copies(const CompactArgs& a, int moves, long at, long step) {
   for (long i = 3L * moves + at; i < 3 * a.capacity; i += step) a.copies[i] = i % 3 == 2 ? 0 : -1;
 }
-// a thread's high pages i0 .. i0 + N - 1; flags: those that move, the first to target `at`
-template <int N, typename I>
+// a thread's high pages i0 .. i0 + 3; flags: those that move, the first to target `at`
+template <typename I>
 __device__ __forceinline__ void move_pages(const CompactArgs& a, long i0, uint32_t moving, const I* targets, int at,
                                            int status) {
-  if (a.after + i0 >= a.pages) return;
-  int32_t v[N];
-  entries(a.shared + a.after, i0, a.pages - a.after, 0, v);
+  const long high = a.pages - a.after;
+  if (i0 >= high) return;
+  int32_t v[PER], to[PER];
+  entries(a.shared + a.after, i0, high, 0, v);
 #pragma unroll
-  for (int k = 0; k < N; k++) {
-    const long i = i0 + k, p = a.after + i;
-    if (p >= a.pages) continue;
-    int to = -1;
+  for (int k = 0; k < PER; k++) {
+    to[k] = -1;
     if (!status && (moving >> k) & 1) {
-      to = (int)targets[at];
-      a.shared_after[to] = v[k];
-      a.copies[3L * at] = (int32_t)p;
-      a.copies[3L * at + 1] = to;
+      to[k] = (int)targets[at];
+      a.shared_after[to[k]] = v[k];
+      a.copies[3L * at] = (int32_t)(a.after + i0 + k);
+      a.copies[3L * at + 1] = to[k];
       a.copies[3L * at + 2] = a.P;
       at++;
     }
-    a.shared_after[p] = status ? v[k] : 0;
-    a.to[i] = to;
+    if (!status) v[k] = 0;
   }
+  put_entries(a.shared_after + a.after, i0, high, v);
+  put_entries(a.to, i0, high, to);
 }
 
 __global__ __launch_bounds__(NT) void k_compact_marks(CompactArgs a) {
@@ -410,49 +559,48 @@ __global__ __launch_bounds__(NT) void k_compact_moves(CompactArgs a) {
     entries(a.to, i0, high, 0, v);
     const uint32_t moving = flags_of(v, [](int mark, int) { return mark == 1; });
     const int some = block_scan<NT>(__popc(moving), ws, before);
-    move_pages<PER>(a, i0, moving, a.targets, base + before, status);
+    move_pages(a, i0, moving, a.targets, base + before, status);
     base += some;
   }
 }
-// pages and list of ALONE entries at most
+// pages and list of COMPACT_ALONE entries at most
 __global__ __launch_bounds__(1024) void k_compact_alone(CompactArgs a) {
-  constexpr int N = ALONE / 1024;
-  __shared__ uint32_t listed[ALONE / 32];  // bit i: high page i is on the list
-  __shared__ uint16_t targets[ALONE];
+  constexpr int N = COMPACT_ALONE / 1024;
+  __shared__ uint32_t listed[COMPACT_ALONE / 32];  // bit i: high page i is on the list
+  __shared__ uint16_t targets[COMPACT_ALONE];
   __shared__ int ws[16];
-  const int t = threadIdx.x, i0 = N * t;
+  const int t = threadIdx.x;
   const long head = head_of(a), high = a.pages - a.after;
   int32_t v[N];
-  entries(a.free_pages, i0, a.nfree, -1, v);
+  entries_alone(a.free_pages, a.nfree, -1, v);
   copy_ints(a.shared_after, a.shared, a.after, t, 1024);
-  if (t < ALONE / 32) listed[t] = 0;
+  if (t < COMPACT_ALONE / 32) listed[t] = 0;
   __syncthreads();
-  uint32_t low = 0;
-#pragma unroll
-  for (int k = 0; k < N; k++) {
-    const int p = v[k];
-    if (i0 + k < head || p < 0 || p >= a.pages) continue;
-    if (p < a.after)
-      low |= 1u << k;
-    else
-      atomicOr(&listed[(p - a.after) >> 5], 1u << ((p - a.after) & 31));
-  }
-  int before;
-  const int below = block_scan<1024>(__popc(low), ws, before);
+  const uint32_t low = flags_of(v, [&](int p, int k) {
+    if (4096 * (k >> 2) + 4 * t + (k & 3) < head || p < 0 || p >= a.pages) return false;
+    if (p >= a.after) atomicOr(&listed[(p - a.after) >> 5], 1u << ((p - a.after) & 31));
+    return p < a.after;
+  });
+  int before[N / 4];
+  const int below = ranks_alone(low, ws, before);
 #pragma unroll
   for (int k = 0; k < N; k++)
-    if ((low >> k) & 1) targets[before++] = (uint16_t)v[k];
+    if ((low >> k) & 1) targets[before[k >> 2]++] = (uint16_t)v[k];
   // the scan's barriers are behind all marks, and before all targets are read
-  uint32_t moving = ~(listed[t >> 1] >> (16 * (t & 1))) & 0xffffu;
-  const long mine = high - i0;
-  moving = mine <= 0 ? 0 : mine < N ? moving & ((1u << mine) - 1) : moving;
-  const int moves = block_scan<1024>(__popc(moving), ws, before);
+  uint32_t moving = 0;
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    const int i = 4096 * (k >> 2) + 4 * t + (k & 3);
+    moving |= (i < high && !((listed[i >> 5] >> (i & 31)) & 1) ? 1u : 0u) << k;
+  }
+  const int moves = ranks_alone(moving, ws, before);
   const int status = compact_status(a, head, below, moves);
   if (t == 0) compact_summary(a, head, below, moves, status);
   no_copies(a, status ? 0 : moves, t, 1024);
   for (long i = t; i < a.nfree; i += 1024)
     a.free_after[i] = status ? a.free_pages[i] : list_after(a, i, targets, below, moves);
-  move_pages<N>(a, i0, moving, targets, before, status);
+#pragma unroll
+  for (int j = 0; j < N / 4; j++) move_pages(a, 4096 * j + 4 * t, (moving >> (4 * j)) & 15u, targets, before[j], status);
 }
 __global__ __launch_bounds__(256) void k_compact_tables(CompactArgs a) {
   const bool good = a.summary[2] == 0;
@@ -548,6 +696,7 @@ extern "C" int sj_paged_fork(void* stream, const int32_t* parents, long requests
   static sj::OncePerDevice once;
   if (int st = sjh::once_per_device(once, [] {
         SJ_HIP(hipFuncSetAttribute((const void*)k_fork_plan, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * FORK_ROWS));
+        SJ_HIP(hipFuncSetAttribute((const void*)k_fork_small, hipFuncAttributeMaxDynamicSharedMemorySize, 4 * ALONE));
         return SJ_OK;
       }))
     return st;
@@ -564,6 +713,11 @@ extern "C" int sj_paged_fork(void* stream, const int32_t* parents, long requests
   a.d_page = make_div((uint32_t)page_size);
   hipStream_t s = (hipStream_t)stream;
   const long most = pages > free_count ? pages : free_count, copying = (most + 4095) / 4096;
+  if (most <= ALONE && requests <= SMALL_REQUESTS && requests_before <= 1024 && requests_before * ldt <= SMALL_CELLS) {
+    k_fork_small<<<(unsigned)requests + 1, 1024, 4 * ALONE, s>>>(a);
+    SJ_LAUNCH_CHECK("paged fork");
+    return SJ_OK;
+  }
   k_fork_plan<<<(unsigned)(1 + (copying < 512 ? copying : 512)), 1024, 8 * a.before, s>>>(a);
   if (requests || requests_before)
     k_fork_rows<<<(unsigned)(requests > requests_before ? requests : requests_before), 256, 0, s>>>(a);
@@ -620,7 +774,7 @@ extern "C" int sj_paged_compact(void* stream, const int32_t* table, long ldt, co
   a.requests = (int)requests; a.P = (int)page_size;
   a.d_page = make_div((uint32_t)page_size);
   hipStream_t s = (hipStream_t)stream;
-  if (pages <= ALONE && free_count <= ALONE) {
+  if (pages <= COMPACT_ALONE && free_count <= COMPACT_ALONE) {
     k_compact_alone<<<1, 1024, 0, s>>>(a);
   } else {
     const long blocks = (pages + 4 * NT - 1) / (4 * NT);

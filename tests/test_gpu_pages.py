@@ -141,6 +141,26 @@ def test_void_forks(status, change):
     assert want["status"] == status and (want["lengths"] == 0).all()
 
 
+@pytest.mark.parametrize("groups,beams,P,hi,spare", [(300, 4, 16, 60, 900), (256, 4, 16, 60, 900), (64, 3, 16, 60, 900),
+                                                     (193, 1, 16, 60, 900), (60, 8, 4, 300, 0), (1, 1, 4, 9, 16000),
+                                                     (1, 1, 4, 9, 17000), (7, 3, 16, 40000, 99), (7, 3, 16, 25000, 99)])
+def test_fork_in_one_launch_and_in_several(groups, beams, P, hi, spare):
+    """Sizes around those that one launch takes: requests, pages, entries of the tables."""
+    rng = np.random.default_rng(groups)
+    lengths, table, shared, free, head, pages = state(rng, groups, beams, P, hi, spare + groups * beams)
+    R = groups * beams
+    parents = rng.integers(-1, R, R)
+    assert Fork(parents, lengths, table, shared, free, head, pages, P).run().check()["status"] == 0
+    keep = np.where(rng.random(R) < 0.5, np.arange(R), -1)  # some end, the others stay
+    assert Fork(keep, lengths, table, shared, free, head, pages, P).run().check()["taken"] == 0
+    # the list begins behind a few places: some pages that come back find none
+    want = Fork(keep, lengths, table, shared, free[max(head - 5, 0):], min(head, 5), pages, P).run().check()
+    assert want["status"] == (BU.LIST_FULL if want["head"] == 0 and (want["shared"] < 0).any() else 0)
+    parents[R // 2] = R
+    assert Fork(parents, lengths, table, shared, free, head, pages, P).run().check()["status"] == 8
+    assert Fork(np.zeros(R, int), lengths, table, shared, free, len(free) + 1, pages, P).run().check()["status"] == 1
+
+
 def test_fork_without_room_on_the_list():
     """Pages that the list has no place for keep their mark, and a later step gives them back."""
     rng = np.random.default_rng(4)
@@ -254,8 +274,8 @@ def test_void_compactions_of_many_workgroups(status, change):
     assert c.check()["status"] == status
 
 
-@pytest.mark.parametrize("pages,rounds", [(16384, 0), (16385, 1), (5_000_003, 2)])
-def test_pools_of_one_workgroup_and_of_rounds(pages, rounds):
+@pytest.mark.parametrize("pages", [8192, 8193, 16384, 16385, 5_000_003])
+def test_pools_of_one_workgroup_and_of_rounds(pages):
     """Pages of which one workgroup holds all, one more, and so many that a workgroup takes several rounds."""
     rng = np.random.default_rng(pages)
     R, P, cols = 40, 4, 60
