@@ -11,11 +11,11 @@
 //
 // What bounds it.  A prompt's step is two dependent halves, its rows and then
 // all of its beams, and each ends with reductions of one workgroup: 64 prompts of
-// 4 beams over 257 f32 take 9.6 us, 2 of them the launch's.  Over 8 rows of
-// 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 16.9 us with the
-// meeting of their parts; a launch of its own for the second half had 8.5 + 15.2.
-// Over 384 rows of 50001 bf16 (38 MB, 7.5 us) the powers of e in 64 bits decide:
-// 14 operations of half rate an entry, 25.6 us, and 7.0 for the second half.
+// 4 beams over 257 f32 take 9.1 us, 2 of them the launch's.  Over 8 rows of
+// 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 16.2 us with the
+// meeting of their parts (64 kept: 31); a launch of its own for the second half
+// had 8.5 + 15.2.  Over 384 rows of 50001 bf16 (38 MB, 7.5 us) the powers of e in
+// 64 bits decide: 18 operations an entry, 25.6 us, and 7.0 for the second half.
 #include <type_traits>
 
 #include "order.h"
@@ -248,7 +248,7 @@ struct GroupShared {
   double total[CAP];
   __attribute__((aligned(16))) u64 best[256];
   u64 last[4];
-  int n;
+  int cols[4], n;
 };
 // sums and entries of the lists, as many as LDS holds
 struct Near {
@@ -268,7 +268,8 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   const int lists = B * S, all = lists * k;  // all lists' first entries, then their second ones
   const u64* sums = a.sums + 2 * row0 * S;
   auto get = [&](const u64* p) { return MEET ? part_get(p) : *p; };
-  const int near_sums = min(2 * lists, 2 * NEAR), near_keys = min(all, 8 * NEAR);
+  // the first two entries of every list; few of the others are looked at
+  const int near_sums = min(2 * lists, 2 * NEAR), near_keys = min(all, min(8 * NEAR, max(512, 2 * lists)));
   if (!there) {
     for (int i = t; i < near_sums; i += 256) near.sums[i] = get(sums + i);
 #pragma unroll 4
@@ -339,18 +340,23 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
 #pragma unroll 1
   for (int list = list0; list < lists; list += 256)
     if (from + list < all) best = larger_of(best, candidate(list, from + list, key_at(from + list)).key);
-  // the threshold: the keep-th largest of 64 columns' largest, 1 where fewer
-  // columns have any
+  // the threshold: the keep-th largest of 64 columns' largest (of 256 above 32,
+  // where the 64th of 64 would let thousands pass), 1 where fewer columns have any.
+  // Few entries lie above it, as the lists' first ones are spread over the columns.
   sh.best[t] = best;
   __syncthreads();
-  if (w == 0) {
-    const u64 col = larger_of(larger_of(best, sh.best[lane + 64]), larger_of(sh.best[lane + 128], sh.best[lane + 192]));
-    sync_wave();
-    sh.best[lane] = col;
-    sync_wave();
+  const bool many = keep > 32;
+  if (w == 0 || many) {
+    u64 col = best;
+    if (!many) {
+      col = larger_of(larger_of(best, sh.best[lane + 64]), larger_of(sh.best[lane + 128], sh.best[lane + 192]));
+      sync_wave();
+      sh.best[lane] = col;
+      sync_wave();
+    }
     int larger = 0;
 #pragma unroll 4
-    for (int i = 0; i < 64; i += 2) {
+    for (int i = 0; i < (many ? 256 : 64); i += 2) {
       const ulonglong2 q = *(const ulonglong2*)(sh.best + i);
       larger += (q.x > col) + (q.y > col);
     }
@@ -361,11 +367,20 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
       const u64 o = __shfl_xor(least, d, 64);
       least = o < least ? o : least;
     }
-    const bool enough = __popcll(__ballot(col != 0)) >= keep;
-    if (lane == 0) sh.last[0] = enough ? least : 1;
+    const int some = __popcll(__ballot(col != 0));
+    if (lane == 0) {
+      sh.last[w] = least;
+      sh.cols[w] = some;
+    }
   }
   __syncthreads();
-  const u64 T0 = sh.last[0];
+  u64 T0 = sh.last[0];
+  int some = sh.cols[0];
+  for (int i = 1; many && i < 4; i++) {
+    T0 = min(T0, sh.last[i]);
+    some += sh.cols[i];
+  }
+  if (some < keep) T0 = 1;
 #pragma unroll 1
   for (int list = list0; list < lists; list += 256)
 #pragma unroll 1

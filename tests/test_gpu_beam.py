@@ -97,12 +97,14 @@ def test_select(dtype, V, groups, beams, keep):
     assert all((a == b.host()).all() for a, b in zip(first, s.ints + [s.out]))  # every output again, the same bits
 
 
-@pytest.mark.parametrize("beams,slices", [(1, 1), (5, 1), (31, 2), (63, 2), (64, 2), (43, 3), (17, 11), (51, 5), (64, 4), (37, 7)])
-def test_select_lists_of_any_number(beams, slices):
+@pytest.mark.parametrize("beams,slices,keep", [(1, 1, 11), (5, 1, 11), (31, 2, 11), (63, 2, 11), (64, 2, 11), (43, 3, 11),
+                                               (17, 11, 11), (51, 5, 11), (64, 4, 11), (37, 7, 11), (1, 1, 40), (5, 1, 64),
+                                               (17, 11, 33), (64, 4, 64), (37, 7, 64)])
+def test_select_lists_of_any_number(beams, slices, keep):
     """As many lists as threads of the workgroup that takes them together, half as many, a few more, a few less."""
     rng = np.random.default_rng(beams)
     x = logits(rng, beams, 4096 * slices - 5, "f32")
-    Select(x, rng.normal(-20, 2, beams), beams, 11, "f32", lengths=np.full(beams, 3)).run().check()
+    Select(x, rng.normal(-20, 2, beams), beams, keep, "f32", lengths=np.full(beams, 3)).run().check()
 
 
 @pytest.mark.parametrize("V", [5, 257, 3000, 9000])
