@@ -502,7 +502,8 @@ int sj_paged_copy(void *stream, void *k_cache, void *v_cache, long ldkv, int dty
  * 1], ascending), whose first prefix[g] positions hold the same keys and
  * values: their table rows name the same pages there, or pages of the same
  * content.  Those are read once for all rows of the group, from the first
- * request's table row; every row's other keys as in sj_paged_attention, whose
+ * request's table row (in small calls, where that takes longer, by every row from
+ * its own); every row's other keys as in sj_paged_attention, whose
  * results these are but for the order of the sums.  starts [requests + 1]: the
  * requests' first rows (sj_paged_plan's; null: row i is request i's).  A row
  * attends alone, all its keys through its own table row, where its owner is

@@ -25,9 +25,10 @@ namespace {
 // alike.  What was summed of a walk goes to the workspace; a second launch joins
 // the parts of each row's two walks.
 //
-// 4 rows over 960 shared keys (6/2 heads of 64, bf16) take 14.6 us: 1.6 to launch,
-// 3.3 for the lists, a walk's chain of page, keys and products, 4.5 for the join.
-// 24 groups of 5 rows over up to 6000 keys (16/4 heads of 64, fp32) take 36.5 us,
+// Small calls go through sj_paged_attention, each row by itself (FEW): together 4
+// rows over 960 shared keys (6/2 heads of 64, bf16) take 14.8 us, 1.6 to launch,
+// 3.3 for the lists, a walk's chain of page, keys and products, 4.5 for the join;
+// alone 10.5.  24 groups of 5 rows over up to 6000 keys (16/4 heads of 64, fp32) take 36.5 us,
 // 12 of them their 61 MB at a copy's rate: each wave waits for two or three tiles.
 // 64 rows over 16384 keys (32/8 heads of 128, bf16) take 56 us, where their 91 MB
 // are 18 and their products, P as two planes, 18: the lists 3, the shared walks
@@ -38,6 +39,13 @@ constexpr int CT = 2, COLS = 16 * CT, BLOCK = 4 * COLS;
 constexpr int WIDE_PLACE = 64;  // keys of a place of a walk whose waves go by columns
 constexpr int MAX_ROWS = 2048, MAX_GROUPS = 256;  // what LDS lists beside two stages of tiles
 constexpr int GROUPS_OF_WAVES = 512;  // workgroups, at most
+// Elements of keys and values that the rows read of as long sequences as the table
+// holds, if each reads its own: up to here they do (us, for the rows together and
+// alone: 4 rows over 960 keys, 2 KV heads of 64, 0.5 M, 14.8 and 10.5; 128 rows of
+// that, 34 M, 17.3 and 12.5; 16 rows over 1024, 8 heads of 128, 42 M, 18.6 and
+// 23.2; 8 rows over 2048, 38 M, 21.4 and 23.0; fp32: 8 groups of 5 rows over up to
+// 2000 keys, 4 heads of 64, 47 M, 20.5 and 15.6, 24 over 1000, 70 M, 23.7 each).
+constexpr double FEW = 33554432.0;
 
 struct SharedArgs {
   PagedArgs p;
@@ -736,8 +744,9 @@ extern "C" int sj_paged_attention_shared(void* stream, const void* q, long ldq, 
     return st;
   if (s.p.rows == 0) return SJ_OK;
   // all places of the line are counted in 31 bits
-  const double places = ((double)rows * hk * (s.p.QT + s.p.G / (double)COLS) + (double)groups * hk) * (ldt * page_size / 64.0 + 1);
-  if (!grouped(rows, head_dim, groups) || places >= 2147483647.0)
+  const long most = ldt * page_size, seen = window > 0 && window < most ? window : most;
+  const double places = ((double)rows * hk * (s.p.QT + s.p.G / (double)COLS) + (double)groups * hk) * (most / 64.0 + 1);
+  if (!grouped(rows, head_dim, groups) || places >= 2147483647.0 || 2.0 * rows * hk * seen * head_dim <= FEW)
     return sj_paged_attention(stream, q, ldq, k_cache, v_cache, ldkv, dtype, pages, page_size, table, ldt, requests, owners,
                               positions, rows, hq, hk, head_dim, window, o, ldo, lse, workspace, workspace_bytes);
   const Layout l = layout_of(rows, hq, hk, head_dim, groups);

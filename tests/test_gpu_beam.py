@@ -252,7 +252,8 @@ def test_a_search_over_the_paged_cache():
     groups, B, P, hq, hk, D, V, steps, END = 3, 4, 8, 4, 2, 64, 257, 7, 5
     R, W, J = groups * B, hq * D, hk * D
     prompt = np.array([21, 8, 40])
-    width = int(-(-(prompt.max() + steps + 2) // P))
+    # wide tables: attention walks the shared prefixes for all of a prompt's beams together
+    width = max(int(-(-(prompt.max() + steps + 2) // P)), 2 ** 24 // (R * hk * D) // P + 1)
     pages = 80
     order = rng.permutation(pages)
     table, shared, made = np.full((R, width), -1), np.zeros(pages, int), 0

@@ -35,9 +35,17 @@ class Shared(Attend):
         self.starts = np.arange(n + 1) * per
         self.use_starts = True
 
+    # calls on small tables go through sj_paged_attention: with empty columns these are large ones
+    wide = True
+
     def upload(self):
-        super().upload()
         n = len(self.pos)
+        if self.wide:
+            keys = 2 ** 24 // (n * self.hk * self.D) + 1
+            more = np.full((len(self.tab), max(keys // self.P + 1 - self.width, 0)), -1)
+            self.tab = np.concatenate([self.tab, more], 1)
+            self.width = self.tab.shape[1]
+        super().upload()
         self.need = native()[1].sj_paged_attention_shared_workspace_bytes(n, self.hq, self.hk, self.D, len(self.prefix))
         self.ws = G.Dev(max(self.need, 16), "u8").upload(np.full(max(self.need, 16), 0xFF))
         self.S, self.F, self.X = PU.ints(self.starts), PU.ints(self.first), PU.ints(np.append(self.prefix, 0))
@@ -101,6 +109,27 @@ def test_shared_windows(dtype, window):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window", [100, 150])
+def test_shared_windows_of_many_rows(dtype, window):
+    """As many rows as the groups are walked for within such windows."""
+    Shared(window, dtype, 16, 16, 128, 16, GROUPS * 4, alone=[400] * 4, window=window).upload().run().check()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hk,D,P", [(6, 2, 64, 16), (14, 2, 96, 7), (5, 5, 256, 32), (3, 3, 7, 16), (40, 2, 64, 64)])
+def test_shared_small_calls(dtype, hq, hk, D, P):
+    """Every row by itself: the bits of sj_paged_attention."""
+    a = Shared(hq * D + P, dtype, hq, hk, D, P, GROUPS, alone=[0, 1, 77], pad=2)
+    a.wide = False
+    a.upload().run().check()
+    first = a.O.host().copy(), a.L.host().copy()
+    for b in (a.O, a.L):
+        b.upload(np.full(b.n, 55.0))
+    Attend.run(a)
+    assert all((x == y.host()).all() for x, y in zip(first, (a.O, a.L)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("D,ldkv,off", [(64, 136, 0), (64, 131, 3), (32, 72, 8), (128, 260, 1), (80, 161, 5)])
 def test_shared_strides_and_alignment(dtype, D, ldkv, off):
     a = Shared(D + off, dtype, 4, 2, D, 16, [(33, [3, 70]), (16, [1, 2, 3])], owners=False, ldkv=max(ldkv, 2 * D), off=off)
@@ -110,7 +139,7 @@ def test_shared_strides_and_alignment(dtype, D, ldkv, off):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_shared_reads_the_first_requests_pages(dtype):
-    """The prefix is read through the first request's row: another row's entries there are not looked at."""
+    """In a large call the prefix is read through the first request's row: another row's entries there are not looked at."""
     a = Shared(3, dtype, 6, 2, 64, 16, [(64, [5, 6, 7])])
     a.upload()
     a.T.upload(np.where((np.arange(len(a.tab))[:, None] > 0) & (np.arange(a.width)[None, :] < 4), -1, a.tab))
