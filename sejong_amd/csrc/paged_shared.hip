@@ -743,6 +743,11 @@ extern "C" int sj_paged_attention_shared(void* stream, const void* q, long ldq, 
                                positions, rows, hq, hk, head_dim, window, o, ldo, lse, s.p))
     return st;
   if (s.p.rows == 0) return SJ_OK;
+  const size_t need = sj_paged_attention_shared_workspace_bytes(rows, hq, hk, head_dim, groups);
+  SJ_REQUIRE(((uintptr_t)workspace & 15) == 0, "paged attention of groups: the workspace is not 16-byte aligned");
+  if (need > workspace_bytes || (need && !workspace))
+    return sjh::fail(SJ_ERR_CAPACITY, "paged attention of groups workspace: required %zu bytes, available %zu bytes", need,
+                     workspace ? workspace_bytes : 0);
   // all places of the line are counted in 31 bits
   const long most = ldt * page_size, seen = window > 0 && window < most ? window : most;
   const double places = ((double)rows * hk * (s.p.QT + s.p.G / (double)COLS) + (double)groups * hk) * (most / 64.0 + 1);
@@ -750,11 +755,6 @@ extern "C" int sj_paged_attention_shared(void* stream, const void* q, long ldq, 
     return sj_paged_attention(stream, q, ldq, k_cache, v_cache, ldkv, dtype, pages, page_size, table, ldt, requests, owners,
                               positions, rows, hq, hk, head_dim, window, o, ldo, lse, workspace, workspace_bytes);
   const Layout l = layout_of(rows, hq, hk, head_dim, groups);
-  const size_t need = sj_paged_attention_shared_workspace_bytes(rows, hq, hk, head_dim, groups);
-  SJ_REQUIRE(((uintptr_t)workspace & 15) == 0, "paged attention of groups: the workspace is not 16-byte aligned");
-  if (need > workspace_bytes || !workspace)
-    return sjh::fail(SJ_ERR_CAPACITY, "paged attention of groups workspace: required %zu bytes, available %zu bytes", need,
-                     workspace ? workspace_bytes : 0);
   s.starts = starts; s.group_starts = group_starts; s.prefix = prefix;
   s.groups = (int)groups;
   s.d_group = make_div((uint32_t)s.p.G);
