@@ -13,7 +13,7 @@
 // all of its beams, and each ends with reductions of one workgroup: 64 prompts of
 // 4 beams over 257 f32 take 9.1 us, 2 of them the launch's.  Over 8 rows of
 // 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 16.2 us with the
-// meeting of their parts (64 kept: 31); a launch of its own for the second half
+// meeting of their parts (64 kept: 25); a launch of its own for the second half
 // had 8.5 + 15.2.  Over 384 rows of 50001 bf16 (38 MB, 7.5 us) the powers of e in
 // 64 bits decide: 18 operations an entry, 25.6 us, and 7.0 for the second half.
 #include <type_traits>
@@ -248,7 +248,8 @@ struct GroupShared {
   double total[CAP];
   __attribute__((aligned(16))) u64 best[256];
   u64 last[4];
-  int cols[4], n;
+  uint16_t pick[CAP];
+  int cols[4], n, picked;
 };
 // sums and entries of the lists, as many as LDS holds
 struct Near {
@@ -259,6 +260,24 @@ struct Candidate {
   int flat;
   double total;
 };
+
+// of a wave's columns, among the n in LDS, the least of those with fewer than keep
+// larger ones (equal columns have one place)
+__device__ __forceinline__ u64 least_of_first(const u64* best, int n, u64 col, int keep) {
+  int larger = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; i += 2) {
+    const ulonglong2 q = *(const ulonglong2*)(best + i);
+    larger += (q.x > col) + (q.y > col);
+  }
+  u64 least = col && larger < keep ? col : ~0ull;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const u64 o = __shfl_xor(least, d, 64);
+    least = o < least ? o : least;
+  }
+  return least;
+}
 
 template <bool MEET>
 __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared& sh, Near& near, bool there) {
@@ -354,19 +373,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
       sh.best[lane] = col;
       sync_wave();
     }
-    int larger = 0;
-#pragma unroll 4
-    for (int i = 0; i < (many ? 256 : 64); i += 2) {
-      const ulonglong2 q = *(const ulonglong2*)(sh.best + i);
-      larger += (q.x > col) + (q.y > col);
-    }
-    // equal columns have one place: the least of those with fewer than keep larger ones
-    u64 least = col && larger < keep ? col : ~0ull;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-      const u64 o = __shfl_xor(least, d, 64);
-      least = o < least ? o : least;
-    }
+    const u64 least = least_of_first(sh.best, many ? 256 : 64, col, keep);
     const int some = __popcll(__ballot(col != 0));
     if (lane == 0) {
       sh.last[w] = least;
@@ -404,11 +411,38 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   };
   const int n = sh.n;
   if (n <= CAP) {
-    for (int i = t >> 2; i < n; i += 64) {
+    // Every entry's place is the number of larger ones.  Among many only the keep
+    // largest of 256 columns, and what lies with them, can have one below keep (384
+    // rows, 32 kept: up to 700 entries, 41 us for all against all, 22 this way).
+    int m = n;
+    if (n > 192) {
+      u64 col = 0;
+      for (int i = t; i < n; i += 256) col = larger_of(col, sh.cand[i]);
+      sh.best[t] = col;
+      if (t == 0) sh.picked = 0;
+      __syncthreads();
+      const u64 least = least_of_first(sh.best, 256, col, keep);
+      if (lane == 0) sh.last[w] = least;
+      __syncthreads();
+      const u64 T1 = min(min(sh.last[0], sh.last[1]), min(sh.last[2], sh.last[3]));
+      for (int i = t; i < n; i += 256)
+        if (sh.cand[i] >= T1) sh.pick[atomicAdd(&sh.picked, 1)] = (uint16_t)i;
+      __syncthreads();
+      m = sh.picked;
+    }
+    for (int q = t >> 2; q < m; q += 64) {
+      const int i = n > 192 ? sh.pick[q] : q;
       const u64 key = sh.cand[i];
       const int flat = sh.where[i];
-      uint32_t place = 0;
-      for (int j = t & 3; j < n; j += 4) place += sh.cand[j] > key || (sh.cand[j] == key && sh.where[j] < flat);
+      uint32_t place = 0, same = 0;
+#pragma unroll 4
+      for (int j = t & 3; j < n; j += 4) {
+        const u64 other = sh.cand[j];
+        place += other > key;
+        same += other == key;
+      }
+      if (same > (uint32_t)((i & 3) == (t & 3)))  // another of the same rank
+        for (int j = t & 3; j < n; j += 4) place += sh.cand[j] == key && sh.where[j] < flat;
       place += dpp<0xB1>(place);
       place += dpp<0x4E>(place);
       if ((t & 3) == 0 && (int)place < keep) write((int)place, true, flat, sh.total[i]);

@@ -190,6 +190,16 @@ def test_select_ties_go_to_the_lowest_index(dtype, V):
     assert (want["tokens"][20:40] == np.arange(20)).all()
 
 
+@pytest.mark.parametrize("values", [1, 2, 40])
+@pytest.mark.parametrize("V,beams,keep", [(100, 8, 64), (300, 8, 32), (9000, 6, 64), (5000, 3, 64)])
+def test_select_many_entries_of_few_ranks(values, V, beams, keep):
+    """Hundreds of candidates at the threshold, all of one rank or of few."""
+    rng = np.random.default_rng(V)
+    x = rng.integers(0, values, (2 * beams, V)) * 0.25
+    x[:] = np.sort(x[:1], 1)[:, rng.permutation(V)]  # every row has the same sum
+    Select(x, np.full(2 * beams, -4.0), beams, keep, "f32", lengths=np.full(2 * beams, 3)).run().check()
+
+
 def test_select_totals_next_to_each_other():
     """Beams whose totals differ by less than fp32 holds of them: the order is that of 64 bits."""
     rng = np.random.default_rng(1)
