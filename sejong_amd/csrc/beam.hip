@@ -11,9 +11,9 @@
 //
 // What bounds it.  A prompt's step is two dependent halves, its rows and then
 // all of its beams, and each ends with reductions of one workgroup: 64 prompts of
-// 4 beams over 257 f32 take 9.1 us, 2 of them the launch's.  Over 8 rows of
-// 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 16.2 us with the
-// meeting of their parts (64 kept: 25); a launch of its own for the second half
+// 4 beams over 257 f32 take 7.5 us, 2 of them the launch's.  Over 8 rows of
+// 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 14.8 us with the
+// meeting of their parts (64 kept: 24); a launch of its own for the second half
 // had 8.5 + 15.2.  Over 384 rows of 50001 bf16 (38 MB, 7.5 us) the powers of e in
 // 64 bits decide: 18 operations an entry, 25.6 us, and 7.0 for the second half.
 #include <type_traits>
@@ -270,13 +270,17 @@ __device__ __forceinline__ u64 least_of_first(const u64* best, int n, u64 col, i
     const ulonglong2 q = *(const ulonglong2*)(best + i);
     larger += (q.x > col) + (q.y > col);
   }
-  u64 least = col && larger < keep ? col : ~0ull;
+  // that is a column with the most larger ones, below keep <= 64: found bit by bit
+  uint64_t lanes = __ballot(col != 0 && larger < keep);
+  if (lanes == 0) return ~0ull;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const u64 o = __shfl_xor(least, d, 64);
-    least = o < least ? o : least;
+  for (int bit = 5; bit >= 0; bit--) {
+    const uint64_t set = lanes & __ballot((larger >> bit) & 1);
+    if (set) lanes = set;
   }
-  return least;
+  const int lane = __builtin_ctzll(lanes);
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(col >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)col, lane);
 }
 
 template <bool MEET>
@@ -290,9 +294,18 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   // the first two entries of every list; few of the others are looked at
   const int near_sums = min(2 * lists, 2 * NEAR), near_keys = min(all, min(8 * NEAR, max(512, 2 * lists)));
   if (!there) {
-    for (int i = t; i < near_sums; i += 256) near.sums[i] = get(sums + i);
+    // two of each a thread, all on their way at once; near_sums is at most 512
+    u64 s0 = 0, s1 = 0, k0 = 0, k1 = 0;
+    if (t < near_sums) s0 = get(sums + t);
+    if (t < near_keys) k0 = get(keys + t);
+    if (t + 256 < near_sums) s1 = get(sums + t + 256);
+    if (t + 256 < near_keys) k1 = get(keys + t + 256);
+    if (t < near_sums) near.sums[t] = s0;
+    if (t < near_keys) near.keys[t] = k0;
+    if (t + 256 < near_sums) near.sums[t + 256] = s1;
+    if (t + 256 < near_keys) near.keys[t + 256] = k1;
 #pragma unroll 4
-    for (int i = t; i < near_keys; i += 256) near.keys[i] = get(keys + i);
+    for (int i = t + 512; i < near_keys; i += 256) near.keys[i] = get(keys + i);
   }
   auto sum_at = [&](int i) { return i < near_sums ? near.sums[i] : get(sums + i); };
   auto key_at = [&](int i) { return i < near_keys ? near.keys[i] : get(keys + i); };
@@ -310,7 +323,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
     if (!ended) {
       for (int s = l; s < S; s += 16) M = fmaxf(M, __uint_as_float((uint32_t)sum_at(2 * (b * S + s))));
 #pragma unroll
-      for (int d = 8; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+      for (int d = 8; S > 1 && d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
 #pragma unroll 1
       for (int s = l; s < S; s += 16) {
         const float m = __uint_as_float((uint32_t)sum_at(2 * (b * S + s)));
@@ -318,7 +331,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
         sum += v * power_of(m, M == -INFINITY ? 0.f : M);
       }
 #pragma unroll
-      for (int d = 8; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+      for (int d = 8; S > 1 && d; d >>= 1) sum += __shfl_xor(sum, d, 64);
     }
     // one logarithm for both
     const double after = (double)max(ended ? (long)len : len + 1L, 1L), ln = log(l == 0 ? sum : after);
@@ -355,39 +368,44 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   // stop at the first below the threshold.
   const int each = max(256 / lists, 1), step = each * lists, from = t / lists * lists;
   const int list0 = t < step ? t - from : lists;
-  u64 best = 0;
+  // (up to 64 entries are simply all ranked: 9.4 us with a threshold for 64 prompts
+  // of 4 beams over 257, 7.8 without)
+  u64 T0 = 1;
+  if (all > 64) {
+    u64 best = 0;
 #pragma unroll 1
-  for (int list = list0; list < lists; list += 256)
-    if (from + list < all) best = larger_of(best, candidate(list, from + list, key_at(from + list)).key);
-  // the threshold: the keep-th largest of 64 columns' largest (of 256 above 32,
-  // where the 64th of 64 would let thousands pass), 1 where fewer columns have any.
-  // Few entries lie above it, as the lists' first ones are spread over the columns.
-  sh.best[t] = best;
-  __syncthreads();
-  const bool many = keep > 32;
-  if (w == 0 || many) {
-    u64 col = best;
-    if (!many) {
-      col = larger_of(larger_of(best, sh.best[lane + 64]), larger_of(sh.best[lane + 128], sh.best[lane + 192]));
-      sync_wave();
-      sh.best[lane] = col;
-      sync_wave();
+    for (int list = list0; list < lists; list += 256)
+      if (from + list < all) best = larger_of(best, candidate(list, from + list, key_at(from + list)).key);
+    // the threshold: the keep-th largest of 64 columns' largest (of 256 above 32,
+    // where the 64th of 64 would let thousands pass), 1 where fewer columns have any.
+    // Few entries lie above it, as the lists' first ones are spread over the columns.
+    sh.best[t] = best;
+    __syncthreads();
+    const bool many = keep > 32;
+    if (w == 0 || many) {
+      u64 col = best;
+      if (!many) {
+        col = larger_of(larger_of(best, sh.best[lane + 64]), larger_of(sh.best[lane + 128], sh.best[lane + 192]));
+        sync_wave();
+        sh.best[lane] = col;
+        sync_wave();
+      }
+      const u64 least = least_of_first(sh.best, many ? 256 : 64, col, keep);
+      const int some = __popcll(__ballot(col != 0));
+      if (lane == 0) {
+        sh.last[w] = least;
+        sh.cols[w] = some;
+      }
     }
-    const u64 least = least_of_first(sh.best, many ? 256 : 64, col, keep);
-    const int some = __popcll(__ballot(col != 0));
-    if (lane == 0) {
-      sh.last[w] = least;
-      sh.cols[w] = some;
+    __syncthreads();
+    int some = sh.cols[0];
+    T0 = sh.last[0];
+    for (int i = 1; many && i < 4; i++) {
+      T0 = min(T0, sh.last[i]);
+      some += sh.cols[i];
     }
+    if (some < keep) T0 = 1;
   }
-  __syncthreads();
-  u64 T0 = sh.last[0];
-  int some = sh.cols[0];
-  for (int i = 1; many && i < 4; i++) {
-    T0 = min(T0, sh.last[i]);
-    some += sh.cols[i];
-  }
-  if (some < keep) T0 = 1;
 #pragma unroll 1
   for (int list = list0; list < lists; list += 256)
 #pragma unroll 1
