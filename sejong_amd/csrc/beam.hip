@@ -85,10 +85,11 @@ __device__ __forceinline__ u64 rank_key(double r) {
 // thread: the maximum, the sum of powers relative to it, and the k largest
 // entries in their order (put(place, key), key 0 where there are fewer).  As in
 // the token scores the largest come from a threshold, the k-th largest of 64 or
-// 256 column maxima.
+// 256 column maxima.  -inf is in no list; in a row with NaN they hold anything,
+// since its sum leaves it without candidates.
 template <int NT, int EV>
 struct RowShared {
-  static constexpr int CAPR = NT == 64 ? 64 * EV : CAP;
+  static constexpr int CAPR = NT == 64 ? 512 : CAP;
   u64 cand[CAPR], last[4];
   double sum[4];
   __attribute__((aligned(16))) float best[NT];
@@ -192,7 +193,7 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
   for (int j = 0; j < PARTS; j++)
     if (index(PART * j) < end && pm[j] >= T0)
 #pragma unroll
-      for (int i = PART * j; i < PART * (j + 1); i++) mine += f(i) >= T0 && index(i) < end;
+      for (int i = PART * j; i < PART * (j + 1); i++) mine += f(i) >= T0 && f(i) > -INFINITY && index(i) < end;
   const uint32_t upto = scan_add(mine);
   int from = 0;
   if (lane == 63 && upto) from = atomicAdd(&sh.n, (int)upto);
@@ -202,20 +203,20 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
     if (index(PART * j) < end && pm[j] >= T0) {
 #pragma unroll
       for (int i = PART * j; i < PART * (j + 1); i++)
-        if (f(i) >= T0 && index(i) < end) {
+        if (f(i) >= T0 && f(i) > -INFINITY && index(i) < end) {
           if (from < CAPR) sh.cand[from] = order_key(f(i), index(i));
           from++;
         }
     }
   sync();
-  const int n = sh.n, held = min(k, end - base);
-  if (n <= CAPR && n >= held) {
+  const int n = sh.n;
+  if (n <= CAPR) {
     rank<NT>(sh.cand, n, k, t, put);
-    for (int i = held + t; i < k; i += NT) put(i, 0ull);
+    for (int i = n + t; i < k; i += NT) put(i, 0ull);
     return;
   }
-  // more than LDS holds at the threshold (a masked row's -inf), or fewer
-  // entries than asked for beside NaN: the largest below the last, k times
+  // more than LDS holds at the threshold (a mask's lowest value): the largest
+  // below the last, k times
   u64 last = ~0ull;
   for (int j = 0; j < k; j++) {
     u64 k0 = 0;
@@ -254,7 +255,7 @@ struct GroupShared {
 };
 // sums and entries of the lists, as many as LDS holds
 struct Near {
-  u64 sums[2 * NEAR], keys[8 * NEAR];
+  u64 sums[2 * NEAR], keys[4 * NEAR];
 };
 struct Candidate {
   u64 key;  // 0: none
@@ -293,7 +294,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   const u64* sums = a.sums + 2 * row0 * S;
   auto get = [&](const u64* p) { return MEET ? part_get(p) : *p; };
   // the first two entries of every list; few of the others are looked at
-  const int near_sums = min(2 * lists, 2 * NEAR), near_keys = min(all, min(8 * NEAR, max(512, 2 * lists)));
+  const int near_sums = min(2 * lists, 2 * NEAR), near_keys = min(all, min(4 * NEAR, max(512, 2 * lists)));
   if (!there) {
     // two of each a thread, all on their way at once; near_sums is at most 512
     u64 s0 = 0, s1 = 0, k0 = 0, k1 = 0;
