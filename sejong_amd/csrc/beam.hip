@@ -11,11 +11,11 @@
 //
 // What bounds it.  A prompt's step is two dependent halves, its rows and then
 // all of its beams, and each ends with reductions of one workgroup: 64 prompts of
-// 4 beams over 257 f32 take 7.5 us, 2 of them the launch's.  Over 8 rows of
-// 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 14.8 us with the
-// meeting of their parts (64 kept: 24); a launch of its own for the second half
+// 4 beams over 257 f32 take 7.8 us, 2 of them the launch's.  Over 8 rows of
+// 131072 f32 (4 MB, 1 us at a copy's rate) 256 workgroups take 15.4 us with the
+// meeting of their parts (64 kept: 26); a launch of its own for the second half
 // had 8.5 + 15.2.  Over 384 rows of 50001 bf16 (38 MB, 7.5 us) the powers of e in
-// 64 bits decide: 18 operations an entry, 25.6 us, and 7.0 for the second half.
+// 64 bits decide: 18 operations an entry, 25.6 us, and 7.2 for the second half.
 #include <type_traits>
 
 #include "order.h"
@@ -244,7 +244,7 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
 struct GroupShared {
   double base[64], factor[64], score[64];  // the beam's L, length^power
   int live[64];                            // 0: no candidate, 1: its tokens, 2: ended
-  int order[64], open, closed;             // the beams of the second, then of the third; as many
+  int order[64];                           // the beams of the second, then of the third
   u64 cand[CAP];
   int32_t where[CAP];
   double total[CAP];
@@ -350,23 +350,21 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   }
   __syncthreads();
   // the beams with candidates: those whose tokens are, then the ended ones
-  if (w == 0) {
-    const int live = lane < B ? sh.live[lane] : 0;
-    const uint64_t open = __ballot(live == 1), closed = __ballot(live == 2), below = (1ull << lane) - 1;
-    if (live == 1) sh.order[__popcll(open & below)] = lane;
-    if (live == 2) sh.order[__popcll(open) + __popcll(closed & below)] = lane;
-    if (lane == 0) {
-      sh.open = __popcll(open);
-      sh.closed = __popcll(closed);
-    }
+  const int state = lane < B ? sh.live[lane] : 0;
+  const uint64_t with = __ballot(state == 1), done = __ballot(state == 2), below = (1ull << lane) - 1;
+  const int beams_open = __popcll(with);
+  const bool in_order = beams_open == B;
+  if (!in_order) {
+    if (w == 0 && state == 1) sh.order[__popcll(with & below)] = lane;
+    if (w == 0 && state == 2) sh.order[beams_open + __popcll(done & below)] = lane;
+    __syncthreads();
   }
-  __syncthreads();
   // their lists: one for each slice of an open beam, one of one entry of an ended one
-  const int open = sh.open * S, some_lists = open + sh.closed;
+  const int open = beams_open * S, closed = __popcll(done), some_lists = open + closed;
   auto candidate = [&](int list, int place) {
     Candidate c = {0, 0, 0.0};
     const bool ended = list >= open;
-    const int nth = ended ? list - open + sh.open : list / S, b = sh.order[nth];
+    const int nth = ended ? list - open + beams_open : list / S, b = in_order ? nth : sh.order[nth];
     c.total = sh.score[b];
     if (ended) {
       if (place) return c;
@@ -390,7 +388,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   // (up to 64 entries are simply all ranked: 9.4 us with a threshold for 64 prompts
   // of 4 beams over 257, 7.8 without)
   u64 T0 = 1;
-  if (open * k + sh.closed > 64) {
+  if (open * k + closed > 64) {
     u64 best = 0;
 #pragma unroll 1
     for (int list = list0; list < some_lists; list += 256)

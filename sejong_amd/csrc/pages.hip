@@ -425,7 +425,7 @@ __global__ __launch_bounds__(1024) void k_fork_small(ForkArgs a) {
 // the list takes its own off, and counts its low pages; they are put in a row,
 // the moving pages counted; moves.  The tables are a launch of their own.
 //
-// 2048 pages to half take 8.9 us (5.2 + 2.7; five launches 16.6), 400001 pages to
+// 2048 pages to half take 7.9 us (5.2 + 2.7; five launches 16.6), 400001 pages to
 // three quarters 19.7 us (2.9 + 3.4 + 3.5 + 6.8 + 4.7; 78 us with 16 entries a
 // thread): again launches, and the moves' scattered writes.
 
