@@ -164,7 +164,9 @@ __device__ __forceinline__ void row_best(const T* x, int base, int end, int k, R
   // sum is only asked for NaN
   const float ref = m == -INFINITY ? 0.f : m;
   const double scaled = -(double)ref * LOG2E_64;
-  const bool far = (double)least_of - (double)ref < -FAR;
+  // past 1024 the rounding of the scaled maximum is no longer less than the
+  // polynomial's error: there, too, the difference comes first, which is exact
+  const bool far = (double)least_of - (double)ref < -FAR || !(fabsf(ref) <= 1024.f);
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < NU; i++)

@@ -148,6 +148,16 @@ def test_select_large_logits(dtype, V, size):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [300, 900, 5000])
+@pytest.mark.parametrize("size", [-1000.0, 1100.0, -7e4, 1e6, 2.0 ** 40, 1e30, -1e30])
+def test_select_logits_near_a_large_one(dtype, V, size):
+    """All logits lie near one far from 0, at the largest sizes on it."""
+    rng = np.random.default_rng(V)
+    x = G.O.round_to(size + rng.normal(0, 2, (8, V)), dtype)
+    Select(x, rng.normal(-8, 3, 8), 4, 7, dtype, lengths=np.full(8, 5)).run().check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("V", [40, 900, 5000, 40000])
 def test_select_masked_entries(dtype, V):
     """Rows whose mask leaves a few tokens, one, or none; masks of the type's lowest value, which are candidates still."""
