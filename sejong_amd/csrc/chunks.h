@@ -1,0 +1,42 @@
+// How a pool's pages and its free list are dealt out to workgroups, and where
+// their counts lie in the workspace.  Host code alone, no HIP.
+#pragma once
+#include <stddef.h>
+
+namespace sj {
+
+// The workgroups of a launch over n entries: chunks of whole rounds.  Every
+// workgroup adds up the counts of those before it, so there are at most
+// CHUNKS.
+constexpr long CHUNK_ROUND = 1024;  // entries of a workgroup's round
+constexpr long CHUNKS = 4096;
+struct Chunks {
+  long chunk, count;
+};
+inline Chunks chunks_of(long n) {
+  const long rounds = n > CHUNK_ROUND * CHUNKS ? (n + CHUNK_ROUND * CHUNKS - 1) / (CHUNK_ROUND * CHUNKS) : 1;
+  return {rounds * CHUNK_ROUND, (n + rounds * CHUNK_ROUND - 1) / (rounds * CHUNK_ROUND)};
+}
+// The most chunks that n entries or any part of them take: the count falls to
+// half where a workgroup begins to take a round more.
+inline long chunks_most(long n) {
+  const long rounds = (n + CHUNK_ROUND - 1) / CHUNK_ROUND;
+  return rounds < CHUNKS ? rounds : CHUNKS;
+}
+
+// The compaction's workspace, in places of 4 bytes: where the high pages go, the
+// free pages below, the workgroups' counts of those and of the pages that move
+// (high pages are any part of the pool).
+struct CompactSpace {
+  size_t targets, below, moves, all;
+};
+inline CompactSpace compact_space(long pages, long free_count) {
+  CompactSpace s;
+  s.targets = (size_t)pages;
+  s.below = s.targets + (size_t)free_count;
+  s.moves = s.below + (size_t)chunks_of(free_count).count;
+  s.all = s.moves + (size_t)chunks_most(pages);
+  return s;
+}
+
+}  // namespace sj

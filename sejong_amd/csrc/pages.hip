@@ -5,23 +5,15 @@
 // `shared` [pages] counts the holders of a page beyond its first: a page that
 // one table row names has 0 and needs no entry when the plan hands it out.  All
 // state is written to arrays of its own, so that a void step leaves what was.
+#include "chunks.h"
 #include "lanes.h"
 
 using namespace sj;
 
 namespace {
 
-// The workgroups of a launch over n entries: chunks of whole rounds, a round
-// four consecutive entries a thread.  Every workgroup adds up the counts of
-// those before it, so there are at most 4096.
-constexpr int NT = 256, PER = 4, ROUND = NT * PER;
-struct Chunks {
-  long chunk, count;
-};
-Chunks chunks_of(long n) {
-  const long rounds = n > ROUND * 4096L ? (n + ROUND * 4096L - 1) / (ROUND * 4096L) : 1;
-  return {rounds * ROUND, (n + rounds * ROUND - 1) / (rounds * ROUND)};
-}
+constexpr int NT = 256, PER = 4, ROUND = NT * PER;  // a round: four consecutive entries a thread
+static_assert(ROUND == CHUNK_ROUND, "a chunk is whole rounds");
 constexpr int ALONE = 16384;  // entries, at most, that one workgroup takes by itself: 16 a thread
 constexpr int COMPACT_ALONE = 8192;  // of a compaction (8192 pages 13.8 us, 16.6 in five launches; 16384 18.9 and 16.8)
 
@@ -736,7 +728,7 @@ extern "C" int sj_paged_fork(void* stream, const int32_t* parents, long requests
 
 extern "C" size_t sj_paged_compact_workspace_bytes(long pages, long free_count) {
   if (pages < 0 || free_count < 0) return 0;
-  return 4 * (size_t)(pages + free_count + chunks_of(pages).count + chunks_of(free_count).count);
+  return 4 * compact_space(pages, free_count).all;
 }
 
 extern "C" int sj_paged_compact(void* stream, const int32_t* table, long ldt, const int32_t* lengths, long requests,
@@ -766,9 +758,10 @@ extern "C" int sj_paged_compact(void* stream, const int32_t* table, long ldt, co
   a.table_after = table_after; a.shared_after = shared_after; a.free_after = free_after; a.copies = copies;
   a.summary = summary;
   a.to = (int32_t*)workspace;
-  a.targets = a.to + pages;
-  a.below = a.targets + free_count;
-  a.moves = a.below + chunks_of(free_count).count;
+  const CompactSpace at = compact_space(pages, free_count);
+  a.targets = a.to + at.targets;
+  a.below = a.to + at.below;
+  a.moves = a.to + at.moves;
   a.ldt = ldt; a.nfree = free_count; a.pages = pages; a.after = pages_after; a.capacity = capacity;
   a.list = chunks_of(free_count); a.high = chunks_of(pages - pages_after);
   a.requests = (int)requests; a.P = (int)page_size;
