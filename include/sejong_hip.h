@@ -845,14 +845,15 @@ int sj_token_logprobs_bwd(void *stream, const void *x, int dtype, long ldx, long
  * (ended[r] != 0, nullable: none; its logits are not read) the end_token alone,
  * total = score.  Per group the `keep` candidates of the highest rank, total /
  * length^length_power with length = lengths[r] + 1 (an ended beam's lengths[r];
- * 1 at least), the lowest beam * vocab + token first among equals, are written
- * in their order to [groups][keep]: parents (the row; what sj_paged_fork
- * takes), tokens, scores_after = total, lengths_after (nullable) = lengths + 1
- * (an ended beam's lengths), ended_after (nullable) 1 where the beam had ended
- * or the token is end_token (-1: no token is), else 0.  Sums, totals and ranks
- * are formed in 64 bits; among a beam's own tokens the logits decide.  A logit
- * of -inf is no candidate, nor any of a beam whose score or whose row's sum is
- * not finite (a first step has one live beam, the others' scores -inf).
+ * 1 at least) are written in their order to [groups][keep]; among equal ranks
+ * the lowest beam is first, of a beam's own tokens the one of the larger logit,
+ * then the lowest: parents (the row; what sj_paged_fork takes), tokens,
+ * scores_after = total, lengths_after (nullable) = lengths + 1 (an ended beam's
+ * lengths), ended_after (nullable) 1 where the beam had ended or the token is
+ * end_token (-1: no token is), else 0.  Sums, totals and ranks are formed in 64
+ * bits; where they leave the same rank of a beam's tokens the logits decide.  A
+ * logit of -inf is no candidate, nor any of a beam whose score or whose row's
+ * sum is not finite (a first step has one live beam, the others' scores -inf).
  * Places without a candidate get parent and token -1, score -inf, length 0 and
  * 1 in ended_after.  lengths is nullable where length_power is 0 and
  * lengths_after null.  length_power 0 .. 16; beams and keep at most SJ_BEAM_MAX; vocab

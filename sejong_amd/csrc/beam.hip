@@ -7,7 +7,8 @@
 //
 // Totals of different beams may lie next to each other, and which is the larger
 // decides what the search goes on with: sums, totals and ranks are 64 bits.
-// Within a beam the order is that of its logits, which are exact.
+// Within a beam the order is that of its logits, which are exact: where 64 bits
+// leave the same total of them (a score of -1e30 all of it), they decide.
 //
 // What bounds it.  A prompt's step is two dependent halves, its rows and then
 // all of its beams, and each ends with reductions of one workgroup: 64 prompts of
@@ -247,9 +248,7 @@ struct GroupShared {
   double base[64], factor[64], score[64];  // the beam's L, length^power
   int live[64];                            // 0: no candidate, 1: its tokens, 2: ended
   int order[64];                           // the beams of the second, then of the third
-  u64 cand[CAP];
-  int32_t where[CAP];
-  double total[CAP];
+  u64 cand[CAP], tie[CAP];                 // ranks' keys, and the order among equals
   __attribute__((aligned(16))) u64 best[256];
   u64 last[4];
   uint16_t pick[CAP];
@@ -259,11 +258,18 @@ struct GroupShared {
 struct Near {
   u64 sums[2 * NEAR], keys[4 * NEAR];
 };
+// tie: its place among those of the same rank, the largest first: the lowest beam
+// (6 bits from 56), the largest logit (32 from 24), the lowest token (24)
 struct Candidate {
   u64 key;  // 0: none
-  int flat;
-  double total;
+  u64 tie;
 };
+__device__ __forceinline__ u64 tie_of(int beam, u64 key) {  // key: the list's
+  return (u64)(63 - beam) << 56 | (key >> 32) << 24 | (key & 0xffffffu);
+}
+__device__ __forceinline__ int tie_beam(u64 tie) { return 63 - (int)(tie >> 56); }
+__device__ __forceinline__ float tie_value(u64 tie) { return key_value(tie << 8); }
+__device__ __forceinline__ int tie_token(u64 tie) { return 0xffffff - (int)(tie & 0xffffffu); }
 
 // of a wave's columns, among the n in LDS, the least of those with fewer than keep
 // larger ones (equal columns have one place)
@@ -364,21 +370,21 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
   // their lists: one for each slice of an open beam, one of one entry of an ended one
   const int open = beams_open * S, closed = __popcll(done), some_lists = open + closed;
   auto candidate = [&](int list, int place) {
-    Candidate c = {0, 0, 0.0};
+    Candidate c = {0, 0};
     const bool ended = list >= open;
     const int nth = ended ? list - open + beams_open : list / S, b = in_order ? nth : sh.order[nth];
-    c.total = sh.score[b];
+    double total = sh.score[b];
     if (ended) {
       if (place) return c;
-      c.flat = b * a.V + max(a.end_token, 0);
+      c.tie = tie_of(b, order_key(0.f, max(a.end_token, 0)));
     } else {
       const u64 key = key_at(place * lists + b * S + list - nth * S);
       const float x = key_value(key);
       if (key == 0 || x == -INFINITY) return c;
-      c.total += (double)x - sh.base[b];
-      c.flat = b * a.V + key_index(key);
+      total += (double)x - sh.base[b];
+      c.tie = tie_of(b, key);
     }
-    c.key = rank_key(a.power == 0.0 ? c.total : c.total / sh.factor[b]);
+    c.key = rank_key(a.power == 0.0 ? total : total / sh.factor[b]);
     return c;
   };
   // Each list is in order: `each` threads go down every each-th entry of it, and
@@ -432,14 +438,15 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
       const Candidate q = candidate(list, place);
       if (q.key < T0) break;
       const int n = atomicAdd(&sh.n, 1);
-      if (n < CAP) sh.cand[n] = q.key, sh.where[n] = q.flat, sh.total[n] = q.total;
+      if (n < CAP) sh.cand[n] = q.key, sh.tie[n] = q.tie;
     }
   __syncthreads();
-  auto write = [&](int place, bool some, int flat, double total) {
+  auto write = [&](int place, bool some, u64 tie) {
     const long at = (long)g * keep + place;
-    const int b = some ? flat / a.V : 0, token = flat - b * a.V;
+    const int b = some ? tie_beam(tie) : 0, token = tie_token(tie);
     const long row = row0 + b;
     const bool was = some && sh.live[b] == 2;
+    const double total = sh.score[b] + (was ? 0.0 : (double)tie_value(tie) - sh.base[b]);
     a.parents[at] = some ? (int)row : -1;
     a.tokens[at] = !some ? -1 : was ? a.end_token : token;
     a.scores_after[at] = some ? (float)total : -INFINITY;
@@ -469,8 +476,7 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
     }
     for (int q = t >> 2; q < m; q += 64) {
       const int i = n > 192 ? sh.pick[q] : q;
-      const u64 key = sh.cand[i];
-      const int flat = sh.where[i];
+      const u64 key = sh.cand[i], tie = sh.tie[i];
       uint32_t place = 0, same = 0;
 #pragma unroll 4
       for (int j = t & 3; j < n; j += 4) {
@@ -479,40 +485,36 @@ __device__ __forceinline__ void group_best(const BeamArgs& a, int g, GroupShared
         same += other == key;
       }
       if (same > (uint32_t)((i & 3) == (t & 3)))  // another of the same rank
-        for (int j = t & 3; j < n; j += 4) place += sh.cand[j] == key && sh.where[j] < flat;
+        for (int j = t & 3; j < n; j += 4) place += sh.cand[j] == key && sh.tie[j] > tie;
       place += dpp<0xB1>(place);
       place += dpp<0x4E>(place);
-      if ((t & 3) == 0 && (int)place < keep) write((int)place, true, flat, sh.total[i]);
+      if ((t & 3) == 0 && (int)place < keep) write((int)place, true, tie);
     }
-    for (int i = n + t; i < keep; i += 256) write(i, false, 0, 0.0);
+    for (int i = n + t; i < keep; i += 256) write(i, false, 0);
     return;
   }
   // more of the same rank than LDS holds: the first behind the last, keep times
-  u64 last = ~0ull;
-  int last_flat = -1;
+  u64 last = ~0ull, last_tie = 0;
   for (int j = 0; j < keep; j++) {
-    Candidate top = {0, 0x7fffffff, 0.0};
+    Candidate top = {0, 0};
     for (int i = t; i < some_lists * k; i += 256) {
       const Candidate q = candidate(i % per, i / per);
-      const bool behind = q.key && (q.key < last || (q.key == last && q.flat > last_flat));
-      if (behind && (q.key > top.key || (q.key == top.key && q.flat < top.flat))) top = q;
+      const bool behind = q.key && (q.key < last || (q.key == last && q.tie < last_tie));
+      if (behind && (q.key > top.key || (q.key == top.key && q.tie > top.tie))) top = q;
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
-      const u64 key = __shfl_xor(top.key, d, 64);
-      const int flat = __shfl_xor(top.flat, d, 64);
-      const double total = __shfl_xor(top.total, d, 64);
-      if (key > top.key || (key == top.key && flat < top.flat)) top = Candidate{key, flat, total};
+      const u64 key = __shfl_xor(top.key, d, 64), tie = __shfl_xor(top.tie, d, 64);
+      if (key > top.key || (key == top.key && tie > top.tie)) top = Candidate{key, tie};
     }
     __syncthreads();
-    if (lane == 0) sh.cand[w] = top.key, sh.where[w] = top.flat, sh.total[w] = top.total;
+    if (lane == 0) sh.cand[w] = top.key, sh.tie[w] = top.tie;
     __syncthreads();
     for (int i = 0; i < 4; i++)
-      if (sh.cand[i] > top.key || (sh.cand[i] == top.key && sh.where[i] < top.flat))
-        top = Candidate{sh.cand[i], sh.where[i], sh.total[i]};
-    if (t == 0) write(j, top.key != 0, top.key ? top.flat : 0, top.total);
+      if (sh.cand[i] > top.key || (sh.cand[i] == top.key && sh.tie[i] > top.tie)) top = Candidate{sh.cand[i], sh.tie[i]};
+    if (t == 0) write(j, top.key != 0, top.tie);
     last = top.key;
-    last_flat = top.flat;
+    last_tie = top.tie;
   }
 }
 
