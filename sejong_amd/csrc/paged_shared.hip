@@ -519,7 +519,9 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
     // a wave's own columns, straight from its registers
     auto put = [&](const auto& wk) {
       typedef std::remove_cv_t<std::remove_reference_t<decltype(wk)>> K;
-      part += (4 * cb + w) * s.lead_slot;
+      // 64 bits: a group's slots pass 2^31 floats at 8.3 M columns of 256; the same for the
+      // whole wave, as a vector product cost 64 rows over 16384 keys 1.5 us
+      part += (long)__builtin_amdgcn_readfirstlane(4 * cb + w) * s.lead_slot;
 #pragma unroll
       for (int ct = 0; ct < CT; ct++) {
         const int c = 16 * ct + (lane & 15);
@@ -554,7 +556,7 @@ __global__ __launch_bounds__(256, per_cu<T>(DC)) void k_shared_walks(SharedArgs 
       WL wk;
       begin(wk);
       wk.run(a, pages, kh, 0, keys, 4 * c0 + w, min(4 * c1, tiles), 4, tile, lane, nt);
-      part += cb * s.lead_slot;
+      part += (long)cb * s.lead_slot;
 #pragma unroll
       for (int ct = 0; ct < CT; ct++) {
         if (ct >= nt) break;
