@@ -1,5 +1,6 @@
-// How a pool's pages and its free list are dealt out to workgroups, and where
-// their counts lie in the workspace.  Host code alone, no HIP.
+// How a pool's pages and its free list are dealt out to workgroups, where their
+// counts lie in the workspace, and what rows of a page are copied as.  Host code
+// alone, no HIP.
 #pragma once
 #include <stddef.h>
 
@@ -37,6 +38,16 @@ inline CompactSpace compact_space(long pages, long free_count) {
   s.moves = s.below + (size_t)chunks_of(free_count).count;
   s.all = s.moves + (size_t)chunks_most(pages);
   return s;
+}
+
+// A row of `width` elements of `size` bytes: 16-byte units, and elements behind
+// them.  Rows may be longer than 2^31 bytes.
+struct RowUnits {
+  int units, tail;
+};
+inline RowUnits row_units(long width, long size) {
+  const long units = width * size / 16;
+  return {(int)units, (int)(width - units * (16 / size))};
 }
 
 }  // namespace sj

@@ -650,7 +650,7 @@ __global__ __launch_bounds__(256) void k_paged_copy(CopyArgs a) {
       if (u0 + 256 * j < all) ((Raw16*)(y + at[j]))->v = v[j];
   }
   for (long e = t; e < (long)n * a.tail; e += 256) {
-    const long r = e / a.tail, at = r * a.row + 16 * a.units + (e - r * a.tail) * (long)sizeof(T);
+    const long r = e / a.tail, at = r * a.row + 16L * a.units + (e - r * a.tail) * (long)sizeof(T);
     *(T*)(y + at) = *(const T*)(x + at);
   }
 }
@@ -798,7 +798,8 @@ extern "C" int sj_paged_copy(void* stream, void* k_cache, void* v_cache, long ld
   a.k = (uint8_t*)k_cache; a.v = (uint8_t*)v_cache; a.copies = copies;
   a.row = ldkv * size; a.layer = layer_stride * size;
   a.layers = (int)layers; a.pages = (int)pages; a.P = (int)page_size;
-  a.units = (int)(width * size / 16); a.tail = (int)(width - a.units * 16 / size);
+  const RowUnits row = row_units(width, size);
+  a.units = row.units; a.tail = row.tail;
   a.d_units = make_div((uint32_t)(a.units ? a.units : 1));
   a.d_layers = make_div((uint32_t)layers);
   const unsigned blocks = (unsigned)(2 * count * layers);

@@ -1,6 +1,6 @@
-"""How pages are dealt out to workgroups and where their counts lie (csrc/chunks.h,
-which needs no HIP), compiled here as host code; and the workspace queries that go
-by it."""
+"""How pages are dealt out to workgroups, where their counts lie, and what rows are
+copied as (csrc/chunks.h, which needs no HIP), compiled here as host code that
+traps on a signed overflow; and the workspace queries that go by it."""
 import os
 import subprocess
 
@@ -16,8 +16,16 @@ PROGRAM = r"""
 #include <cstdio>
 #include "chunks.h"
 
-int main() {
+int main(int argc, char**) {
   long pages, after, listed;
+  if (argc > 1) {
+    long width, size;
+    while (scanf("%ld %ld", &width, &size) == 2) {
+      const sj::RowUnits r = sj::row_units(width, size);
+      printf("%d %d\n", r.units, r.tail);
+    }
+    return 0;
+  }
   while (scanf("%ld %ld %ld", &pages, &after, &listed) == 3) {
     const sj::Chunks high = sj::chunks_of(pages - after), list = sj::chunks_of(listed);
     const sj::CompactSpace s = sj::compact_space(pages, listed);
@@ -67,3 +75,13 @@ def test_a_larger_pool_needs_no_less():
             if high <= pages:
                 moves = -(-high // (-(-high // EDGE) * ROUND))  # workgroups that count the high pages
                 assert lib.sj_paged_compact_workspace_bytes(pages, 0) >= 4 * (pages + moves)
+
+
+def test_units_of_rows_of_any_length(program):
+    """Rows of 2^31 bytes and more too: the units and the elements behind them are the row."""
+    cases = [(w, size) for size in (2, 4) for w in list(range(1, 40)) + [k * 2 ** 29 + d for k in (1, 2, 3) for d in range(-9, 10)]
+             + [2 ** 31 - 1 - d for d in range(9)]]
+    out = subprocess.run([program, "rows"], input="".join("%d %d\n" % c for c in cases), check=True, capture_output=True,
+                         text=True, timeout=60).stdout.splitlines()
+    for (width, size), line in zip(cases, out, strict=True):
+        assert line.split() == [str(width * size // 16), str(width * size % 16 // size)], (width, size)
