@@ -610,15 +610,19 @@ __global__ __launch_bounds__(256) void k_compact_tables(CompactArgs a) {
 
 // ------------------------------------------------------------------- copy
 //
-// One workgroup per copy, layer and cache: reads and writes of 16 bytes, four
-// in flight a thread.  600 pages of 16 rows of 512 bf16 in 8 layers take 65.6 us,
+// One workgroup per copy, layer and cache, in launches of MOST_BLOCKS (a loop over
+// further ones in the kernel cost small calls a quarter of a microsecond): reads
+// and writes of 16 bytes, four in flight a thread.  600 pages of 16 rows of 512 bf16 in 8 layers take 65.6 us,
 // 4.8 TB/s read and written, the rate of a large copy; the filled parts of 64
 // pages 3.7 us, a launch and one round trip.
+
+constexpr long MOST_BLOCKS = 1L << 23;  // of 256 threads: a launch holds fewer than 2^32
 
 struct CopyArgs {
   uint8_t *k, *v;
   const int32_t* copies;
   long row, layer;  // bytes between rows and layers
+  uint32_t first;  // of the launch, among copies, layers and caches
   int layers, pages, P, units, tail;  // 16-byte units of a row, its elements behind them
   Div d_units, d_layers;
 };
@@ -628,10 +632,11 @@ struct __attribute__((packed, aligned(2))) Raw16 {
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_paged_copy(CopyArgs a) {
-  const int t = threadIdx.x, item = blockIdx.x >> 1, i = div(item, a.d_layers), layer = item - i * a.layers;
+  const uint32_t part = a.first + blockIdx.x;
+  const int t = threadIdx.x, item = (int)(part >> 1), i = div(item, a.d_layers), layer = item - i * a.layers;
   const int from = a.copies[3 * (long)i], to = a.copies[3 * (long)i + 1], n = min(a.copies[3 * (long)i + 2], a.P);
   if (from < 0 || from >= a.pages || to < 0 || to >= a.pages || from == to || n <= 0) return;
-  uint8_t* base = (blockIdx.x & 1 ? a.v : a.k) + layer * a.layer;
+  uint8_t* base = (part & 1 ? a.v : a.k) + layer * a.layer;
   const uint8_t* x = base + (long)from * a.P * a.row;
   uint8_t* y = base + (long)to * a.P * a.row;
   const long all = (long)n * a.units;
@@ -802,12 +807,16 @@ extern "C" int sj_paged_copy(void* stream, void* k_cache, void* v_cache, long ld
   a.units = row.units; a.tail = row.tail;
   a.d_units = make_div((uint32_t)(a.units ? a.units : 1));
   a.d_layers = make_div((uint32_t)layers);
-  const unsigned blocks = (unsigned)(2 * count * layers);
+  const long parts = 2 * count * layers;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == SJ_BF16)
-    k_paged_copy<bf16_t><<<blocks, 256, 0, s>>>(a);
-  else
-    k_paged_copy<float><<<blocks, 256, 0, s>>>(a);
-  SJ_LAUNCH_CHECK("paged copy");
+  for (long first = 0; first < parts; first += MOST_BLOCKS) {
+    a.first = (uint32_t)first;
+    const unsigned blocks = (unsigned)(parts - first < MOST_BLOCKS ? parts - first : MOST_BLOCKS);
+    if (dtype == SJ_BF16)
+      k_paged_copy<bf16_t><<<blocks, 256, 0, s>>>(a);
+    else
+      k_paged_copy<float><<<blocks, 256, 0, s>>>(a);
+    SJ_LAUNCH_CHECK("paged copy");
+  }
   return SJ_OK;
 }

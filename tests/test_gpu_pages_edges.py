@@ -4,6 +4,7 @@ import ctypes
 import numpy as np
 import pytest
 
+from tests import beam_util as BU
 from tests import gpu_util as G
 from tests import paged_util as PU
 from tests.test_gpu_pages import native
@@ -40,3 +41,23 @@ def test_copy_of_rows_past_32_bits(dtype, width):
     N.api.sj_download(ctypes.c_void_p(back.ctypes.data), K.at(ld + width - 40), back.nbytes)
     np.testing.assert_array_equal(back[:40], parts[-1])
     assert (back[40:] == 77).all()
+
+
+@pytest.mark.parametrize("count,layers", [(2 ** 22 - 1, 1), (2 ** 22 + 1, 1), (2 ** 23 + 5, 3), (2 ** 24, 1), (260_000, 40)])
+def test_copies_of_long_lists(count, layers):
+    """Lists with more places than one launch has workgroups for, few of them taken: the first, the last, some between."""
+    rng = np.random.default_rng(count)
+    N = native()[0]
+    P, width, taken = 2, 8, 40
+    pages = 2 * taken
+    copies = np.tile([-1, -1, 0], (count, 1)).astype(np.int32)
+    at = np.unique(np.concatenate([[0, count - 1], rng.integers(0, count, taken - 2)]))
+    names = rng.permutation(pages)
+    copies[at] = np.stack([names[:len(at)], names[taken:taken + len(at)], 1 + np.arange(len(at)) % P], 1)
+    kv = [G.rnd((layers, pages * P, width), "bf16", rng) for _ in range(2)]
+    K, V = (G.dev(x.ravel(), "bf16") for x in kv)
+    C = PU.ints(copies)
+    N.api.sj_paged_copy(None, K.p, V.p, width, 4, layers, pages * P * width, pages, P, width, C.p, count)
+    for x, d in zip(kv, (K, V)):
+        want = BU.copy(x.copy(), copies[at], P, width)
+        np.testing.assert_array_equal(d.host(), want.ravel())
