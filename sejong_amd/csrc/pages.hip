@@ -14,6 +14,7 @@ namespace {
 
 constexpr int NT = 256, PER = 4, ROUND = NT * PER;  // a round: four consecutive entries a thread
 static_assert(ROUND == CHUNK_ROUND, "a chunk is whole rounds");
+constexpr long MOST_BLOCKS = 1L << 23;  // of 256 threads: a launch holds fewer than 2^32
 constexpr int ALONE = 16384;  // entries, at most, that one workgroup takes by itself: 16 a thread
 constexpr int COMPACT_ALONE = 8192;  // of a compaction (8192 pages 13.8 us, 16.6 in five launches; 16384 18.9 and 16.8)
 
@@ -594,9 +595,9 @@ __global__ __launch_bounds__(1024) void k_compact_alone(CompactArgs a) {
 #pragma unroll
   for (int j = 0; j < N / 4; j++) move_pages(a, 4096 * j + 4 * t, (moving >> (4 * j)) & 15u, targets, before[j], status);
 }
-__global__ __launch_bounds__(256) void k_compact_tables(CompactArgs a) {
+__global__ __launch_bounds__(256) void k_compact_tables(CompactArgs a, long first) {
   const bool good = a.summary[2] == 0;
-  const long r = blockIdx.x;
+  const long r = first + blockIdx.x;
   const int n = max(a.lengths[r], 0), full = div(n, a.d_page), cols = full + (full * a.P != n);
   for (long c = threadIdx.x; c < a.ldt; c += 256) {
     int p = a.table[r * a.ldt + c];
@@ -615,8 +616,6 @@ __global__ __launch_bounds__(256) void k_compact_tables(CompactArgs a) {
 // and writes of 16 bytes, four in flight a thread.  600 pages of 16 rows of 512 bf16 in 8 layers take 65.6 us,
 // 4.8 TB/s read and written, the rate of a large copy; the filled parts of 64
 // pages 3.7 us, a launch and one round trip.
-
-constexpr long MOST_BLOCKS = 1L << 23;  // of 256 threads: a launch holds fewer than 2^32
 
 struct CopyArgs {
   uint8_t *k, *v;
@@ -782,7 +781,8 @@ extern "C" int sj_paged_compact(void* stream, const int32_t* table, long ldt, co
     if (both) k_compact_rank<<<both, NT, 0, s>>>(a);
     k_compact_moves<<<both ? both : 1, NT, 0, s>>>(a);
   }
-  if (requests) k_compact_tables<<<(unsigned)requests, 256, 0, s>>>(a);
+  for (long first = 0; first < requests; first += MOST_BLOCKS)
+    k_compact_tables<<<(unsigned)(requests - first < MOST_BLOCKS ? requests - first : MOST_BLOCKS), 256, 0, s>>>(a, first);
   SJ_LAUNCH_CHECK("paged compact");
   return SJ_OK;
 }

@@ -61,3 +61,31 @@ def test_copies_of_long_lists(count, layers):
     for x, d in zip(kv, (K, V)):
         want = BU.copy(x.copy(), copies[at], P, width)
         np.testing.assert_array_equal(d.host(), want.ravel())
+
+
+@pytest.mark.parametrize("requests", [2 ** 23 + 3, 2 ** 24])
+def test_compaction_of_many_requests(requests):
+    """As many requests as one launch has workgroups for, and as many as there can be: rows of one page that many share."""
+    rng = np.random.default_rng(requests)
+    N, lib = native()
+    P, pages, after, used = 4, 300, 200, 150
+    names = rng.permutation(pages)
+    table = names[rng.integers(0, used, requests)].astype(np.int32)
+    lengths = rng.integers(0, P + 1, requests).astype(np.int32)
+    free = np.concatenate([np.full(used, -1), names[used:]]).astype(np.int32)
+    below = free[used:][free[used:] < after]
+    moved = np.setdiff1d(np.arange(after, pages), free[used:])
+    to = np.arange(pages)
+    to[moved] = below[:len(moved)]
+    ins = [PU.ints(x) for x in (table, lengths, np.zeros(pages), free, [used])]
+    out = PU.ints(np.full(requests + 1, 55))
+    shared, listed, copies, summary = (PU.ints(np.full(n, 55)) for n in (pages, pages, 3 * 100, 4))
+    need = lib.sj_paged_compact_workspace_bytes(pages, pages)
+    ws = G.Dev(need, "u8")
+    T, L, S, F, H = (b.p for b in ins)
+    N.api.sj_paged_compact(None, T, 1, L, requests, P, pages, after, S, F, pages, H, out.p, shared.p, listed.p, copies.p, 100,
+                           summary.p, ws.p, need)
+    assert summary.host().tolist() == [len(moved), pages - len(below) + len(moved), 0, len(below) - len(moved)]
+    got = out.host()
+    assert got[-1] == 55
+    np.testing.assert_array_equal(got[:-1], np.where(lengths > 0, to[table], -1))
