@@ -626,7 +626,8 @@ extern "C" int sj_beam_select(void* stream, const void* x, int dtype, long ldx, 
   SJ_REQUIRE(groups >= 0 && groups <= 1L << 24 && beams > 0 && beams <= SJ_BEAM_MAX && keep > 0 && keep <= SJ_BEAM_MAX &&
                  vocab > 0 && vocab <= 1L << 24 && ldx >= vocab,
              "beam selection: %ld prompts of %ld beams, %ld of %ld (stride %ld)", groups, beams, keep, vocab, ldx);
-  SJ_REQUIRE(groups * beams * slices_of(vocab) < 1L << 23, "beam selection: %ld rows of %ld", groups * beams, vocab);
+  // the most workgroups of a launch: more than MEETING slices are of 8192 entries or more
+  SJ_REQUIRE(groups * beams * ((vocab + 2 * SLICE - 1) / (2 * SLICE)) < 1L << 23, "beam selection: %ld rows of %ld", groups * beams, vocab);
   SJ_REQUIRE(end_token >= -1 && end_token < vocab, "beam selection: end token %d of %ld", end_token, vocab);
   SJ_REQUIRE(length_power >= 0.0 && length_power <= 16.0, "beam selection: length power %g", length_power);
   if (groups == 0) return SJ_OK;
