@@ -1,4 +1,5 @@
-"""Attention over shared prefixes at the largest sizes that it takes."""
+"""Attention over shared prefixes of prompts (many tokens a request), and at the
+largest sizes that it takes."""
 import ctypes
 
 import numpy as np
@@ -7,6 +8,7 @@ import pytest
 from tests import gpu_util as G
 from tests import paged_util as PU
 from tests.test_gpu_paged import HALF_ULP, native
+from tests.test_gpu_shared import Shared
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +49,28 @@ def test_columns_of_a_group_past_32_bits_of_the_workspace():
         tol = (2 * err[:, None] + 2.0 ** -15) * mag + np.abs(o) * HALF_ULP["bf16"] * 1.01 + 1e-38
         assert (np.abs(got - o) <= tol).all(), r
         assert (np.abs(lse - ls) <= err * 2 + 2.0 ** -21 * (1 + np.abs(ls))).all(), r
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("groups,per,hq,hk,D,P,window", [([(96, [40, 17, 33]), (50, [64])], 17, 6, 2, 64, 16, 0),
+                                                         ([(300, [128, 130])], 128, 4, 2, 64, 24, 0),
+                                                         ([(64, [70] * 4)], 64, 8, 2, 128, 16, 0),
+                                                         ([(1000, [200])], 200, 3, 1, 32, 7, 0),
+                                                         ([(96, [40, 50])], 33, 6, 2, 64, 16, 60),
+                                                         ([(96, [40, 50])], 33, 16, 1, 256, 16, 120)])
+def test_prompts_over_a_shared_prefix(dtype, groups, per, hq, hk, D, P, window):
+    """Requests with many tokens at once: every one sees the prefix and its request's tokens up to itself."""
+    a = Shared(per + D, dtype, hq, hk, D, P, groups, alone=[per, per + 9], per=per, pad=2, window=window)
+    a.upload().run().check()
+    first = a.O.host().copy(), a.L.host().copy()
+    for b in (a.O, a.L):
+        b.upload(np.full(b.n, 55.0))
+    a.run()
+    assert all((x == y.host()).all() for x, y in zip(first, (a.O, a.L)))  # every output again, the same bits
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_more_rows_of_prompts_than_are_walked_together(dtype):
+    """2048 rows in one group, and a few more, which attend alone."""
+    for per in (256, 257):
+        Shared(per, dtype, 2, 1, 32, 16, [(40, [per] * 8)], per=per).upload().run().check()

@@ -3,7 +3,10 @@ import numpy as np
 import pytest
 
 from tests import gpu_util as G
-from tests.test_gpu_pages import Compact
+from tests.test_gpu_beam import Select, logits
+from tests.test_gpu_pages import Compact, Fork, state
+from tests.test_gpu_paged import Attend
+from tests.test_gpu_shared import Shared
 
 pytestmark = pytest.mark.gpu
 GUARD = 16384
@@ -34,3 +37,37 @@ def test_compaction(pages, after):
     free = np.concatenate([np.full(R * cols, -1), names[R * cols:]])
     c = Compact(lengths, table, np.zeros(pages, int), free, R * cols, pages, P, after, 5000)
     assert Guarded(c).run()["status"] == 0
+
+
+@pytest.mark.parametrize("groups,beams,P,hi,spare", [(1, 1, 16, 40, 4), (16, 4, 16, 900, 200), (300, 8, 16, 200, 20000),
+                                                     (2000, 5, 16, 64, 12000), (2, 2, 16, 100, 4_194_305), (2, 2, 16, 100, 16400)])
+def test_fork(groups, beams, P, hi, spare):
+    rng = np.random.default_rng(groups)
+    lengths, table, shared, free, head, pages = state(rng, groups, beams, P, hi, spare)
+    parents = np.arange(groups)[:, None] * beams + rng.integers(0, beams, (groups, beams))
+    assert Guarded(Fork(parents.ravel(), lengths, table, shared, free, head, pages, P)).run()["status"] == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V,groups,beams,keep", [(1, 1, 1, 1), (3, 2, 5, 64), (257, 7, 4, 4), (1000, 2, 33, 64), (4096, 3, 3, 8),
+                                                 (4097, 1, 1, 1), (50001, 2, 4, 64), (8193, 70, 8, 5), (16385, 40, 8, 64)])
+def test_selection(dtype, V, groups, beams, keep):
+    rng = np.random.default_rng(V)
+    rows = groups * beams
+    Guarded(Select(logits(rng, rows, V, dtype), rng.normal(-20, 2, rows), beams, keep, dtype)).run()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("groups,alone,hq,hk,D,P", [([(40, [1, 2])], [], 2, 1, 8, 16), ([(200, [3] * 5)], [7], 6, 2, 64, 16),
+                                                    ([(9000, [1] * 40)], [], 8, 2, 64, 16), ([(300, [20] * 70)], [1], 8, 1, 256, 16),
+                                                    ([(100, [4] * 300)], [], 16, 2, 96, 16), ([(9, [1] * 8)] * 255, [5], 2, 2, 32, 4),
+                                                    ([(16, [1] * 2047)], [], 33, 1, 16, 16), ([(600, [2, 3])] * 60, [], 17, 1, 128, 24)])
+def test_shared_attention(dtype, groups, alone, hq, hk, D, P):
+    Guarded(Shared(len(groups) + D, dtype, hq, hk, D, P, groups, alone=alone).upload()).run()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lengths,hq,hk,D", [([20000], 6, 2, 64), ([9000, 3], 8, 8, 128), ([3000, 4000, 1], 2, 1, 32),
+                                             ([5000] * 5, 17, 1, 256), ([6000], 33, 1, 64)])
+def test_attention(dtype, lengths, hq, hk, D):
+    Guarded(Attend(D, dtype, hq, hk, D, 16, lengths).upload()).run()
