@@ -14,8 +14,9 @@ LIB_PATH = os.path.join(HERE, "libsejong_hip.so")
 SJ_F32, SJ_F64, SJ_F16, SJ_I32, SJ_BF16 = 0, 1, 2, 3, 4
 SJ_ROPE_INTERLEAVED, SJ_ROPE_HALF = 0, 1
 SJ_ROPE_SCALE_NONE, SJ_ROPE_SCALE_LINEAR, SJ_ROPE_SCALE_BASE, SJ_ROPE_SCALE_PARTS = 0, 1, 2, 3
-SJ_PLAN_NO_PAGES, SJ_PLAN_TABLE_WIDTH, SJ_PLAN_ROWS, SJ_PLAN_LENGTHS = 1, 2, 4, 8
+SJ_PLAN_NO_PAGES, SJ_PLAN_TABLE_WIDTH, SJ_PLAN_ROWS, SJ_PLAN_LENGTHS, SJ_FORK_LIST_FULL = 1, 2, 4, 8, 16
 SJ_LOGPROBS_MAX_TOP = 64
+SJ_BEAM_MAX = 64
 
 _P = ctypes.c_void_p
 _L = ctypes.c_long
