@@ -511,8 +511,9 @@ int sj_paged_copy(void *stream, void *k_cache, void *v_cache, long ldkv, int dty
  * whole prefix (its position, or a window), and where prefix[g] is 0 or less or
  * longer than the table; all rows do where group_starts or their starts
  * descend, and beyond 2048 rows, 256 groups, 2^31 - 1 key tiles, or in heads
- * of another width than multiples of 8.  Padded rows, bad pages, strides,
- * types and limits as there; o may be q.  Workspace:
+ * of another width than multiples of 8.  (Where a window is shorter than the
+ * prefixes sj_paged_attention is faster: they are walked for nothing.)  Padded
+ * rows, bad pages, strides, types and limits as there; o may be q.  Workspace:
  * sj_paged_attention_shared_workspace_bytes, 16-byte aligned, not cleared and
  * not kept; calls that share one must not overlap. */
 size_t sj_paged_attention_shared_workspace_bytes(long rows, long hq, long hk, long head_dim, long groups);
@@ -851,9 +852,10 @@ int sj_token_logprobs_bwd(void *stream, const void *x, int dtype, long ldx, long
  * scores_after = total, lengths_after (nullable) = lengths + 1 (an ended beam's
  * lengths), ended_after (nullable) 1 where the beam had ended or the token is
  * end_token (-1: no token is), else 0.  Sums, totals and ranks are formed in 64
- * bits; where they leave the same rank of a beam's tokens the logits decide.  A
- * logit of -inf is no candidate, nor any of a beam whose score or whose row's
- * sum is not finite (a first step has one live beam, the others' scores -inf).
+ * bits, from powers of e and of the lengths that are good to 2^-40; where they
+ * leave the same rank of a beam's tokens the logits decide.  A logit of -inf is
+ * no candidate, nor any of a beam whose score or whose row's sum is not finite
+ * (a first step has one live beam, the others' scores -inf).
  * Places without a candidate get parent and token -1, score -inf, length 0 and
  * 1 in ended_after.  lengths is nullable where length_power is 0 and
  * lengths_after null.  length_power 0 .. 16; beams and keep at most SJ_BEAM_MAX; vocab

@@ -30,10 +30,16 @@ namespace {
 // 3.3 for the lists, a walk's chain of page, keys and products, 4.5 for the join;
 // alone 10.5.  24 groups of 5 rows over up to 6000 keys (16/4 heads of 64, fp32) take 36.5 us,
 // 12 of them their 61 MB at a copy's rate: each wave waits for two or three tiles.
-// 64 rows over 16384 keys (32/8 heads of 128, bf16) take 56 us, where their 91 MB
-// are 18 and their products, P as two planes, 18: the lists 3, the shared walks
-// 37 (the multiplying waves' own instructions 21), own walks 6, the join of 34 MB
-// of parts 10.  One plane (54 us) would round P to 8 bits.
+// 64 rows over 16384 keys (32/8 heads of 128, bf16) take 60 us, where their 91 MB
+// are 18 and their products, P as two planes, 18: the walks' launch 50 (the lists
+// 3, the shared walks 37 to 41, the multiplying waves' own instructions 21 of them,
+// own walks 6), the join of 34 MB of parts 10.  One plane would round P to 8 bits,
+// and took 2 us less.
+//
+// A group's prefix is walked whether or not any row shares it: within a window
+// that begins behind position 0 no row does, and each walks its window alone (32
+// rows over 16384 keys, 32/8 heads of 128, a window of 1024 48 us, by
+// sj_paged_attention 23; of 8192 142 and 123).
 
 constexpr int CT = 2, COLS = 16 * CT, BLOCK = 4 * COLS;
 constexpr int WIDE_PLACE = 64;  // keys of a place of a walk whose waves go by columns
@@ -41,10 +47,11 @@ constexpr int MAX_ROWS = 2048, MAX_GROUPS = 256;  // what LDS lists beside two s
 constexpr int GROUPS_OF_WAVES = 512;  // workgroups, at most
 // Elements of keys and values that the rows read of as long sequences as the table
 // holds, if each reads its own: up to here they do (us, for the rows together and
-// alone: 4 rows over 960 keys, 2 KV heads of 64, 0.5 M, 14.8 and 10.5; 128 rows of
+// alone: 4 rows over 960 keys, 2 KV heads of 64, 1 M, 14.8 and 10.5; 128 rows of
 // that, 34 M, 17.3 and 12.5; 16 rows over 1024, 8 heads of 128, 42 M, 18.6 and
-// 23.2; 8 rows over 2048, 38 M, 21.4 and 23.0; fp32: 8 groups of 5 rows over up to
-// 2000 keys, 4 heads of 64, 47 M, 20.5 and 15.6, 24 over 1000, 70 M, 23.7 each).
+// 23.2; 8 rows over 2048, 38 M, 21.4 and 23.0).  One number for both types, though
+// fp32 would change later: 8 groups of 5 rows over up to 2000 keys, 4 heads of 64,
+// 47 M, 20.5 and 15.6; 24 over 1000, 70 M, 23.7 each.
 constexpr double FEW = 33554432.0;
 
 struct SharedArgs {
